@@ -62,7 +62,8 @@ def lib() -> ctypes.CDLL:
 # Number of native calls that launch at least one of this library's kernels (benchmarks read and
 # reset it to report how many launches a step takes).
 LAUNCHES = 0
-_LAUNCH_PREFIXES = ("mep_launch_", "mep_gemm_launch", "mep_router_", "mep_swiglu_", "mep_sgd_", "mep_ce_")
+_LAUNCH_PREFIXES = ("mep_launch_", "mep_gemm_launch", "mep_router_", "mep_swiglu_", "mep_sgd_", "mep_ce_",
+                    "mep_mx_quantize", "mep_mx_dequantize", "mep_mx_gemm_launch")
 
 
 def call(name: str, *args):

@@ -13,6 +13,7 @@
 //        Also large products with fp32 output.
 //   ep_dense_f32_kernel (dense_f32.cuh): one product with fp32 output (router logits).
 //   ep_weight_grad_kernel (weight_grad.cuh): weight grads, fp32 output or with the SGD step in the epilogue.
+//   ep_mx_gemm_kernel (mx_gemm.cuh): token-major products of microscaled 4-bit operands.
 // Group g < split reads/writes allocation 0 (local experts), g >= split allocation 1 (this
 // rank's prefetch / reduce slots): the [2*epn] compute view never has to be contiguous.
 // CTA pairs (template TWO, clusters of two CTAs, tcgen05 cta_group::2): the leader issues
@@ -144,7 +145,8 @@ __device__ __forceinline__ bool arrive_wait(const int32_t* ctr, int expect, int 
 
 // Rows of a group that hold tokens (its real rows if the padding ranges are known); at least one
 // for a group that is not empty.
-__device__ __forceinline__ int group_valid(const GemmKParams& p, int g, int start, int end) {
+template <class Params>
+__device__ __forceinline__ int group_valid(const Params& p, int g, int start, int end) {
   if (p.pads == nullptr || end <= start) return end - start;
   const int first = p.pads[2 * g], n = p.pads[2 * g + 1];
   return (n > 0 && first >= start && first < end) ? max(1, first - start) : end - start;
@@ -155,6 +157,7 @@ __device__ __forceinline__ int group_valid(const GemmKParams& p, int g, int star
 #include "device/dense_f32.cuh"
 #include "device/token_gemm.cuh"
 #include "device/weight_grad.cuh"
+#include "device/mx_gemm.cuh"
 
 namespace mep {
 
@@ -198,6 +201,19 @@ struct GemmDesc {
   int32_t rows_used;               // weight grad: rows that hold tokens, on the host's knowledge (0: total_rows)
 };
 
+// Product of microscaled 4-bit operands: tokens [rows][K], weights [ngroups][w_rows][K] (`gated`: gate and up packed).
+struct MxDesc {
+  const void *a_codes, *a_scales, *w_codes, *w_scales;
+  int32_t rows, K, ngroups, w_rows, N, gated;
+  const int32_t* cu_seqlens;
+  const int32_t* pads;
+  const float* row_scale;
+  void *out, *gate, *up, *codes, *scales;                // codes, scales: the activation, quantised along its columns
+  int64_t ldc;
+  int32_t* status;
+  int64_t timeout_ns;
+};
+
 typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                              CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
@@ -224,6 +240,25 @@ static int make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols
   return 0;
 }
 
+// 2-D tensor [rows][cols] of bytes in 128-byte boxes with the 128-byte swizzle, or [rows][cols / 4] words in boxes of 256
+// words x 1 row, unswizzled.
+static int make_byte_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int box_rows) {
+  EncodeFn enc = (EncodeFn)driver_tensor_map_encode();
+  if (!enc) return fail(-10, "CUDA driver entry cuTensorMapEncodeTiled not available");
+  if (((uintptr_t)base & 15) != 0 || cols % 16 != 0) return fail(-11, "mx operands must be 16-byte aligned");
+  const bool words = box_rows == 0;
+  cuuint64_t dims[2] = {(cuuint64_t)(words ? cols / 4 : cols), (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)cols};
+  cuuint32_t box[2] = {words ? 256u : 128u, words ? 1u : (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(m, words ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims,
+                   strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   words ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(-12, "cuTensorMapEncodeTiled failed with code %d", (int)r);
+  return 0;
+}
+
 // Fused dispatch launches: CTAs of different ranks wait for one another's copy warps, so the whole
 // grid must be resident at once.  The grid never exceeds what the device holds next to the weight
 // ops' CTAs, and a cooperative launch makes the driver guarantee the residency; MOONEP_B200_FD_COOP=0
@@ -243,7 +278,8 @@ struct PairLaunch {
   std::atomic<unsigned long long> raised{0};
   std::atomic<int> max_clusters{-1};
 };
-static int launch_pair(const void* kern, PairLaunch& once, GemmKParams kp, int grid, int threads, int smem, bool coop,
+template <class Params>
+static int launch_pair(const void* kern, PairLaunch& once, const Params& kp, int grid, int threads, int smem, bool coop,
                        cudaStream_t stream) {
   MEP_CUDA_OK(raise_smem_limit(kern, once.raised));
   cudaLaunchConfig_t cfg;
@@ -354,6 +390,12 @@ static int launch_dense_f32(const DenseParams& dp, cudaStream_t stream) {
   void* args[] = {(void*)&dp};
   MEP_CUDA_OK(cudaLaunchKernel(kern, grid, dim3(DN_THREADS), args, smem, stream));
   return 0;
+}
+
+template <int EPI>
+static int launch_mx(const MxParams& p, int grid, cudaStream_t stream) {
+  static PairLaunch once;
+  return launch_pair((const void*)ep_mx_gemm_kernel<EPI>, once, p, grid, MXG_THREADS, MXG_SMEM, false, stream);
 }
 
 template <bool A_MN, int EPI, bool DISP>
@@ -552,6 +594,39 @@ int mep_gemm_launch(const GemmDesc* d, cudaStream_t stream) {
                    : launch_token<false, EPI_PUSH, false>(kp, two, grid, stream);
   }
   return fail(-7, "gemm: unknown epilogue %d", d->epi);
+}
+
+int mep_mx_desc_bytes() { return (int)sizeof(MxDesc); }
+
+int mep_mx_gemm_launch(const MxDesc* d, cudaStream_t stream) {
+  if (d->ngroups < 1 || d->ngroups > MAX_GROUPS) return fail(-1, "mx product: ngroups=%d out of range", d->ngroups);
+  if (d->rows < 0 || d->K < 1 || d->N < 1 || d->w_rows < 1) return fail(-2, "mx product: %d x %d x %d", d->rows, d->K, d->N);
+  if (d->rows == 0) return 0;
+  MxParams p;
+  std::memset(&p, 0, sizeof(p));
+  const int64_t k_bytes = (int64_t)((d->K + MX_BLOCK - 1) / MX_BLOCK) * (MX_BLOCK / 2);
+  const int64_t s_bytes = (int64_t)mx_atoms(d->K) * MX_ATOM_BYTES;
+  p.w_rows = d->w_rows; p.w_atoms = mx_atoms(d->w_rows); p.t_atoms = mx_atoms(d->rows);
+  int rc = 0;
+  if ((rc = make_byte_map(&p.w, d->w_codes, (int64_t)d->ngroups * d->w_rows, k_bytes, 128))) return rc;
+  if ((rc = make_byte_map(&p.ws, d->w_scales, (int64_t)d->ngroups * p.w_atoms, s_bytes, 0))) return rc;
+  for (int b = 0; b < 4; ++b)
+    if ((rc = make_byte_map(&p.tok[b], d->a_codes, d->rows, k_bytes, b < 3 ? 32 * (b + 1) : MXG_MAX_N / 2))) return rc;
+  if ((rc = make_byte_map(&p.ts, d->a_scales, (int64_t)MX_PHASES * p.t_atoms, s_bytes, 0))) return rc;
+  p.cu_seqlens = d->cu_seqlens; p.pads = d->pads; p.ngroups = d->ngroups; p.total_rows = d->rows; p.K = d->K; p.N = d->N;
+  p.out = (__nv_bfloat16*)d->out; p.gate = (__nv_bfloat16*)d->gate; p.up = (__nv_bfloat16*)d->up;
+  p.codes = (uint8_t*)d->codes; p.scales = (uint8_t*)d->scales;
+  p.code_bytes = (d->N + MX_BLOCK - 1) / MX_BLOCK * (MX_BLOCK / 2); p.k_atoms = mx_atoms(d->N);
+  p.out_atoms = mx_atoms(d->rows);
+  p.vec_out = d->ldc % 8 == 0 && (((uintptr_t)d->out | (uintptr_t)d->gate | (uintptr_t)d->up) & 15) == 0;
+  p.row_scale = d->row_scale; p.ldc = d->ldc; p.status = d->status;
+  p.timeout_ns = (unsigned long long)(d->timeout_ns > 0 ? d->timeout_ns : 2000000000ll);
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (!d->gated) return launch_mx<MX_EPI_BF16>(p, sms, stream);
+  return p.gate != nullptr || p.up != nullptr ? launch_mx<MX_EPI_SWIGLU_SAVE>(p, sms, stream)
+                                              : launch_mx<MX_EPI_SWIGLU>(p, sms, stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,449 @@
+// Grouped product of microscaled 4-bit operands (mx_format.cuh) on the tensor cores' block-scaled form,
+// tcgen05.mma.kind::mxf4.block_scale: C[rows of g] = A[rows of g] * W[g]^T, fp32 sums, computed as C^T = W[g] * A^T
+// like ep_token_gemm_kernel (token_gemm.cuh): the weights' rows take the fixed M side (256 a CTA pair), the tokens N.
+//
+// In bytes a tile is what it is there: a k-step of the MMA reads 32 bytes of an operand row (64 elements instead of
+// 16 of bf16) and takes as long, so a stage of 128 bytes a row feeds four MMAs and the same ring carries four times the
+// operations.  What is new are the scales.  They lie in memory in the atoms that tensor memory takes (128 rows x 4
+// blocks), come with their stage by TMA, and tcgen05.cp puts them into tensor memory in front of the stage's MMAs; both
+// run in the tensor core's order, and two sets of columns are used in turn.  In a pair either CTA has the scales of its
+// own 128 weight rows and those of all tokens.
+//
+// Tensor memory: two accumulators of 224 columns and two sets of 24 for scales.  (256 tokens a tile would leave no
+// room for scales beside a second accumulator.)
+// Token tiles start at multiples of 32 rows of the whole tensor, whatever row a group starts at: then a tile's scales
+// are whole atoms of one of their four phases.  Rows of a neighbouring group in a tile are computed and not stored.
+//
+//   warp 0  TMA producer
+//   warp 1  MMA issuer
+//   warps 2..5, 6..9 epilogue, two sets of four, as in ep_token_gemm_kernel
+//
+// SwiGLU: gate and up columns come packed in turns of 16 rows, so that a warp's 32 rows of tensor memory hold both of 16
+// activations: read as two fragments of 16 rows, gate and up of an element meet in one thread's registers, in fp32.
+// The activation is rounded to bf16 and, if it is the next product's operand, quantised while it is in shared memory.
+#pragma once
+
+#include "device/mx_format.cuh"
+
+namespace mep {
+
+enum { MX_EPI_BF16 = 0, MX_EPI_SWIGLU = 1, MX_EPI_SWIGLU_SAVE = 2 };
+
+constexpr int MXG_MAX_N = 224;                   // tokens of a tile
+constexpr int MXG_BK = 256;                      // elements of a k-block: 128 bytes a row
+constexpr int MXG_STAGES = 5;
+constexpr int MXG_W_BYTES = 128 * 128;
+constexpr int MXG_T_BYTES = MXG_MAX_N / 2 * 128;
+constexpr int MXG_S_BYTES = 2 * MX_ATOM_BYTES;   // scales of 128 rows and one k-block
+constexpr int MXG_STAGE = MXG_W_BYTES + MXG_T_BYTES + MXG_S_BYTES * 3;
+constexpr int MXG_SETS = 2;
+constexpr int MXG_THREADS = 64 + MXG_SETS * 128;
+constexpr int MXG_SMEM = MXG_STAGES * MXG_STAGE + 1024;
+constexpr uint32_t MXG_SCALES_AT = 2 * MXG_MAX_N;
+constexpr uint32_t MXG_SCALE_COLS = 24;             // columns of tensor memory of a set: 8 of weights, 16 of tokens
+static_assert(MXG_SCALES_AT + 2 * MXG_SCALE_COLS <= 512, "tensor memory");
+static_assert(MXG_STAGE % 1024 == 0 && MXG_T_BYTES % 1024 == 0, "swizzle atoms");
+
+struct MxParams {
+  CUtensorMap w, ws;               // weights' codes, 128-byte x 128-row boxes; scales, two atoms a box
+  CUtensorMap tok[4], ts;          // token rows in boxes of 32, 64, 96, 112 rows; scales
+  const int32_t* cu_seqlens;
+  const int32_t* pads;
+  int ngroups, total_rows, K;
+  int w_rows, w_atoms;             // rows and row atoms of a group's weights
+  int t_atoms;                     // row atoms of a phase of the tokens' scales
+  int N;                           // output columns
+  __nv_bfloat16* out;              // y or act, or null
+  __nv_bfloat16 *gate, *up;
+  uint8_t *codes, *scales;         // act quantised, or null (scales at four phases, out_atoms row atoms each)
+  int code_bytes, k_atoms, out_atoms;      // of act
+  int vec_out;
+  const float* row_scale;
+  long long ldc;
+  int32_t* status;
+  unsigned long long timeout_ns;
+};
+
+struct MxTile {
+  int g, row0, n;          // first row (a multiple of 32), tokens computed (a multiple of 32)
+  int lo, hi, zero_to;     // rows stored: [lo, hi); this tile also zeroes the rows [hi, zero_to)
+  int m;                   // first weight row
+};
+
+// D (+)= A * B with one E8M0 scale per 32 elements; A and B E2M1, K = 64; issued by one thread for the pair.
+__device__ __forceinline__ void umma_mxf4_2cta(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
+                                               uint32_t scale_a, uint32_t scale_b, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate)
+      : "memory");
+}
+// An atom of scales (32 rows of 16 bytes) from shared memory into four columns of tensor memory, in every warp's quarter;
+// in both CTAs of the pair, each from its own shared memory.
+__device__ __forceinline__ void tmem_cp_scales_2cta(uint32_t tmem_dst, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem_dst), "l"(desc) : "memory");
+}
+// Unswizzled rows of 16 bytes: groups of eight rows 128 bytes apart.
+__device__ __forceinline__ uint64_t make_scale_desc(uint32_t smem_addr) {
+  return (uint64_t)((smem_addr >> 4) & 0x3FFF) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+// kind::mxf4: bits 4..5 scale byte of B, 7..9 A format and 10..11 B format (1 = E2M1), 17..22 N >> 3, 23 scale format
+// (1 = E8M0), 24..28 M >> 4, 29..30 scale byte of A.
+__host__ __device__ constexpr uint32_t make_instr_desc_mxf4(int M, int N, int scale_byte) {
+  return ((uint32_t)scale_byte << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | (1u << 23) |
+         ((uint32_t)(M >> 4) << 24) | ((uint32_t)scale_byte << 29);
+}
+
+template <int EPI>
+__global__ void __launch_bounds__(MXG_THREADS, 1)
+ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
+  constexpr bool GATED = EPI != MX_EPI_BF16, SAVE = EPI == MX_EPI_SWIGLU_SAVE;
+  constexpr int NST = MXG_STAGES;
+  constexpr int TOK_ROW = (SAVE ? 384 : GATED ? 128 : 256) + 16;     // bytes of a staged token
+  const int crank = (int)cluster_cta_rank();
+  const int work_id0 = (int)(blockIdx.x >> 1), work_stride = (int)(gridDim.x >> 1);
+  extern __shared__ uint8_t smem_dyn[];
+  __shared__ __align__(8) uint64_t full[NST];
+  __shared__ __align__(8) uint64_t empty[NST];
+  __shared__ __align__(8) uint64_t acc_full[2];
+  __shared__ __align__(8) uint64_t acc_empty[2];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  __shared__ int s_end[MAX_GROUPS];
+  __shared__ int s_prefix[MAX_GROUPS + 1];
+  __shared__ __align__(128) uint8_t s_stage[MXG_SETS][TG_CHUNK * TOK_ROW];
+  __shared__ float s_scale[GATED ? 2 : 1][GATED ? MXG_MAX_N : 1];
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  uint8_t* stages = (uint8_t*)(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
+  volatile int* abortp = &s_abort;
+
+  if (tid == 0) {
+    // both CTAs' loads count on the leader's full barrier, on which only its producer arrives
+    for (int s = 0; s < NST; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int a = 0; a < 2; ++a) { mbar_init(&acc_full[a], 1); mbar_init(&acc_empty[a], 8 * MXG_SETS); }
+    mbar_fence_init();
+    s_abort = 0;
+  }
+  for (int g = tid; g < p.ngroups; g += MXG_THREADS) {
+    const int end = p.cu_seqlens != nullptr ? p.cu_seqlens[g] : p.total_rows;
+    s_end[g] = min(max(end, 0), p.total_rows);      // (no row outside the tensors is stored, whatever cu_seqlens says)
+  }
+  __syncthreads();
+  // rows of the group with tokens, from the multiple of 32 at or before its first
+  auto span = [&](int g) {
+    const int start = g == 0 ? 0 : s_end[g - 1], end = s_end[g];
+    return end > start ? (start & 31) + group_valid(p, g, start, end) : 0;
+  };
+  if (warp == 0) {      // exclusive prefix of token tiles per group
+    int run = 0;
+    for (int g0 = 0; g0 < p.ngroups; g0 += 32) {
+      const int g = g0 + lane;
+      const int nt = g < p.ngroups ? (span(g) + MXG_MAX_N - 1) / MXG_MAX_N : 0;
+      int incl = nt;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      if (g < p.ngroups) s_prefix[g] = run + incl - nt;
+      run += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) s_prefix[p.ngroups] = run;
+  }
+  if (warp == 1) { tmem_alloc2(&s_tmem, 512); tmem_relinquish2(); }
+  tc_fence_before();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = s_tmem;
+
+  const int m_tiles = (p.w_rows + 255) / 256;
+  const long long total_tiles = (long long)s_prefix[p.ngroups] * m_tiles;
+  auto get = [&](long long id) {
+    MxTile t;
+    int lo = 0, hi = p.ngroups - 1;      // largest g with prefix[g] * m_tiles <= id
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if ((long long)s_prefix[mid] * m_tiles <= id) lo = mid; else hi = mid - 1;
+    }
+    t.g = lo;
+    const int nt = s_prefix[lo + 1] - s_prefix[lo];
+    const int local = (int)(id - (long long)s_prefix[lo] * m_tiles);
+    const int mi = local / nt, ti = local - mi * nt;       // tiles that share weights are neighbours
+    const int start = lo == 0 ? 0 : s_end[lo - 1], end = s_end[lo];
+    const int length = span(lo), valid = start + length - (start & 31);
+    t.n = ((length + nt - 1) / nt + 31) & ~31;
+    t.row0 = (start & ~31) + ti * t.n;
+    t.lo = max(t.row0, start);
+    t.hi = max(t.lo, min(t.row0 + t.n, valid));
+    t.zero_to = ti == nt - 1 ? end : 0;
+    t.m = mi * 256;
+    return t;
+  };
+  const int num_kb = (p.K + MXG_BK - 1) / MXG_BK;
+  auto warp_wait = [&](uint64_t* bar, uint32_t parity, int where) {
+    return __all_sync(0xffffffffu, gemm_wait(bar, parity, abortp, p, where)) != 0;
+  };
+  // (the same in every lane: said so, see ep_token_gemm_kernel)
+  auto uniform = [&](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+
+  if (warp == 0) {
+    // ================= TMA producer =================
+    const bool issue = elect_one();
+    if (issue) { tma_prefetch_desc(&p.w); tma_prefetch_desc(&p.ws); tma_prefetch_desc(&p.ts); }
+    RingSlot st;
+    bool ok = true;
+    for (long long id = work_id0; id < total_tiles && ok; id += work_stride) {
+      const MxTile t = get(id);
+      const int n = uniform(t.n), row0 = uniform(t.row0), g = uniform(t.g), m = uniform(t.m);
+      const int box = min(4, (n / 2 + 31) / 32);
+      const int atoms = (n + 127) / 128;       // row atoms that hold the tokens' scales
+      const CUtensorMap* tmap = &p.tok[0] + (box - 1);
+      const uint32_t bytes = 2u * (uint32_t)(MXG_W_BYTES + min(box * 32, MXG_MAX_N / 2) * 128 + (1 + atoms) * MXG_S_BYTES);
+      const int wrow = g * p.w_rows + m + 128 * crank, watom = g * p.w_atoms + m / 128 + crank;
+      const int trow = row0 + crank * (n / 2), tatom = (row0 >> 5 & 3) * p.t_atoms + (row0 >> 7);
+      for (int kb = 0; kb < num_kb; ++kb, st.next(NST)) {
+        const int s = st.slot;
+        ok = warp_wait(&empty[s], st.parity ^ 1u, 1);
+        if (!ok) break;
+        if (!issue) continue;
+        uint8_t* sw = stages + (size_t)s * MXG_STAGE;
+        uint8_t* ss = sw + MXG_W_BYTES + MXG_T_BYTES;
+        const uint32_t bar = mapa_u32(&full[s], 0);
+        if (crank == 0) mbar_expect_tx(&full[s], bytes);
+        tma_load_2d_pair(sw, &p.w, kb * 128, wrow, bar);
+        tma_load_2d_pair(sw + MXG_W_BYTES, tmap, kb * 128, trow, bar);
+        tma_load_2d_pair(ss, &p.ws, kb * 256, watom, bar);
+        for (int a = 0; a < atoms; ++a) tma_load_2d_pair(ss + (1 + a) * MXG_S_BYTES, &p.ts, kb * 256, tatom + a, bar);
+      }
+    }
+  } else if (warp == 1) {
+    // ================= MMA issuer (the leader issues for both CTAs of the pair) =================
+    if (crank == 0) {
+      const bool issue = elect_one();
+      const uint64_t desc_w = make_smem_desc(smem_u32(stages), 16, 1024);
+      const uint64_t desc_t = make_smem_desc(smem_u32(stages) + MXG_W_BYTES, 16, 1024);
+      const uint64_t desc_s = make_scale_desc(smem_u32(stages) + MXG_W_BYTES + MXG_T_BYTES);
+      RingSlot st;
+      int tile_n = 0;
+      uint32_t set = 0;
+      bool ok = true;
+      for (long long id = work_id0; id < total_tiles && ok; id += work_stride, ++tile_n) {
+        const MxTile t = get(id);
+        const int n = uniform(t.n), atoms = (n + 127) / 128;
+        const uint32_t idesc = make_instr_desc_mxf4(256, n, 0);
+        const int acc = tile_n & 1;
+        if (!warp_wait(&acc_empty[acc], ((uint32_t)(tile_n >> 1) & 1u) ^ 1u, 2)) break;
+        tc_fence_after();
+        const uint32_t tacc = tmem_base + (uint32_t)acc * MXG_MAX_N;
+        for (int kb = 0; kb < num_kb; ++kb, st.next(NST), set ^= MXG_SCALE_COLS) {
+          const int s = st.slot;
+          ok = warp_wait(&full[s], st.parity, 3);
+          if (!ok) break;
+          tc_fence_after();
+          if (issue) {
+            const uint32_t at = (uint32_t)(s * (MXG_STAGE >> 4));
+            const uint64_t da = desc_w + at, db = desc_t + at, ds = desc_s + at;
+            const uint32_t tsa = tmem_base + MXG_SCALES_AT + set, tsb = tsa + 8;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {        // block atoms of the k-block
+              tmem_cp_scales_2cta(tsa + 4 * j, ds + j * (MX_ATOM_BYTES >> 4));
+              for (int a = 0; a < atoms; ++a)
+                tmem_cp_scales_2cta(tsb + 8 * j + 4 * a, ds + (((1 + a) * MXG_S_BYTES + j * MX_ATOM_BYTES) >> 4));
+            }
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)       // 64 elements: two of an atom row's four scales
+              umma_mxf4_2cta(tacc, da + kk * 2, db + kk * 2, idesc | ((uint32_t)(kk & 1) << 5) | ((uint32_t)(kk & 1) << 30),
+                             tsa + 4 * (kk >> 1), tsb + 8 * (kk >> 1), (kb > 0 || kk > 0) ? 1u : 0u);
+            umma_commit_2cta(&empty[s], 3);
+          }
+        }
+        if (!ok) break;
+        if (issue) umma_commit_2cta(&acc_full[acc], 3);
+      }
+    }
+  } else {
+    // ========= epilogue: two sets of four warps, each warp one quarter of the CTA's weight rows =========
+    const int q = warp & 3, set = (warp - 2) >> 2;
+    const int te = tid - 64 - set * 128;                    // 0..127
+    const int first = set * TG_CHUNK, step = MXG_SETS * TG_CHUNK;
+    const int my_tok = (te >> 5) * step + first + (te & 31);
+    int tile_n = 0;
+    uint8_t* const sb = s_stage[set];
+    // this thread's row of the matrices that its warp stores: token 8 (lane / 16) + lane % 8, columns 8 (lane / 8 % 2)
+    const uint32_t st_addr = smem_u32(sb) + (uint32_t)((8 * (lane >> 4) + (lane & 7)) * TOK_ROW + q * (GATED ? 32 : 64) +
+                                                       ((lane >> 3) & 1) * 16);
+    const bool vec_ok = p.vec_out != 0;
+    for (long long id = work_id0; id < total_tiles; id += work_stride, ++tile_n) {
+      const MxTile t = get(id);
+      const int acc = tile_n & 1;
+      if constexpr (GATED) {       // (published by the barriers below)
+        for (int i = my_tok; i < t.n; i += 4 * step) {
+          const int r = t.row0 + i;
+          s_scale[acc][i] = r >= t.lo && r < t.hi && p.row_scale != nullptr ? p.row_scale[r] : 1.f;
+        }
+      }
+      const bool have = gemm_wait(&acc_full[acc], (uint32_t)(tile_n >> 1) & 1u, abortp, p, 4);
+      __syncwarp();
+      if (!epilogue_all(set, have)) break;
+      tc_fence_after();
+      const uint32_t tacc = tmem_base + (uint32_t)acc * MXG_MAX_N + ((uint32_t)(q * 32) << 16);
+      uint32_t r[32];
+      auto release_acc = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (crank != 0) mbar_arrive_remote(&acc_empty[acc], 0);
+          else mbar_arrive(&acc_empty[acc]);
+        }
+      };
+      // the two scales of this CTA's 64 activations of a row: four of its eight threads store one phase each
+      auto store_scales = [&](int row, uint32_t both) {
+        const int s = te & 7, at = row - 32 * s, k = t.m / 2 + 64 * crank;
+        if (s < MX_PHASES && at >= 0 && (k >> 7) < p.k_atoms)
+          *reinterpret_cast<uint16_t*>(p.scales + (long long)s * p.out_atoms * p.k_atoms * MX_ATOM_BYTES +
+                                       mx_scale_offset(at, k >> 7, p.k_atoms) + (k >> 5 & 3)) = (uint16_t)both;
+      };
+      if (first < t.n) {
+        tmem_ld_16x256_x4(tacc + first, r);
+        tmem_ld_16x256_x4(tacc + first + (16u << 16), r + 16);
+      } else {
+        release_acc();
+      }
+#pragma unroll 1
+      for (int c = first; c < t.n; c += step) {
+        __syncwarp();
+        tmem_ld_wait();
+        uint32_t pk[16];       // [16-row half][token block][lower, upper 8 rows]
+        uint32_t pa[8];        // activations [token block][lower, upper 8 columns]
+        auto pack = [](float a, float b) {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+          return *reinterpret_cast<const uint32_t*>(&h);
+        };
+        if constexpr (GATED) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float a[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float g = __uint_as_float(r[2 * i + e]), u = __uint_as_float(r[16 + 2 * i + e]);
+              a[e] = g / (1.f + __expf(-g)) * u * s_scale[acc][c + 8 * (i >> 1) + 2 * (lane & 3) + e];
+            }
+            pa[i] = pack(a[0], a[1]);
+          }
+        }
+        if constexpr (!GATED || SAVE) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) pk[i] = pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+        }
+        if (c + step < t.n) {            // the next 32 tokens travel while these leave
+          tmem_ld_16x256_x4(tacc + c + step, r);
+          tmem_ld_16x256_x4(tacc + c + step + (16u << 16), r + 16);
+        } else {
+          release_acc();
+        }
+        __syncwarp();
+        if constexpr (GATED) {
+#pragma unroll
+          for (int j = 0; j < 4; j += 2)
+            stmatrix_x4_trans(st_addr + (uint32_t)(j * 8 * TOK_ROW), pa[2 * j], pa[2 * j + 1], pa[2 * j + 2], pa[2 * j + 3]);
+        }
+        if constexpr (!GATED || SAVE) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 4; j += 2)
+              stmatrix_x4_trans(st_addr + (uint32_t)(j * 8 * TOK_ROW + (SAVE ? 128 * (1 + h) : h * 32)),
+                                pk[8 * h + 2 * j], pk[8 * h + 2 * j + 1], pk[8 * h + 2 * j + 2], pk[8 * h + 2 * j + 3]);
+        }
+        __syncwarp();
+        epilogue_sync(set);
+        if constexpr (GATED) {
+          const int f = (te & 7) * 8, col0 = t.m / 2 + 64 * crank + f;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int k = (te >> 3) + 16 * i, row = t.row0 + c + k;
+            const bool mine = row >= t.lo && row < t.hi;
+            const uint4 a4 = *reinterpret_cast<const uint4*>(sb + k * TOK_ROW + f * 2);
+            const long long off = (long long)row * p.ldc + col0;
+            if (mine && col0 < p.N) {
+              if (p.out) store8(p.out + off, a4, p.N - col0, vec_ok);
+              if constexpr (SAVE) {
+                if (p.gate) store8(p.gate + off, *reinterpret_cast<const uint4*>(sb + k * TOK_ROW + 128 + f * 2), p.N - col0, vec_ok);
+                if (p.up) store8(p.up + off, *reinterpret_cast<const uint4*>(sb + k * TOK_ROW + 256 + f * 2), p.N - col0, vec_ok);
+              }
+            }
+            if (p.codes != nullptr) {      // four neighbouring threads hold a block, eight a row's two
+              const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&a4);
+              float v[8];
+              uint32_t a = 0u;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                v[j] = col0 + j < p.N ? __bfloat162float(e[j]) : 0.f;
+                a = max(a, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+              }
+              a = max(a, __shfl_xor_sync(0xffffffffu, a, 1));
+              a = max(a, __shfl_xor_sync(0xffffffffu, a, 2));
+              const uint32_t b = mx_scale(a);
+              const float inv = mx_inverse(b);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[j] = b == 255u ? 0.f : v[j] * inv;
+              const uint32_t both = __shfl_sync(0xffffffffu, b, lane & 24) | __shfl_sync(0xffffffffu, b, (lane & 24) + 4) << 8;
+              if (mine) {
+                if (col0 < 2 * p.code_bytes)
+                  *reinterpret_cast<uint32_t*>(p.codes + (long long)row * p.code_bytes + col0 / 2) = mx_codes(v);
+                store_scales(row, both);
+              }
+            }
+          }
+        } else {
+          const int f = (te & 15) * 8, col0 = t.m + 128 * crank + f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = (te >> 4) + 8 * i, row = t.row0 + c + k;
+            if (row < t.lo || row >= t.hi || col0 >= p.N) continue;
+            store8(p.out + (long long)row * p.ldc + col0, *reinterpret_cast<const uint4*>(sb + k * TOK_ROW + f * 2), p.N - col0, vec_ok);
+          }
+        }
+        epilogue_sync(set);              // every row of the set's buffer has been read: it may be filled again
+      }
+      {      // padding rows that no tile computes
+        constexpr int V = GATED ? 8 : 16;                    // vectors of this CTA's columns in a row
+        const int f = (te & (V - 1)) * 8, col0 = (GATED ? t.m / 2 : t.m) + V * 8 * crank + f;
+        for (int row = t.hi + (te + 128 * set) / V; row < t.zero_to; row += 128 * MXG_SETS / V) {
+          const uint4 zero = make_uint4(0, 0, 0, 0);
+          const long long off = (long long)row * p.ldc + col0;
+          if (col0 < p.N) {
+            if (p.out) store8(p.out + off, zero, p.N - col0, vec_ok);
+            if constexpr (SAVE) {
+              if (p.gate) store8(p.gate + off, zero, p.N - col0, vec_ok);
+              if (p.up) store8(p.up + off, zero, p.N - col0, vec_ok);
+            }
+          }
+          if constexpr (GATED) {
+            if (p.codes != nullptr) {
+              if (col0 < 2 * p.code_bytes) *reinterpret_cast<uint32_t*>(p.codes + (long long)row * p.code_bytes + col0 / 2) = 0u;
+              store_scales(row, 0u);
+            }
+          }
+        }
+      }
+    }
+  }
+  // ---- teardown: everything joins, in-flight work is given time to land on an abort ----------
+  tc_fence_before();
+  __syncthreads();
+  if (s_abort) {
+    unsigned long long t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) { }
+  }
+  cluster_sync_all();        // neither CTA leaves while its peer may still touch it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc2(tmem_base, 512);
+  }
+}
+
+}  // namespace mep

@@ -1,0 +1,312 @@
+// Quantisation into microscaled 4-bit operands (mx_format.cuh) and back.  Both directions are bandwidth kernels: one
+// pass, every element read and written once.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "device/mx_format.cuh"
+#include "host/ctx.h"
+#include "host/errors.h"
+
+namespace mep {
+
+enum { MX_BF16 = 0, MX_FP16 = 1, MX_FP32 = 2 };
+
+__device__ __forceinline__ float mx_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float mx_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float mx_float(float x) { return x; }
+__device__ __forceinline__ uint32_t mx_abs(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+
+// Where row r of the output goes: as it is, or as gate (1) / up (2) column of the packed pair, sixteen of either in turn.
+__device__ __forceinline__ int mx_out_row(int r, int interleave) {
+  return interleave == 0 ? r : (r >> 4) * 32 + (r & 15) + (interleave == 2 ? 16 : 0);
+}
+
+struct MxQuantParams {
+  const void* x;
+  long long batch, stride;      // elements between matrices, and between rows of x
+  int mats, rows, cols;         // of x
+  int out_rows;                 // rows of a matrix of the output (codes)
+  int code_bytes, k_atoms, row_atoms;
+  uint8_t* codes;
+  uint8_t* scales;
+  const int32_t* rows_ptr;      // rows of x that hold something, on the device; or null
+  int interleave;
+  int phases;                   // 4: token rows, whose scales are stored at four phases
+};
+
+// Four scales of row r, once a phase: thread `s` of each group of `phases` stores them.
+__device__ __forceinline__ void mx_store_scales(const MxQuantParams& p, int mat, int r, int ka, int s, uint32_t w) {
+  if (s >= p.phases || r < 32 * s || ka >= p.k_atoms) return;
+  const long long copy = p.phases == 1 ? mat : s;
+  *reinterpret_cast<uint32_t*>(p.scales + copy * p.row_atoms * p.k_atoms * MX_ATOM_BYTES + mx_scale_offset(r - 32 * s, ka, p.k_atoms)) = w;
+}
+
+// Eight elements of a row from column c on; behind the row's end zeros.
+template <class T, bool VEC>
+__device__ __forceinline__ void mx_load8(const T* row, int c, int cols, float* v) {
+  if constexpr (VEC) {
+    if (c < cols) {               // (cols is a multiple of 8)
+      uint4 q[sizeof(T) / 2];
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) q[i] = __ldcs(reinterpret_cast<const uint4*>(row + c) + i);
+      const T* e = reinterpret_cast<const T*>(q);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = mx_float(e[i]);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? mx_float(row[c + i]) : 0.f;
+  }
+}
+
+// Along the rows.  A warp takes 256 elements of a row, a lane eight: four lanes share a block, sixteen the four scales
+// of an atom's row, which leave as one word.
+constexpr int MXQ_WARPS = 8, MXQ_DEPTH = 4;
+
+template <class T, bool VEC>
+__global__ void __launch_bounds__(MXQ_WARPS * 32) ep_mx_quant_rows_kernel(const __grid_constant__ MxQuantParams p) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rows = p.rows_ptr ? max(0, min(*p.rows_ptr, p.rows)) : p.rows;
+  const int parts = (p.k_atoms + 1) / 2;
+  const long long total = (long long)p.mats * rows * parts, stride = (long long)gridDim.x * MXQ_WARPS;
+  for (long long t0 = (long long)blockIdx.x * MXQ_WARPS + warp; t0 < total; t0 += stride * MXQ_DEPTH) {
+    float v[MXQ_DEPTH][8];
+    int mat[MXQ_DEPTH], row[MXQ_DEPTH], col[MXQ_DEPTH];
+#pragma unroll
+    for (int i = 0; i < MXQ_DEPTH; ++i) {
+      const long long t = t0 + i * stride;
+      if (t >= total) break;
+      const long long line = t / parts;
+      col[i] = (int)(t - line * parts) * 256 + lane * 8;
+      mat[i] = (int)(line / rows);
+      row[i] = (int)(line - (long long)mat[i] * rows);
+      mx_load8<T, VEC>((const T*)p.x + mat[i] * p.batch + row[i] * p.stride, col[i], p.cols, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < MXQ_DEPTH; ++i) {
+      if (t0 + i * stride >= total) break;
+      uint32_t a = 0u;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a = max(a, mx_abs(v[i][e]));
+      a = max(a, __shfl_xor_sync(0xffffffffu, a, 1));
+      a = max(a, __shfl_xor_sync(0xffffffffu, a, 2));
+      const uint32_t b = mx_scale(a);
+      const float inv = mx_inverse(b);
+      // (a NaN scale: zeros, whatever inf * 0 would give)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = b == 255u ? 0.f : v[i][e] * inv;
+      const int r = mx_out_row(row[i], p.interleave);
+      if (col[i] < 2 * p.code_bytes)
+        *reinterpret_cast<uint32_t*>(p.codes + ((long long)mat[i] * p.out_rows + r) * p.code_bytes + col[i] / 2) = mx_codes(v[i]);
+      // bytes of lanes 0, 4, 8, 12 (16, ...) to lane 0 (16)
+      uint32_t w = b | (__shfl_down_sync(0xffffffffu, b, 4) << 8);
+      w |= __shfl_down_sync(0xffffffffu, w, 8) << 16;
+      w = __shfl_sync(0xffffffffu, w, lane & 16);
+      mx_store_scales(p, mat[i], r, col[i] >> 7, lane & 15, w);
+    }
+  }
+}
+
+// Along the columns: the output is the transpose.  A block takes 256 rows x 64 columns of x, a warp one block of 32 rows,
+// a lane two columns of it; the codes of a column meet in shared memory and leave as 128-byte rows.
+constexpr int MXT_COLS = 64, MXT_ROWS = 256, MXT_PITCH = 128 + 16;
+
+template <class T, bool VEC>
+__global__ void __launch_bounds__(256) ep_mx_quant_cols_kernel(const __grid_constant__ MxQuantParams p) {
+  __shared__ __align__(16) uint8_t s_codes[MXT_COLS * MXT_PITCH];
+  __shared__ __align__(4) uint8_t s_scale[MXT_COLS][8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int r0 = blockIdx.y * MXT_ROWS, c0 = blockIdx.x * MXT_COLS;
+  for (int m = blockIdx.z; m < p.mats; m += gridDim.z) {
+    const T* x = (const T*)p.x + m * p.batch;
+    const int c = c0 + 2 * lane;
+    float v[2][MX_BLOCK];
+    uint32_t a[2] = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < MX_BLOCK; ++i) {
+      const int r = r0 + warp * MX_BLOCK + i;
+      v[0][i] = v[1][i] = 0.f;
+      if (r < p.rows) {
+        const T* e = x + (long long)r * p.stride + c;
+        if constexpr (VEC) {           // (an even number of columns)
+          if (c < p.cols) {
+            struct __align__(2 * sizeof(T)) Pair { T a, b; };
+            const Pair q = *reinterpret_cast<const Pair*>(e);
+            v[0][i] = mx_float(q.a);
+            v[1][i] = mx_float(q.b);
+          }
+        } else {
+          if (c < p.cols) v[0][i] = mx_float(e[0]);
+          if (c + 1 < p.cols) v[1][i] = mx_float(e[1]);
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < MX_BLOCK; ++i) a[h] = max(a[h], mx_abs(v[h][i]));
+      const uint32_t b = mx_scale(a[h]);
+      const float inv = mx_inverse(b);
+#pragma unroll
+      for (int i = 0; i < MX_BLOCK; ++i) v[h][i] = b == 255u ? 0.f : v[h][i] * inv;
+      uint4 q;
+      q.x = mx_codes(v[h]); q.y = mx_codes(v[h] + 8); q.z = mx_codes(v[h] + 16); q.w = mx_codes(v[h] + 24);
+      *reinterpret_cast<uint4*>(s_codes + (2 * lane + h) * MXT_PITCH + warp * 16) = q;
+      s_scale[2 * lane + h][warp] = (uint8_t)b;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < MXT_COLS * 8; i += 256) {       // 16 bytes of a column's codes
+      const int n = i >> 3, k = r0 / 2 + (i & 7) * 16;
+      if (c0 + n < p.cols && k < p.code_bytes)
+        *reinterpret_cast<uint4*>(p.codes + ((long long)m * p.out_rows + mx_out_row(c0 + n, p.interleave)) * p.code_bytes + k) =
+            *reinterpret_cast<const uint4*>(s_codes + n * MXT_PITCH + (i & 7) * 16);
+    }
+    for (int i = threadIdx.x; i < 2 * MXT_COLS * p.phases; i += 256) {
+      const int n = (i >> 1) % MXT_COLS, h = i & 1;
+      if (c0 + n < p.cols)
+        mx_store_scales(p, m, mx_out_row(c0 + n, p.interleave), r0 / MX_ATOM_K + h, i / (2 * MXT_COLS),
+                        *reinterpret_cast<const uint32_t*>(&s_scale[n][4 * h]));
+    }
+    __syncthreads();
+  }
+}
+
+struct MxDequantParams {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  int mats, rows, cols;         // of the values; `rows` of gate or up where they are a packed pair
+  int in_rows, code_bytes, k_atoms, row_atoms;
+  void* out;                    // [mats][rows][cols]
+  const int32_t* rows_ptr;
+  int interleave;
+};
+
+// A lane takes eight values of a row, a warp 256.  (Exact in bf16 but for what a bf16 subnormal rounds, fp32 always.)
+template <class T, bool VEC>
+__global__ void __launch_bounds__(MXQ_WARPS * 32) ep_mx_dequant_kernel(const __grid_constant__ MxDequantParams p) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rows = p.rows_ptr ? max(0, min(*p.rows_ptr, p.rows)) : p.rows;
+  const int parts = (p.cols + 255) / 256;
+  const long long total = (long long)p.mats * rows * parts, stride = (long long)gridDim.x * MXQ_WARPS;
+  for (long long t0 = (long long)blockIdx.x * MXQ_WARPS + warp; t0 < total; t0 += stride * MXQ_DEPTH) {
+    uint32_t code[MXQ_DEPTH], b[MXQ_DEPTH];
+    T* dst[MXQ_DEPTH];
+    int col[MXQ_DEPTH];
+#pragma unroll
+    for (int i = 0; i < MXQ_DEPTH; ++i) {
+      const long long t = t0 + i * stride;
+      if (t >= total) break;
+      const long long line = t / parts;
+      const int c = (int)(t - line * parts) * 256 + lane * 8;
+      const int mat = (int)(line / rows), row = (int)(line - (long long)mat * rows), r = mx_out_row(row, p.interleave);
+      col[i] = c;
+      dst[i] = (T*)p.out + ((long long)mat * p.rows + row) * p.cols + c;
+      if (c < p.cols) {
+        code[i] = __ldcs(reinterpret_cast<const uint32_t*>(p.codes + ((long long)mat * p.in_rows + r) * p.code_bytes + c / 2));
+        b[i] = p.scales[(long long)mat * p.row_atoms * p.k_atoms * MX_ATOM_BYTES + mx_scale_offset(r, c >> 7, p.k_atoms) + ((c >> 5) & 3)];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < MXQ_DEPTH; ++i) {
+      if (t0 + i * stride >= total) break;
+      if (col[i] >= p.cols) continue;
+      const float s = mx_value(b[i]);
+      __align__(16) T v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float f = mx_element(code[i] >> (4 * e)) * s;
+        if constexpr (sizeof(T) == 2) v[e] = __float2bfloat16(f);
+        else v[e] = f;
+      }
+      if constexpr (VEC) {
+#pragma unroll
+        for (int q = 0; q < (int)sizeof(T) / 2; ++q) __stcs(reinterpret_cast<uint4*>(dst[i]) + q, reinterpret_cast<const uint4*>(v)[q]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) if (col[i] + e < p.cols) dst[i][e] = v[e];
+      }
+    }
+  }
+}
+
+static int mx_blocks(long long tasks) {
+  const long long blocks = (tasks + MXQ_WARPS - 1) / MXQ_WARPS, most = 148 * 8;
+  return (int)(blocks < most ? blocks : most);
+}
+
+template <class T>
+static int mx_quant(const MxQuantParams& p, bool along_cols, cudaStream_t stream) {
+  const bool rows16 = (uintptr_t)p.x % 16 == 0 && (p.stride * sizeof(T)) % 16 == 0 && (p.batch * sizeof(T)) % 16 == 0 && p.cols % 8 == 0;
+  const bool pairs = (uintptr_t)p.x % (2 * sizeof(T)) == 0 && p.stride % 2 == 0 && p.batch % 2 == 0 && p.cols % 2 == 0;
+  if (along_cols) {
+    const dim3 grid((unsigned)((p.cols + MXT_COLS - 1) / MXT_COLS), (unsigned)((p.rows + MXT_ROWS - 1) / MXT_ROWS),
+                    (unsigned)(p.mats < 65535 ? p.mats : 65535));
+    if (grid.y > 65535) return fail(-5, "mx quantise: %d rows are too many along the last but one axis", p.rows);
+    if (pairs) ep_mx_quant_cols_kernel<T, true><<<grid, 256, 0, stream>>>(p);
+    else ep_mx_quant_cols_kernel<T, false><<<grid, 256, 0, stream>>>(p);
+  } else {
+    const int blocks = mx_blocks((long long)p.mats * p.rows * ((p.k_atoms + 1) / 2));
+    if (rows16) ep_mx_quant_rows_kernel<T, true><<<blocks, MXQ_WARPS * 32, 0, stream>>>(p);
+    else ep_mx_quant_rows_kernel<T, false><<<blocks, MXQ_WARPS * 32, 0, stream>>>(p);
+  }
+  MEP_CUDA_OK(cudaGetLastError());
+  return 0;
+}
+
+}  // namespace mep
+
+using namespace mep;
+
+extern "C" {
+
+// x [mats][rows][cols] of `type` (bf16, fp16, fp32), `batch` and `stride` elements apart.  along_cols = 0: blocks along the
+// columns, output rows are x's; 1: blocks along the rows, output rows are x's columns.  out_rows: rows of an output matrix.
+// phases = 4 (one matrix): scales for token rows, else 1.
+int mep_mx_quantize(const void* x, int type, int64_t batch, int64_t stride, int mats, int rows, int cols, int along_cols,
+                    int interleave, int out_rows, int phases, const int32_t* rows_ptr, void* codes, void* scales, cudaStream_t stream) {
+  if (mats < 0 || rows < 0 || cols < 0) return fail(-1, "mx quantise: %d x %d x %d elements", mats, rows, cols);
+  if (along_cols && rows_ptr) return fail(-2, "mx quantise: a device row count goes with blocks along the rows");
+  if (phases != 1 && (phases != MX_PHASES || mats > 1)) return fail(-4, "mx quantise: %d phases of %d matrices", phases, mats);
+  if (mats == 0 || rows == 0 || cols == 0) return 0;
+  MxQuantParams p;
+  const int K = along_cols ? rows : cols;
+  p.x = x; p.batch = batch; p.stride = stride; p.mats = mats; p.rows = rows; p.cols = cols;
+  p.out_rows = out_rows; p.code_bytes = (K + MX_BLOCK - 1) / MX_BLOCK * (MX_BLOCK / 2);
+  p.k_atoms = mx_atoms(K); p.row_atoms = mx_atoms(out_rows);
+  p.codes = (uint8_t*)codes; p.scales = (uint8_t*)scales; p.rows_ptr = rows_ptr; p.interleave = interleave; p.phases = phases;
+  if (type == MX_BF16) return mx_quant<__nv_bfloat16>(p, along_cols != 0, stream);
+  if (type == MX_FP16) return mx_quant<__half>(p, along_cols != 0, stream);
+  if (type == MX_FP32) return mx_quant<float>(p, along_cols != 0, stream);
+  return fail(-3, "mx quantise: unknown type %d", type);
+}
+
+// The values [mats][rows][cols] in bf16, or fp32.
+int mep_mx_dequantize(const void* codes, const void* scales, int mats, int rows, int cols, int interleave, int in_rows,
+                      const int32_t* rows_ptr, int fp32, void* out, cudaStream_t stream) {
+  if (mats < 0 || rows < 0 || cols < 0) return fail(-1, "mx dequantise: %d x %d x %d elements", mats, rows, cols);
+  if (mats == 0 || rows == 0 || cols == 0) return 0;
+  MxDequantParams p;
+  p.codes = (const uint8_t*)codes; p.scales = (const uint8_t*)scales; p.mats = mats; p.rows = rows; p.cols = cols;
+  p.in_rows = in_rows; p.code_bytes = (cols + MX_BLOCK - 1) / MX_BLOCK * (MX_BLOCK / 2);
+  p.k_atoms = mx_atoms(cols); p.row_atoms = mx_atoms(in_rows);
+  p.out = out; p.rows_ptr = rows_ptr; p.interleave = interleave;
+  const int blocks = mx_blocks((long long)mats * rows * ((cols + 255) / 256));
+  const bool vec = cols % 8 == 0 && (uintptr_t)out % 16 == 0;
+  if (fp32) {
+    if (vec) ep_mx_dequant_kernel<float, true><<<blocks, MXQ_WARPS * 32, 0, stream>>>(p);
+    else ep_mx_dequant_kernel<float, false><<<blocks, MXQ_WARPS * 32, 0, stream>>>(p);
+  } else {
+    if (vec) ep_mx_dequant_kernel<__nv_bfloat16, true><<<blocks, MXQ_WARPS * 32, 0, stream>>>(p);
+    else ep_mx_dequant_kernel<__nv_bfloat16, false><<<blocks, MXQ_WARPS * 32, 0, stream>>>(p);
+  }
+  MEP_CUDA_OK(cudaGetLastError());
+  return 0;
+}
+
+}  // extern "C"

@@ -258,17 +258,19 @@ def down_dgrad(dy, wd, cu_seqlens, *, wd_slot=None, split=None, out=None, g_begi
 
 
 def gateup_dgrad(dg, du, wg, wu, cu_seqlens, *, wg_slot=None, wu_slot=None, split=None, out=None,
-                 push=None, grid=0, pads=None):
+                 push=None, grid=0, pads=None, transposed=False):
     """``dx[rows,H] = dg Wg[g]^T + du Wu[g]^T`` (two K segments into one accumulator); ``push`` as
-    in :func:`down`."""
+    in :func:`down`.  ``transposed``: the weights are stored ``[G, H', H]`` (:func:`.mx.pack_gate_up`'s values)."""
     rows, Hp = dg.shape
-    H = wg.shape[1]
+    H = wg.shape[2 if transposed else 1]
+    assert wg.shape[1 if transposed else 2] == Hp and wu.shape == wg.shape
+    per_expert = wg.shape[1]
     if push is not None:
-        _tokens_gemm([dg, du], [wg, wu], [wg_slot, wu_slot], cu_seqlens, split, H, Hp, H, False,
+        _tokens_gemm([dg, du], [wg, wu], [wg_slot, wu_slot], cu_seqlens, split, H, Hp, per_expert, transposed,
                      EPI_BF16, [], H, push=push, grid=grid, pads=pads)
         return None
     dx = torch.empty(rows, H, dtype=torch.bfloat16, device=dg.device) if out is None else out
-    _tokens_gemm([dg, du], [wg, wu], [wg_slot, wu_slot], cu_seqlens, split, H, Hp, H, False,
+    _tokens_gemm([dg, du], [wg, wu], [wg_slot, wu_slot], cu_seqlens, split, H, Hp, per_expert, transposed,
                  EPI_BF16, [dx], dx.stride(0), grid=grid, pads=pads)
     return dx
 

@@ -1,0 +1,487 @@
+"""Microscaled 4-bit operators against the definition in 64 bits.
+
+Quantised values have to be equal.  A product's result is within half a bf16 step, 2^-8 of its value, and what K sums in
+fp32 can lose, K 2^-24 of the sum of magnitudes."""
+import pytest
+import torch
+
+from tests import mx_oracle as ox
+
+gpu = pytest.mark.gpu
+HALF = 2.0 ** -8
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+@pytest.fixture(autouse=True)
+def _status():
+    yield
+    if torch.cuda.is_available():
+        from moonep_b200.ops import gemm
+        torch.cuda.synchronize()
+        gemm.check_status()
+
+
+def _equal(got, want):
+    got = got.cpu().double()
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
+
+
+def _spread(gen, *shape):
+    """Values of many magnitudes, among them zeros and exact borders between codes."""
+    x = torch.randn(*shape, generator=gen) * torch.exp2(torch.randint(-20, 20, shape[:-1] + (1,), generator=gen).float())
+    border = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0, 0.0])[torch.randint(0, 10, shape, generator=gen)]
+    return torch.where(torch.rand(*shape, generator=gen) < 0.3, border, x)
+
+
+def test_oracle_values():
+    x = torch.tensor([[7.9, 0.25, -0.75, 1.25, 1.75, -2.5, 3.5, 5.0, 0.2, -6.0] + [0.0] * 22])
+    want = torch.tensor([[6.0, 0.0, -1.0, 1.0, 2.0, -2.0, 4.0, 4.0, 0.0, -6.0] + [0.0] * 22]).double()
+    assert torch.equal(ox.quantise(x), want)
+    assert torch.equal(ox.quantise(x * 2.0 ** -30), want * 2.0 ** -30)
+    assert ox.quantise(torch.tensor([[1.0, float("inf")]])).isnan().all()
+
+
+# ---- quantisation ------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", [(1, 1), (3, 32), (16, 7168), (129, 1003), (2, 65, 40), (5, 130, 264)])
+def test_quantise_rows(shape, dtype):
+    from moonep_b200.ops import mx
+    x = _spread(_gen(1), *shape).clamp(-60000, 60000).to(dtype)
+    q = mx.quantize(x.cuda())
+    assert q.shape == tuple(shape)
+    want = ox.quantise(x)
+    _equal(q.dequantize(torch.float32), want)
+    _equal(q.dequantize(), want)                      # (no magnitude here is below bf16's subnormals)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", [(1, 1), (32, 3), (2048, 96), (1003, 129), (2, 40, 65), (3, 264, 130)])
+def test_quantise_columns(shape, dtype):
+    from moonep_b200.ops import mx
+    x = _spread(_gen(2), *shape).clamp(-60000, 60000).to(dtype)
+    q = mx.quantize(x.cuda(), axis=-2)
+    assert q.shape == (*shape[:-2], shape[-1], shape[-2])
+    _equal(q.dequantize(torch.float32), ox.quantise(x.transpose(-1, -2).contiguous()))
+
+
+@gpu
+@pytest.mark.parametrize("axis", [-1, -2])
+def test_quantise_strides(axis):
+    from moonep_b200.ops import mx
+    base = _spread(_gen(3), 4, 70, 200).cuda()
+    for x in (base[1:3, 5:69, 8:136], base[:, ::2, 3:166], base[::2, 1:2], base[0, :, 1:]):
+        want = ox.quantise(x.cpu() if axis == -1 else x.cpu().transpose(-1, -2).contiguous())
+        _equal(mx.quantize(x, axis).dequantize(torch.float32), want)
+
+
+@gpu
+def test_quantise_extremes():
+    """Largest, smallest, subnormal and non-finite values; zero blocks; a block that is not full."""
+    from moonep_b200.ops import mx
+    x = torch.randn(8, 70, generator=_gen(4))
+    x[0, :32] = 0.0
+    x[1, 3], x[2, 40], x[3, 69] = float("nan"), float("inf"), -float("inf")
+    x[4, :32] *= 2.0 ** -126
+    x[4, 32:64] = 2.0 ** -149
+    x[5] *= 3.0e38 / x[5].abs().max()
+    x[6, 0], x[6, 1] = 3.4e38, 2.0 ** -149
+    x[7, :] = -0.0
+    q = mx.quantize(x.cuda())
+    _equal(q.dequantize(torch.float32), ox.quantise(x))
+    _equal(mx.quantize(x.t().contiguous().cuda(), axis=-2).dequantize(torch.float32), ox.quantise(x))
+
+
+@gpu
+def test_quantise_row_count_on_the_device():
+    from moonep_b200.ops import mx
+    x = torch.randn(300, 96, generator=_gen(5)).bfloat16()
+    n = torch.tensor([131], dtype=torch.int32).cuda()
+    q = mx.quantize(x.cuda(), rows_ptr=n)
+    _equal(q.dequantize()[:131], ox.quantise(x[:131]))
+    out = mx.quantize(x.cuda()).dequantize(rows_ptr=n)
+    _equal(out[:131], ox.quantise(x[:131]))
+    for bad in (-5, 0, 1000):
+        mx.quantize(x.cuda(), rows_ptr=torch.tensor([bad], dtype=torch.int32).cuda())
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(2, 96, 40), (1, 130, 16), (3, 64, 515), (70, 33)])
+def test_pack_gate_up(shape):
+    from moonep_b200.ops import mx
+    gen = _gen(6)
+    wg, wu = (_spread(gen, *shape).bfloat16() for _ in range(2))
+    q = mx.pack_gate_up(wg.cuda(), wu.cuda())
+    v = q.dequantize(torch.float32)
+    three = [w if w.dim() == 3 else w[None] for w in (wg, wu)]
+    assert q.shape == (2, three[0].shape[0], shape[-1], shape[-2])
+    for i in range(2):
+        _equal(v[i], ox.quantise(three[i].transpose(1, 2).contiguous()))
+
+
+@gpu
+def test_empty_operands():
+    from moonep_b200.ops import mx
+    q = mx.quantize(torch.empty(0, 64, device="cuda", dtype=torch.bfloat16))
+    w = mx.quantize(torch.randn(1, 48, 64, device="cuda"))
+    assert q.dequantize().shape == (0, 64)
+    assert mx.matmul(q, w, torch.zeros(1, dtype=torch.int32, device="cuda")).shape == (0, 48)
+    some = mx.quantize(torch.randn(5, 64, device="cuda"))
+    out = torch.full((5, 48), 7.0, device="cuda", dtype=torch.bfloat16)
+    mx.matmul(some, w, torch.zeros(1, dtype=torch.int32, device="cuda"), out=out)
+    assert (out == 7).all()
+
+
+# ---- products ----------------------------------------------------------------------------------
+GROUPS = [[5], [1, 0, 2], [128, 256, 0, 128], [100, 0, 300, 1, 129, 64], [225, 31, 33, 7], [448, 449, 1000]]
+
+
+def _ends(sizes):
+    return torch.tensor(sizes).cumsum(0).to(torch.int32)
+
+
+def _product_case(sizes, N, K, seed):
+    gen = _gen(seed)
+    rows = sum(sizes)
+    a, w = torch.randn(rows, K, generator=gen).bfloat16(), (torch.randn(len(sizes), N, K, generator=gen) * K ** -0.5).bfloat16()
+    return a, w, ox.quantise(a), ox.quantise(w)
+
+
+@gpu
+@pytest.mark.parametrize("N,K", [(256, 256), (8, 32), (515, 1000), (640, 2048), (1, 1)])
+@pytest.mark.parametrize("sizes", GROUPS)
+def test_product(sizes, N, K):
+    from moonep_b200.ops import mx
+    a, w, av, wv = _product_case(sizes, N, K, 7)
+    ends = _ends(sizes)
+    y = mx.matmul(mx.quantize(a.cuda()), mx.quantize(w.cuda()), ends.cuda()).cpu().double()
+    ref, mag = ox.product(av, wv, ends.tolist())
+    err = (y - ref).abs() - HALF * ref.abs() - (K + 2) * 2.0 ** -24 * mag
+    assert float(err.max()) <= 0, f"{float((y - ref).abs().max())} off, {int((err > 0).sum())} of {err.numel()}"
+
+
+@gpu
+def test_product_far_from_one():
+    """Scales at both ends of what E8M0 holds, and a NaN block: its rows and columns are NaN, the others are not."""
+    from moonep_b200.ops import mx
+    gen = _gen(8)
+    a, w = torch.randn(70, 96, generator=gen), torch.randn(1, 40, 96, generator=gen)
+    a[3] *= 2.0 ** 60
+    a[4] *= 2.0 ** -110
+    w[0, 5] *= 2.0 ** -60
+    a[7, 95], w[0, 9, 0] = float("nan"), float("inf")
+    y = mx.matmul(mx.quantize(a.cuda()), mx.quantize(w.cuda()), _ends([70]).cuda()).cpu().double()
+    ref, mag = ox.product(ox.quantise(a), ox.quantise(w), [70])
+    assert torch.equal(y.isnan(), ref.isnan())
+    # (row 4 times column 5 is of the size of 2^-170: bf16's smallest step is 2^-133, half of it rounding's at any size)
+    err = (y - ref).abs() - HALF * ref.abs() - 98 * 2.0 ** -24 * mag - 2.0 ** -134
+    assert float(err.nan_to_num(-1).max()) <= 0
+
+
+@gpu
+def test_product_leaves_other_rows():
+    """Rows in front of, between and behind the groups' tiles: only the groups' rows are written, padding becomes zero."""
+    from moonep_b200.ops import mx
+    sizes, K, N = [37, 128, 0, 90], 320, 200
+    a, w, av, wv = _product_case(sizes, N, K, 9)
+    ends = _ends(sizes)
+    pads = torch.tensor([[20, 17], [165, 0], [165, 0], [200, 55]], dtype=torch.int32)
+    out = torch.full((sum(sizes) + 50, N + 24), 7.0).bfloat16().cuda()
+    more = torch.cat([a, torch.full((30, K), float("nan"))]).cuda()
+    y = mx.matmul(mx.quantize(more), mx.quantize(w.cuda()), ends.cuda(), out=out[:-20, 8:8 + N], pads=pads.cuda())
+    assert y.data_ptr() == out[0, 8:].data_ptr()
+    ref, _ = ox.product(av, wv, ends.tolist())
+    ref[20:37], ref[200:255] = 0, 0
+    got = out.cpu().double()
+    assert float((got[:255, 8:8 + N] - ref).abs().max()) < 0.05
+    assert (got[20:37, 8:8 + N] == 0).all() and (got[200:255, 8:8 + N] == 0).all()
+    got[:255, 8:8 + N] = 7.0
+    assert (got == 7.0).all()
+
+
+@gpu
+def test_product_of_one_matrix():
+    """Without groups; the same numbers as one group, and on another stream."""
+    from moonep_b200.ops import mx
+    a, w, av, wv = _product_case([777], 384, 512, 10)
+    ref, mag = ox.product(av, wv, [777])
+    qa, qw = mx.quantize(a.cuda()), mx.quantize(w[0].cuda())
+    y = mx.matmul(qa, qw)
+    assert float(((y.cpu().double() - ref).abs() - HALF * ref.abs() - 514 * 2.0 ** -24 * mag).max()) <= 0
+    assert torch.equal(y, mx.matmul(qa, mx.quantize(w.cuda()), _ends([777]).cuda()))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        z = mx.matmul(mx.quantize(a.cuda()), qw)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(y, z)
+
+
+# ---- gate and up -------------------------------------------------------------------------------
+def _gated_ref(xv, gv, uv, ends, scale):
+    """act, gate, up and how far act may be off: fp32 sums, exp to 2^-16 (|x| steps), half a bf16 step."""
+    K = xv.shape[1]
+    gate, gm = ox.product(xv, gv, ends)
+    up, um = ox.product(xv, uv, ends)
+    sig = torch.sigmoid(gate)
+    act = gate * sig * up * scale[:, None]
+    dg, du = (K + 2) * 2.0 ** -24 * gm, (K + 2) * 2.0 ** -24 * um
+    off = ((1.1 * dg * up.abs()) + (gate * sig).abs() * du + 1.1 * dg * du) * scale[:, None].abs()
+    return act, gate, up, dg, du, off + act.abs() * (HALF + 1e-5 * (1 + gate.abs()))
+
+
+@gpu
+@pytest.mark.parametrize("H,Hp", [(256, 256), (64, 8), (1000, 515), (2048, 640), (32, 1)])
+@pytest.mark.parametrize("sizes", GROUPS)
+def test_gateup_swiglu(sizes, H, Hp):
+    from moonep_b200.ops import mx
+    gen = _gen(11)
+    rows, G = sum(sizes), len(sizes)
+    x = torch.randn(rows, H, generator=gen).bfloat16()
+    wg, wu = ((torch.randn(G, H, Hp, generator=gen) * 2 * H ** -0.5).bfloat16() for _ in range(2))
+    scale = torch.rand(rows, generator=gen) + 0.1
+    ends = _ends(sizes)
+    gv, uv = (ox.quantise(w.transpose(1, 2).contiguous()) for w in (wg, wu))
+    act_ref, gate_ref, up_ref, dg, du, off = _gated_ref(ox.quantise(x), gv, uv, ends.tolist(), scale.double())
+    xq, w = mx.quantize(x.cuda()), mx.pack_gate_up(wg.cuda(), wu.cuda())
+    act, gate, up = mx.gateup_swiglu(xq, w, ends.cuda(), row_scale=scale.cuda(), save_gate_up=True)
+    for got, ref, tol in ((act, act_ref, off), (gate, gate_ref, HALF * gate_ref.abs() + dg), (up, up_ref, HALF * up_ref.abs() + du)):
+        assert float(((got.cpu().double() - ref).abs() - tol).max()) <= 1e-30
+    alone, none, _ = mx.gateup_swiglu(xq, w, ends.cuda(), row_scale=scale.cuda())
+    assert none is None and torch.equal(alone, act)
+    want = mx.quantize(act).dequantize()
+    for save in (False, True):
+        q, g2, _ = mx.gateup_swiglu(xq, w, ends.cuda(), row_scale=scale.cuda(), quantize=True, save_gate_up=save)
+        assert torch.equal(q.dequantize(), want) and (not save or torch.equal(g2, gate))
+        # as an operand it is what quantising the activation gives
+        wd = mx.quantize(torch.randn(G, 72, Hp, generator=gen).cuda())
+        assert torch.equal(mx.matmul(q, wd, ends.cuda()), mx.matmul(mx.quantize(act), wd, ends.cuda()))
+
+
+@gpu
+def test_gateup_padding_rows():
+    from moonep_b200.ops import mx
+    gen = _gen(12)
+    H, Hp, ends = 256, 160, _ends([128, 64, 192])
+    pads = torch.tensor([[100, 28], [128, 64], [192, 0]], dtype=torch.int32)
+    x = torch.randn(384, H, generator=gen).bfloat16()
+    x[100:128], x[129:192] = 0, 0
+    pads[1] = torch.tensor([129, 63])
+    wg, wu = ((torch.randn(3, H, Hp, generator=gen) * H ** -0.5).bfloat16().cuda() for _ in range(2))
+    xq, w = mx.quantize(x.cuda()), mx.pack_gate_up(wg, wu)
+    plain = mx.gateup_swiglu(xq, w, ends.cuda(), save_gate_up=True)
+    padded = mx.gateup_swiglu(xq, w, ends.cuda(), save_gate_up=True, pads=pads.cuda())
+    for a, b in zip(plain, padded):
+        assert torch.equal(a, b)
+    q = mx.gateup_swiglu(xq, w, ends.cuda(), quantize=True, pads=pads.cuda())[0]
+    assert torch.equal(q.dequantize(), mx.quantize(plain[0]).dequantize())
+
+
+# ---- the FFN -----------------------------------------------------------------------------------
+def _ffn_ref(x, wg, wu, wd, ends, scale, dy=None):
+    """y, and with dy the gradients of x, wg, wu, wd, scale, by the formulas.  (The activation is rounded to bf16, then
+    quantised: act is given as the kernel's where a rounding may fall to either side.)"""
+    xv = ox.quantise(x)
+    gv, uv, dv = ox.quantise(wg.transpose(1, 2).contiguous()), ox.quantise(wu.transpose(1, 2).contiguous()), ox.quantise(wd)
+    gate, up = ox.product(xv, gv, ends)[0], ox.product(xv, uv, ends)[0]
+    sig = torch.sigmoid(gate)
+    act = ox.quantise((gate * sig * up * scale[:, None]).bfloat16())
+    y = ox.product(act, dv, ends)[0]
+    if dy is None:
+        return y
+    dy = dy.double()
+    d_act = ox.product(dy, dv.transpose(1, 2), ends)[0]
+    d_scale = (d_act * gate * sig * up).sum(1)
+    d_act = d_act * scale[:, None]
+    dg, du = d_act * up * sig * (1 + gate * (1 - sig)), d_act * gate * sig
+    dx = ox.product(dg, gv.transpose(1, 2), ends)[0] + ox.product(du, uv.transpose(1, 2), ends)[0]
+    dw = [torch.zeros(wg.shape, dtype=torch.float64) for _ in range(3)]
+    for g, s, e in ox.groups(ends):
+        dw[0][g], dw[1][g], dw[2][g] = xv[s:e].T @ dg[s:e], xv[s:e].T @ du[s:e], dy[s:e].T @ act[s:e]
+    return y, dx, dw[0], dw[1], dw[2], d_scale
+
+
+def _near(got, ref, tol):
+    """2-norm of the difference over that of the result."""
+    d = float((got.cpu().double() - ref).norm() / ref.norm().clamp_min(1e-30))
+    assert d <= tol, d
+
+
+# Independent roundings to bf16 are off by 2^-9 / sqrt(3) of a value in the mean square, at most 2^-8.  y has one; an
+# activation near a border may be quantised to either side (relative difference of the sums 2^-20, borders some 0.3
+# apart: one in 10^5, by a third of its value: 2^-10 in the norm).  A gradient of x passes the roundings of
+# d act, gate / up, d gate / d up, the bf16 weights exactly, and its own: four.
+Y_TOL, GRAD_TOL = 2 * HALF, 4 * HALF
+
+
+@gpu
+@pytest.mark.parametrize("sizes,H,Hp,scaled", [([777], 256, 72, False), ([64, 0, 192, 320], 384, 200, True), ([1], 128, 8, True),
+                                               ([128], 1024, 512, False)])
+def test_expert_ffn_gradients(sizes, H, Hp, scaled):
+    from moonep_b200.ops import mx
+    gen = _gen(13)
+    rows, G = sum(sizes), len(sizes)
+    x = torch.randn(rows, H, generator=gen).bfloat16()
+    wg, wu, wd = ((torch.randn(G, H, Hp, generator=gen) * s).bfloat16() for s in (H ** -0.5, H ** -0.5, Hp ** -0.5))
+    scale = torch.rand(rows, generator=gen) + 0.1 if scaled else torch.ones(rows)
+    dy = (torch.randn(rows, H, generator=gen) * 0.01).bfloat16()
+    ends = _ends(sizes)
+    ref = _ffn_ref(x, wg, wu, wd, ends.tolist(), scale.double(), dy)
+    one = G == 1
+    leaves = [t.cuda().requires_grad_(True) for t in (x, *((w[0] if one else w) for w in (wg, wu, wd)))]
+    s = scale.cuda().requires_grad_(True) if scaled else None
+    y = mx.expert_ffn(*leaves, None if one else ends.cuda(), row_scale=s)
+    _near(y, ref[0], Y_TOL)
+    grads = torch.autograd.grad(y, leaves + ([s] if scaled else []), dy.cuda())
+    for got, want in zip(grads, ref[1:]):
+        assert got.shape == (want[0] if one and want.dim() == 3 else want).shape
+        _near(got, want[0] if one and want.dim() == 3 else want, GRAD_TOL)
+
+
+@gpu
+def test_expert_ffn_gradient_against_differences():
+    """Along a direction of the (already quantised) weights of the down projection, in which y is linear, and of the
+    scale, in which it is too while no activation's code changes (powers of two)."""
+    from moonep_b200.ops import mx
+    gen = _gen(14)
+    rows, H, Hp = 192, 256, 128
+    x = torch.randn(rows, H, generator=gen).bfloat16().cuda()
+    wg, wu = ((torch.randn(H, Hp, generator=gen) * H ** -0.5).bfloat16().cuda() for _ in range(2))
+    dy = torch.randn(rows, H, generator=gen).bfloat16().cuda()
+    wd = mx.quantize(torch.randn(H, Hp, generator=gen).cuda()).dequantize().requires_grad_(True)
+    y = mx.expert_ffn(x, wg, wu, wd)
+    g, = torch.autograd.grad(y, wd, dy)
+    # twice the weights of every second output column: still values of the format
+    v = torch.zeros_like(wd)
+    v[::2] = wd.detach()[::2]
+    diff = ((mx.expert_ffn(x, wg, wu, wd.detach() + v).double() - y.double()) * dy.double()).sum()
+    along = (g.double() * v.double()).sum()
+    # both sums have terms of either sign: compared with their sizes' sum over sqrt of their number
+    size = ((y.double() * dy.double()) ** 2).sum().sqrt() + ((g.double() * v.double()) ** 2).sum().sqrt()
+    assert float((diff - along).abs()) <= 8 * HALF * float(size), (float(diff), float(along))
+    scale = torch.ones(rows, device="cuda", requires_grad=True)
+    y = mx.expert_ffn(x, wg, wu, wd.detach(), row_scale=scale)
+    g, = torch.autograd.grad(y, scale, dy)
+    two = mx.expert_ffn(x, wg, wu, wd.detach(), row_scale=torch.full_like(scale, 2.0).detach())
+    assert torch.equal(two, y.detach() * 2)          # y's slope along its scale is y itself ...
+    d = ((two.double() - y.double()) * dy.double()).sum(1)
+    # ... of the quantised activation; the straight-through gradient has the activation before, off by an eighth at most
+    # of each value (half a step of 1 in [4, 6), of 0.5 in [2, 4); less in the mean), over sqrt(H') independent terms
+    assert float((d - g.double()).norm() / d.norm()) < 0.25
+
+
+@gpu
+def test_expert_ffn_packed_weights():
+    from moonep_b200.ops import mx
+    gen = _gen(15)
+    sizes, H, Hp = [64, 128, 0], 256, 96
+    ends = _ends(sizes).cuda()
+    x = torch.randn(192 + 40, H, generator=gen).bfloat16().cuda()
+    wg, wu, wd = ((torch.randn(3, H, Hp, generator=gen) * 0.1).bfloat16().cuda() for _ in range(3))
+    dy = torch.randn(232, H, generator=gen).bfloat16().cuda()
+    xs = [x.clone().requires_grad_(True) for _ in range(2)]
+    ys = [mx.expert_ffn(xs[0], wg, wu, wd, ends), mx.expert_ffn(xs[1], mx.pack_gate_up(wg, wu), None, mx.quantize(wd), ends)]
+    gs = [torch.autograd.grad(y, v, dy)[0] for y, v in zip(ys, xs)]
+    assert torch.equal(ys[0], ys[1]) and torch.equal(gs[0], gs[1])
+    assert (ys[0][192:] == 0).all() and (gs[0][192:] == 0).all()      # rows of no group
+    assert float(gs[0][:192].float().abs().sum()) > 0
+
+
+@gpu
+def test_expert_ffn_captured():
+    """One token, and a training step, captured and replayed on new inputs."""
+    from moonep_b200.ops import mx
+    from moonep_b200.utils.graph import GraphedStep
+    gen = _gen(16)
+    H, Hp = 256, 128
+    wg, wu, wd = ((torch.randn(4, H, Hp, generator=gen) * 0.1).bfloat16().cuda() for _ in range(3))
+    packed = mx.pack_gate_up(wg, wu), None, mx.quantize(wd)
+
+    def serve(x, ends):
+        with torch.no_grad():
+            return mx.expert_ffn(x, *packed, ends)
+
+    def train(x, ends, dy):
+        leaves = [t.detach().requires_grad_(True) for t in (x, wg, wu, wd)]
+        y = mx.expert_ffn(*leaves, ends)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    new = lambda rows: torch.randn(rows, H, generator=gen).bfloat16().cuda()
+    e1 = [torch.tensor(e, dtype=torch.int32, device="cuda") for e in ([0, 0, 1, 1], [1, 1, 1, 1])]
+    step = GraphedStep(serve, [new(1), e1[0]])
+    for e in e1:
+        x = new(1)
+        assert torch.equal(step(x, e), serve(x, e))
+    e2 = [torch.tensor(e, dtype=torch.int32, device="cuda") for e in ([64, 64, 192, 256], [0, 128, 192, 256])]
+    step = GraphedStep(train, [new(256), e2[0], new(256)])
+    for e in e2:
+        x, dy = new(256), new(256)
+        for a, b in zip(step(x, e, dy), train(x, e, dy)):
+            assert torch.equal(a, b)
+
+
+# ---- refusals ----------------------------------------------------------------------------------
+@gpu
+def test_refusals():
+    from moonep_b200.ops import mx
+    bf = dict(device="cuda", dtype=torch.bfloat16)
+    x, w = torch.randn(8, 64, **bf), torch.randn(2, 32, 64, **bf)
+    q, qw, ends = mx.quantize(x), mx.quantize(w), torch.tensor([4, 8], dtype=torch.int32, device="cuda")
+    gu = mx.pack_gate_up(torch.randn(2, 64, 32, **bf), torch.randn(2, 64, 32, **bf))
+    n = torch.tensor([3], dtype=torch.int32, device="cuda")
+    bad = [
+        lambda: mx.quantize(x.cpu()),
+        lambda: mx.quantize(x.double()),
+        lambda: mx.quantize(x.t()),
+        lambda: mx.quantize(x[0]),
+        lambda: mx.quantize(x, axis=0),
+        lambda: mx.quantize(x[:, :0]),
+        lambda: mx.quantize(x[:0], axis=-2),
+        lambda: mx.quantize(w, rows_ptr=n),
+        lambda: mx.quantize(x, rows_ptr=n.long()),
+        lambda: mx.pack_gate_up(w, w[:, :, :32]),
+        lambda: mx.pack_gate_up(w, w.float()),
+        lambda: qw.dequantize(torch.float16),
+        lambda: mx.MxTensor(q.codes, q.scales[:1].contiguous(), q.shape),
+        lambda: mx.MxTensor(q.codes, q.scales, (8, 96)),
+        lambda: mx.matmul(x, qw, ends),
+        lambda: mx.matmul(q, qw),
+        lambda: mx.matmul(q, qw, ends.long()),
+        lambda: mx.matmul(q, qw, ends[:1]),
+        lambda: mx.matmul(q, qw, ends.cpu()),
+        lambda: mx.matmul(q, gu, ends),
+        lambda: mx.matmul(qw, qw, ends),
+        lambda: mx.matmul(q, mx.quantize(torch.randn(2, 32, 96, **bf)), ends),
+        lambda: mx.matmul(q, qw, ends, out=torch.empty(8, 31, **bf)),
+        lambda: mx.matmul(q, qw, ends, out=torch.empty(7, 32, **bf)),
+        lambda: mx.matmul(q, qw, ends, out=torch.empty(8, 32, device="cuda")),
+        lambda: mx.matmul(q, qw, ends, out=torch.empty(1, 32, **bf).expand(8, 32)),
+        lambda: mx.matmul(q, qw, ends, pads=torch.zeros(1, 2, dtype=torch.int32, device="cuda")),
+        lambda: mx.gateup_swiglu(q, qw, ends),
+        lambda: mx.gateup_swiglu(q, gu, ends, row_scale=torch.ones(7, device="cuda")),
+        lambda: mx.gateup_swiglu(q, gu, ends, row_scale=torch.ones(8, **bf)),
+        lambda: mx.expert_ffn(x.float(), w, w, w, ends),
+        lambda: mx.expert_ffn(x, w, w, w, ends),
+        lambda: mx.expert_ffn(x, gu, w, qw, ends),
+        lambda: mx.expert_ffn(x, gu, None, qw, ends),
+        lambda: mx.expert_ffn(x.requires_grad_(True), *(torch.randn(2, 64, 32, **bf) for _ in range(3)), ends),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(AssertionError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+
+
+def test_refusals_without_a_gpu():
+    from moonep_b200.ops import mx
+    with pytest.raises(AssertionError, match="CUDA"):
+        mx.quantize(torch.randn(4, 32))
+    with pytest.raises(AssertionError, match="CUDA"):
+        mx.pack_gate_up(torch.randn(1, 4, 32), torch.randn(1, 4, 32))
+    with pytest.raises(AssertionError):
+        mx.MxTensor(torch.zeros(4, 16, dtype=torch.uint8), torch.zeros(1, 1, 512, dtype=torch.uint8), (4, 32))
