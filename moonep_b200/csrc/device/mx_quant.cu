@@ -44,120 +44,120 @@ __device__ __forceinline__ void mx_store_scales(const MxQuantParams& p, int mat,
   *reinterpret_cast<uint32_t*>(p.scales + copy * p.row_atoms * p.k_atoms * MX_ATOM_BYTES + mx_scale_offset(r - 32 * s, ka, p.k_atoms)) = w;
 }
 
+// Raw elements are loaded first, all of a thread's, and converted when they are there: a load beside its use in one guarded
+// block made a chain of load latencies (the kernel along the columns: 925 us for 32 x 7168 x 2048 in bf16, 4.2x).
+template <class T> struct MxVec;          // eight elements
+template <class T> __device__ __forceinline__ void mx_unpack(const MxVec<T>& v, float* f) {
+  const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = mx_float(e[i]);
+}
+template <> struct MxVec<__nv_bfloat16> { uint4 q[1]; };
+template <> struct MxVec<__half> { uint4 q[1]; };
+template <> struct MxVec<float> { uint4 q[2]; };
+
 // Eight elements of a row from column c on; behind the row's end zeros.
 template <class T, bool VEC>
-__device__ __forceinline__ void mx_load8(const T* row, int c, int cols, float* v) {
-  if constexpr (VEC) {
-    if (c < cols) {               // (cols is a multiple of 8)
-      uint4 q[sizeof(T) / 2];
+__device__ __forceinline__ MxVec<T> mx_load8(const T* row, int c, int cols) {
+  MxVec<T> v;
+  if constexpr (VEC) {                    // (cols is a multiple of 8)
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) q[i] = __ldcs(reinterpret_cast<const uint4*>(row + c) + i);
-      const T* e = reinterpret_cast<const T*>(q);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = mx_float(e[i]);
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+      v.q[i] = c < cols ? __ldcs(reinterpret_cast<const uint4*>(row + c) + i) : make_uint4(0, 0, 0, 0);
   } else {
+    T* e = reinterpret_cast<T*>(&v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? mx_float(row[c + i]) : 0.f;
+    for (int i = 0; i < 8; ++i) e[i] = c + i < cols ? row[c + i] : T(0.f);
   }
+  return v;
 }
 
-// Along the rows.  A warp takes 256 elements of a row, a lane eight: four lanes share a block, sixteen the four scales
-// of an atom's row, which leave as one word.
+// Along the rows.  A warp takes MXQ_DEPTH parts of 256 elements of a row, a lane eight of each: four lanes share a
+// block, sixteen the four scales of an atom's row, which leave as one word (a phase).
 constexpr int MXQ_WARPS = 8, MXQ_DEPTH = 4;
 
 template <class T, bool VEC>
 __global__ void __launch_bounds__(MXQ_WARPS * 32) ep_mx_quant_rows_kernel(const __grid_constant__ MxQuantParams p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rows = p.rows_ptr ? max(0, min(*p.rows_ptr, p.rows)) : p.rows;
-  const int parts = (p.k_atoms + 1) / 2;
-  const long long total = (long long)p.mats * rows * parts, stride = (long long)gridDim.x * MXQ_WARPS;
-  for (long long t0 = (long long)blockIdx.x * MXQ_WARPS + warp; t0 < total; t0 += stride * MXQ_DEPTH) {
-    float v[MXQ_DEPTH][8];
-    int mat[MXQ_DEPTH], row[MXQ_DEPTH], col[MXQ_DEPTH];
+  const unsigned lines = (unsigned)p.mats * (unsigned)rows;
+  for (unsigned line = blockIdx.x * MXQ_WARPS + warp; line < lines; line += gridDim.x * MXQ_WARPS) {
+    const int mat = p.mats > 1 ? (int)(line / (unsigned)rows) : 0, row = (int)(line - (unsigned)mat * (unsigned)rows);
+    const int r = mx_out_row(row, p.interleave);
+    const T* x = (const T*)p.x + mat * p.batch + row * p.stride;
+    uint8_t* codes = p.codes + ((long long)mat * p.out_rows + r) * p.code_bytes;
+    for (int c0 = blockIdx.y * 256 * MXQ_DEPTH; c0 < p.cols; c0 += gridDim.y * 256 * MXQ_DEPTH) {
+      MxVec<T> raw[MXQ_DEPTH];
 #pragma unroll
-    for (int i = 0; i < MXQ_DEPTH; ++i) {
-      const long long t = t0 + i * stride;
-      if (t >= total) break;
-      const long long line = t / parts;
-      col[i] = (int)(t - line * parts) * 256 + lane * 8;
-      mat[i] = (int)(line / rows);
-      row[i] = (int)(line - (long long)mat[i] * rows);
-      mx_load8<T, VEC>((const T*)p.x + mat[i] * p.batch + row[i] * p.stride, col[i], p.cols, v[i]);
-    }
+      for (int i = 0; i < MXQ_DEPTH; ++i) raw[i] = mx_load8<T, VEC>(x, c0 + i * 256 + lane * 8, p.cols);
 #pragma unroll
-    for (int i = 0; i < MXQ_DEPTH; ++i) {
-      if (t0 + i * stride >= total) break;
-      uint32_t a = 0u;
+      for (int i = 0; i < MXQ_DEPTH; ++i) {
+        if (c0 + i * 256 >= p.cols) break;          // (the same for the whole warp)
+        const int c = c0 + i * 256 + lane * 8;
+        float v[8];
+        mx_unpack<T>(raw[i], v);
+        uint32_t a = 0u;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) a = max(a, mx_abs(v[i][e]));
-      a = max(a, __shfl_xor_sync(0xffffffffu, a, 1));
-      a = max(a, __shfl_xor_sync(0xffffffffu, a, 2));
-      const uint32_t b = mx_scale(a);
-      const float inv = mx_inverse(b);
-      // (a NaN scale: zeros, whatever inf * 0 would give)
+        for (int e = 0; e < 8; ++e) a = max(a, mx_abs(v[e]));
+        a = max(a, __shfl_xor_sync(0xffffffffu, a, 1));
+        a = max(a, __shfl_xor_sync(0xffffffffu, a, 2));
+        const uint32_t b = mx_scale(a);
+        const float inv = mx_inverse(b);
+        // (a NaN scale: zeros, whatever inf * 0 would give)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = b == 255u ? 0.f : v[i][e] * inv;
-      const int r = mx_out_row(row[i], p.interleave);
-      if (col[i] < 2 * p.code_bytes)
-        *reinterpret_cast<uint32_t*>(p.codes + ((long long)mat[i] * p.out_rows + r) * p.code_bytes + col[i] / 2) = mx_codes(v[i]);
-      // bytes of lanes 0, 4, 8, 12 (16, ...) to lane 0 (16)
-      uint32_t w = b | (__shfl_down_sync(0xffffffffu, b, 4) << 8);
-      w |= __shfl_down_sync(0xffffffffu, w, 8) << 16;
-      w = __shfl_sync(0xffffffffu, w, lane & 16);
-      mx_store_scales(p, mat[i], r, col[i] >> 7, lane & 15, w);
+        for (int e = 0; e < 8; ++e) v[e] *= inv;
+        const uint32_t q = b == 255u ? 0u : mx_codes(v);
+        if (c < 2 * p.code_bytes) *reinterpret_cast<uint32_t*>(codes + c / 2) = q;
+        // bytes of lanes 0, 4, 8, 12 (16, ...) to their sixteen lanes
+        uint32_t w = b | (__shfl_xor_sync(0xffffffffu, b, 4) << 8);
+        w = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 8), 0x5410);
+        w = __shfl_sync(0xffffffffu, w, lane & 16);
+        mx_store_scales(p, mat, r, c >> 7, lane & 15, w);
+      }
     }
   }
 }
 
 // Along the columns: the output is the transpose.  A block takes 256 rows x 64 columns of x, a warp one block of 32 rows,
 // a lane two columns of it; the codes of a column meet in shared memory and leave as 128-byte rows.
-constexpr int MXT_COLS = 64, MXT_ROWS = 256, MXT_PITCH = 128 + 16;
+constexpr int MXT_COLS = 64, MXT_ROWS = 256;
+
+template <class T> struct __align__(2 * sizeof(T)) MxPair { T e[2]; };
 
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256) ep_mx_quant_cols_kernel(const __grid_constant__ MxQuantParams p) {
-  __shared__ __align__(16) uint8_t s_codes[MXT_COLS * MXT_PITCH];
+  __shared__ __align__(16) uint8_t s_codes[MXT_COLS * 128];
   __shared__ __align__(4) uint8_t s_scale[MXT_COLS][8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r0 = blockIdx.y * MXT_ROWS, c0 = blockIdx.x * MXT_COLS;
   for (int m = blockIdx.z; m < p.mats; m += gridDim.z) {
-    const T* x = (const T*)p.x + m * p.batch;
-    const int c = c0 + 2 * lane;
-    float v[2][MX_BLOCK];
-    uint32_t a[2] = {0u, 0u};
+    const int c = c0 + 2 * lane, rw = r0 + warp * MX_BLOCK;
+    const T* x = (const T*)p.x + m * p.batch + (long long)rw * p.stride + c;
+    MxPair<T> raw[MX_BLOCK];
 #pragma unroll
     for (int i = 0; i < MX_BLOCK; ++i) {
-      const int r = r0 + warp * MX_BLOCK + i;
-      v[0][i] = v[1][i] = 0.f;
-      if (r < p.rows) {
-        const T* e = x + (long long)r * p.stride + c;
-        if constexpr (VEC) {           // (an even number of columns)
-          if (c < p.cols) {
-            struct __align__(2 * sizeof(T)) Pair { T a, b; };
-            const Pair q = *reinterpret_cast<const Pair*>(e);
-            v[0][i] = mx_float(q.a);
-            v[1][i] = mx_float(q.b);
-          }
-        } else {
-          if (c < p.cols) v[0][i] = mx_float(e[0]);
-          if (c + 1 < p.cols) v[1][i] = mx_float(e[1]);
-        }
+      const T* e = x + i * p.stride;
+      if constexpr (VEC) {             // (an even number of columns)
+        raw[i] = rw + i < p.rows && c < p.cols ? *reinterpret_cast<const MxPair<T>*>(e) : MxPair<T>{T(0.f), T(0.f)};
+      } else {
+        raw[i].e[0] = rw + i < p.rows && c < p.cols ? e[0] : T(0.f);
+        raw[i].e[1] = rw + i < p.rows && c + 1 < p.cols ? e[1] : T(0.f);
       }
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
+      uint32_t a = 0u;
+      float v[MX_BLOCK];
 #pragma unroll
-      for (int i = 0; i < MX_BLOCK; ++i) a[h] = max(a[h], mx_abs(v[h][i]));
-      const uint32_t b = mx_scale(a[h]);
+      for (int i = 0; i < MX_BLOCK; ++i) { v[i] = mx_float(raw[i].e[h]); a = max(a, mx_abs(v[i])); }
+      const uint32_t b = mx_scale(a);
       const float inv = mx_inverse(b);
 #pragma unroll
-      for (int i = 0; i < MX_BLOCK; ++i) v[h][i] = b == 255u ? 0.f : v[h][i] * inv;
-      uint4 q;
-      q.x = mx_codes(v[h]); q.y = mx_codes(v[h] + 8); q.z = mx_codes(v[h] + 16); q.w = mx_codes(v[h] + 24);
-      *reinterpret_cast<uint4*>(s_codes + (2 * lane + h) * MXT_PITCH + warp * 16) = q;
+      for (int i = 0; i < MX_BLOCK; ++i) v[i] *= inv;
+      uint4 q = make_uint4(0, 0, 0, 0);
+      if (b != 255u) { q.x = mx_codes(v); q.y = mx_codes(v + 8); q.z = mx_codes(v + 16); q.w = mx_codes(v + 24); }
+      // (16-byte pieces of a row in an order by column: neighbouring lanes' fall into different banks)
+      *reinterpret_cast<uint4*>(s_codes + (2 * lane + h) * 128 + (warp ^ (lane & 7)) * 16) = q;
       s_scale[2 * lane + h][warp] = (uint8_t)b;
     }
     __syncthreads();
@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(256) ep_mx_quant_cols_kernel(const __grid_cons
       const int n = i >> 3, k = r0 / 2 + (i & 7) * 16;
       if (c0 + n < p.cols && k < p.code_bytes)
         *reinterpret_cast<uint4*>(p.codes + ((long long)m * p.out_rows + mx_out_row(c0 + n, p.interleave)) * p.code_bytes + k) =
-            *reinterpret_cast<const uint4*>(s_codes + n * MXT_PITCH + (i & 7) * 16);
+            *reinterpret_cast<const uint4*>(s_codes + n * 128 + ((i & 7) ^ (n >> 1 & 7)) * 16);
     }
     for (int i = threadIdx.x; i < 2 * MXT_COLS * p.phases; i += 256) {
       const int n = (i >> 1) % MXT_COLS, h = i & 1;
@@ -187,57 +187,61 @@ struct MxDequantParams {
   int interleave;
 };
 
-// A lane takes eight values of a row, a warp 256.  (Exact in bf16 but for what a bf16 subnormal rounds, fp32 always.)
+// A lane takes eight values of a row, a warp MXD_DEPTH times 256.  (Exact in bf16 but for what a bf16 subnormal rounds,
+// fp32 always.)
+constexpr int MXD_DEPTH = 8;
+
 template <class T, bool VEC>
 __global__ void __launch_bounds__(MXQ_WARPS * 32) ep_mx_dequant_kernel(const __grid_constant__ MxDequantParams p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rows = p.rows_ptr ? max(0, min(*p.rows_ptr, p.rows)) : p.rows;
-  const int parts = (p.cols + 255) / 256;
-  const long long total = (long long)p.mats * rows * parts, stride = (long long)gridDim.x * MXQ_WARPS;
-  for (long long t0 = (long long)blockIdx.x * MXQ_WARPS + warp; t0 < total; t0 += stride * MXQ_DEPTH) {
-    uint32_t code[MXQ_DEPTH], b[MXQ_DEPTH];
-    T* dst[MXQ_DEPTH];
-    int col[MXQ_DEPTH];
+  const unsigned lines = (unsigned)p.mats * (unsigned)rows;
+  for (unsigned line = blockIdx.x * MXQ_WARPS + warp; line < lines; line += gridDim.x * MXQ_WARPS) {
+    const int mat = p.mats > 1 ? (int)(line / (unsigned)rows) : 0, row = (int)(line - (unsigned)mat * (unsigned)rows);
+    const int r = mx_out_row(row, p.interleave);
+    const uint8_t* codes = p.codes + ((long long)mat * p.in_rows + r) * p.code_bytes;
+    const uint8_t* scales = p.scales + (long long)mat * p.row_atoms * p.k_atoms * MX_ATOM_BYTES + mx_scale_offset(r, 0, p.k_atoms);
+    T* out = (T*)p.out + ((long long)mat * p.rows + row) * p.cols;
+    for (int c0 = blockIdx.y * 256 * MXD_DEPTH + lane * 8; c0 < p.cols; c0 += gridDim.y * 256 * MXD_DEPTH) {
+      uint32_t code[MXD_DEPTH], b[MXD_DEPTH];
 #pragma unroll
-    for (int i = 0; i < MXQ_DEPTH; ++i) {
-      const long long t = t0 + i * stride;
-      if (t >= total) break;
-      const long long line = t / parts;
-      const int c = (int)(t - line * parts) * 256 + lane * 8;
-      const int mat = (int)(line / rows), row = (int)(line - (long long)mat * rows), r = mx_out_row(row, p.interleave);
-      col[i] = c;
-      dst[i] = (T*)p.out + ((long long)mat * p.rows + row) * p.cols + c;
-      if (c < p.cols) {
-        code[i] = __ldcs(reinterpret_cast<const uint32_t*>(p.codes + ((long long)mat * p.in_rows + r) * p.code_bytes + c / 2));
-        b[i] = p.scales[(long long)mat * p.row_atoms * p.k_atoms * MX_ATOM_BYTES + mx_scale_offset(r, c >> 7, p.k_atoms) + ((c >> 5) & 3)];
+      for (int i = 0; i < MXD_DEPTH; ++i) {
+        const int c = c0 + i * 256;
+        code[i] = c < p.cols ? __ldcs(reinterpret_cast<const uint32_t*>(codes + c / 2)) : 0u;
+        b[i] = c < p.cols ? scales[(long long)(c >> 7) * MX_ATOM_BYTES + (c >> 5 & 3)] : 0u;
       }
-    }
 #pragma unroll
-    for (int i = 0; i < MXQ_DEPTH; ++i) {
-      if (t0 + i * stride >= total) break;
-      if (col[i] >= p.cols) continue;
-      const float s = mx_value(b[i]);
-      __align__(16) T v[8];
+      for (int i = 0; i < MXD_DEPTH; ++i) {
+        const int c = c0 + i * 256;
+        if (c >= p.cols) break;
+        const float s = mx_value(b[i]);
+        __align__(16) T v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float f = mx_element(code[i] >> (4 * e)) * s;
-        if constexpr (sizeof(T) == 2) v[e] = __float2bfloat16(f);
-        else v[e] = f;
-      }
-      if constexpr (VEC) {
+        for (int e = 0; e < 8; ++e) {
+          const float f = mx_element(code[i] >> (4 * e)) * s;
+          if constexpr (sizeof(T) == 2) v[e] = __float2bfloat16(f);
+          else v[e] = f;
+        }
+        if constexpr (VEC) {
 #pragma unroll
-        for (int q = 0; q < (int)sizeof(T) / 2; ++q) __stcs(reinterpret_cast<uint4*>(dst[i]) + q, reinterpret_cast<const uint4*>(v)[q]);
-      } else {
+          for (int q = 0; q < (int)sizeof(T) / 2; ++q) __stcs(reinterpret_cast<uint4*>(out + c) + q, reinterpret_cast<const uint4*>(v)[q]);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) if (col[i] + e < p.cols) dst[i][e] = v[e];
+          for (int e = 0; e < 8; ++e) if (c + e < p.cols) out[c + e] = v[e];
+        }
       }
     }
   }
 }
 
-static int mx_blocks(long long tasks) {
-  const long long blocks = (tasks + MXQ_WARPS - 1) / MXQ_WARPS, most = 148 * 8;
-  return (int)(blocks < most ? blocks : most);
+// Blocks for so many rows (one a warp) of so many parts: enough for a few rounds of the device, columns shared out only
+// where the rows are too few for that.
+static dim3 mx_grid(long long lines, int parts) {
+  const long long most = 148 * 16;
+  const long long x = (lines + MXQ_WARPS - 1) / MXQ_WARPS;
+  long long y = x >= most ? 1 : most / x;
+  if (y > parts) y = parts;
+  return dim3((unsigned)(x < most ? x : most), (unsigned)y);
 }
 
 template <class T>
@@ -251,9 +255,9 @@ static int mx_quant(const MxQuantParams& p, bool along_cols, cudaStream_t stream
     if (pairs) ep_mx_quant_cols_kernel<T, true><<<grid, 256, 0, stream>>>(p);
     else ep_mx_quant_cols_kernel<T, false><<<grid, 256, 0, stream>>>(p);
   } else {
-    const int blocks = mx_blocks((long long)p.mats * p.rows * ((p.k_atoms + 1) / 2));
-    if (rows16) ep_mx_quant_rows_kernel<T, true><<<blocks, MXQ_WARPS * 32, 0, stream>>>(p);
-    else ep_mx_quant_rows_kernel<T, false><<<blocks, MXQ_WARPS * 32, 0, stream>>>(p);
+    const dim3 grid = mx_grid((long long)p.mats * p.rows, (p.k_atoms * MX_ATOM_K + 256 * MXQ_DEPTH - 1) / (256 * MXQ_DEPTH));
+    if (rows16) ep_mx_quant_rows_kernel<T, true><<<grid, MXQ_WARPS * 32, 0, stream>>>(p);
+    else ep_mx_quant_rows_kernel<T, false><<<grid, MXQ_WARPS * 32, 0, stream>>>(p);
   }
   MEP_CUDA_OK(cudaGetLastError());
   return 0;
@@ -270,7 +274,8 @@ extern "C" {
 // phases = 4 (one matrix): scales for token rows, else 1.
 int mep_mx_quantize(const void* x, int type, int64_t batch, int64_t stride, int mats, int rows, int cols, int along_cols,
                     int interleave, int out_rows, int phases, const int32_t* rows_ptr, void* codes, void* scales, cudaStream_t stream) {
-  if (mats < 0 || rows < 0 || cols < 0) return fail(-1, "mx quantise: %d x %d x %d elements", mats, rows, cols);
+  if (mats < 0 || rows < 0 || cols < 0 || cols > 0x7F000000 || (int64_t)mats * rows > 0x7FFFFFFF)
+    return fail(-1, "mx quantise: %d x %d x %d elements", mats, rows, cols);
   if (along_cols && rows_ptr) return fail(-2, "mx quantise: a device row count goes with blocks along the rows");
   if (phases != 1 && (phases != MX_PHASES || mats > 1)) return fail(-4, "mx quantise: %d phases of %d matrices", phases, mats);
   if (mats == 0 || rows == 0 || cols == 0) return 0;
@@ -289,21 +294,22 @@ int mep_mx_quantize(const void* x, int type, int64_t batch, int64_t stride, int 
 // The values [mats][rows][cols] in bf16, or fp32.
 int mep_mx_dequantize(const void* codes, const void* scales, int mats, int rows, int cols, int interleave, int in_rows,
                       const int32_t* rows_ptr, int fp32, void* out, cudaStream_t stream) {
-  if (mats < 0 || rows < 0 || cols < 0) return fail(-1, "mx dequantise: %d x %d x %d elements", mats, rows, cols);
+  if (mats < 0 || rows < 0 || cols < 0 || cols > 0x7F000000 || (int64_t)mats * rows > 0x7FFFFFFF)
+    return fail(-1, "mx dequantise: %d x %d x %d elements", mats, rows, cols);
   if (mats == 0 || rows == 0 || cols == 0) return 0;
   MxDequantParams p;
   p.codes = (const uint8_t*)codes; p.scales = (const uint8_t*)scales; p.mats = mats; p.rows = rows; p.cols = cols;
   p.in_rows = in_rows; p.code_bytes = (cols + MX_BLOCK - 1) / MX_BLOCK * (MX_BLOCK / 2);
   p.k_atoms = mx_atoms(cols); p.row_atoms = mx_atoms(in_rows);
   p.out = out; p.rows_ptr = rows_ptr; p.interleave = interleave;
-  const int blocks = mx_blocks((long long)mats * rows * ((cols + 255) / 256));
+  const dim3 grid = mx_grid((long long)mats * rows, (cols + 256 * MXD_DEPTH - 1) / (256 * MXD_DEPTH));
   const bool vec = cols % 8 == 0 && (uintptr_t)out % 16 == 0;
   if (fp32) {
-    if (vec) ep_mx_dequant_kernel<float, true><<<blocks, MXQ_WARPS * 32, 0, stream>>>(p);
-    else ep_mx_dequant_kernel<float, false><<<blocks, MXQ_WARPS * 32, 0, stream>>>(p);
+    if (vec) ep_mx_dequant_kernel<float, true><<<grid, MXQ_WARPS * 32, 0, stream>>>(p);
+    else ep_mx_dequant_kernel<float, false><<<grid, MXQ_WARPS * 32, 0, stream>>>(p);
   } else {
-    if (vec) ep_mx_dequant_kernel<__nv_bfloat16, true><<<blocks, MXQ_WARPS * 32, 0, stream>>>(p);
-    else ep_mx_dequant_kernel<__nv_bfloat16, false><<<blocks, MXQ_WARPS * 32, 0, stream>>>(p);
+    if (vec) ep_mx_dequant_kernel<__nv_bfloat16, true><<<grid, MXQ_WARPS * 32, 0, stream>>>(p);
+    else ep_mx_dequant_kernel<__nv_bfloat16, false><<<grid, MXQ_WARPS * 32, 0, stream>>>(p);
   }
   MEP_CUDA_OK(cudaGetLastError());
   return 0;
