@@ -14,10 +14,40 @@ namespace mep {
 
 enum { MX_BF16 = 0, MX_FP16 = 1, MX_FP32 = 2 };
 
-__device__ __forceinline__ float mx_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float mx_float(__half x) { return __half2float(x); }
-__device__ __forceinline__ float mx_float(float x) { return x; }
 __device__ __forceinline__ uint32_t mx_abs(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+
+// Two neighbouring elements as they are stored: largest magnitudes of either side, and products with a power of two per
+// side, in as few instructions as their type allows (magnitudes of 16 bits compare like integers, two at once; a bf16
+// times a power of two is a bf16, exactly).
+template <class T> struct __align__(2 * sizeof(T)) MxPair { T e[2]; };
+template <class T> struct MxMax;         // largest magnitudes so far of the left and the right elements
+template <> struct MxMax<float> {
+  uint32_t a = 0u, b = 0u;
+  __device__ __forceinline__ void add(const MxPair<float>& x) { a = max(a, mx_abs(x.e[0])); b = max(b, mx_abs(x.e[1])); }
+  __device__ __forceinline__ uint32_t left() const { return a; }
+  __device__ __forceinline__ uint32_t right() const { return b; }
+};
+template <class T> struct MxMax16 {
+  uint32_t m = 0u;
+  __device__ __forceinline__ void add(const MxPair<T>& x) { m = __vmaxu2(m, *reinterpret_cast<const uint32_t*>(&x) & 0x7FFF7FFFu); }
+};
+template <> struct MxMax<__nv_bfloat16> : MxMax16<__nv_bfloat16> {
+  __device__ __forceinline__ uint32_t left() const { return m << 16; }
+  __device__ __forceinline__ uint32_t right() const { return m & 0xFFFF0000u; }
+};
+template <> struct MxMax<__half> : MxMax16<__half> {
+  __device__ __forceinline__ uint32_t left() const { return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m))); }
+  __device__ __forceinline__ uint32_t right() const { return __float_as_uint(__half2float(__ushort_as_half((unsigned short)(m >> 16)))); }
+};
+__device__ __forceinline__ float2 mx_times(const MxPair<float>& x, float s, float t) { return make_float2(x.e[0] * s, x.e[1] * t); }
+__device__ __forceinline__ float2 mx_times(const MxPair<__half>& x, float s, float t) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x));
+  return make_float2(f.x * s, f.y * t);
+}
+__device__ __forceinline__ float2 mx_times(const MxPair<__nv_bfloat16>& x, float s, float t) {
+  const __nv_bfloat162 k = __floats2bfloat162_rn(s, t), y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x), k);
+  return __bfloat1622float2(y);
+}
 
 // Where row r of the output goes: as it is, or as gate (1) / up (2) column of the packed pair, sixteen of either in turn.
 __device__ __forceinline__ int mx_out_row(int r, int interleave) {
@@ -37,37 +67,29 @@ struct MxQuantParams {
   int phases;                   // 4: token rows, whose scales are stored at four phases
 };
 
-// Four scales of row r, once a phase: thread `s` of each group of `phases` stores them.
-__device__ __forceinline__ void mx_store_scales(const MxQuantParams& p, int mat, int r, int ka, int s, uint32_t w) {
-  if (s >= p.phases || r < 32 * s || ka >= p.k_atoms) return;
+// Where the first four scales of row r are in phase s, the next ones 512 bytes further each; null where there is no such copy.
+__device__ __forceinline__ uint32_t* mx_scale_row(const MxQuantParams& p, int mat, int r, int s) {
+  if (s >= p.phases || r < 32 * s) return nullptr;
   const long long copy = p.phases == 1 ? mat : s;
-  *reinterpret_cast<uint32_t*>(p.scales + copy * p.row_atoms * p.k_atoms * MX_ATOM_BYTES + mx_scale_offset(r - 32 * s, ka, p.k_atoms)) = w;
+  return reinterpret_cast<uint32_t*>(p.scales + copy * p.row_atoms * p.k_atoms * MX_ATOM_BYTES + mx_scale_offset(r - 32 * s, 0, p.k_atoms));
 }
 
 // Raw elements are loaded first, all of a thread's, and converted when they are there: a load beside its use in one guarded
 // block made a chain of load latencies (the kernel along the columns: 925 us for 32 x 7168 x 2048 in bf16, 4.2x).
-template <class T> struct MxVec;          // eight elements
-template <class T> __device__ __forceinline__ void mx_unpack(const MxVec<T>& v, float* f) {
-  const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = mx_float(e[i]);
-}
-template <> struct MxVec<__nv_bfloat16> { uint4 q[1]; };
-template <> struct MxVec<__half> { uint4 q[1]; };
-template <> struct MxVec<float> { uint4 q[2]; };
+template <class T> struct __align__(16) MxEight { MxPair<T> p[4]; };
 
 // Eight elements of a row from column c on; behind the row's end zeros.
 template <class T, bool VEC>
-__device__ __forceinline__ MxVec<T> mx_load8(const T* row, int c, int cols) {
-  MxVec<T> v;
+__device__ __forceinline__ MxEight<T> mx_load8(const T* row, int c, int cols) {
+  MxEight<T> v;
   if constexpr (VEC) {                    // (cols is a multiple of 8)
+    uint4* q = reinterpret_cast<uint4*>(&v);
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-      v.q[i] = c < cols ? __ldcs(reinterpret_cast<const uint4*>(row + c) + i) : make_uint4(0, 0, 0, 0);
+      q[i] = c < cols ? __ldcs(reinterpret_cast<const uint4*>(row + c) + i) : make_uint4(0, 0, 0, 0);
   } else {
-    T* e = reinterpret_cast<T*>(&v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = c + i < cols ? row[c + i] : T(0.f);
+    for (int i = 0; i < 8; ++i) v.p[i / 2].e[i % 2] = c + i < cols ? row[c + i] : T(0.f);
   }
   return v;
 }
@@ -86,92 +108,106 @@ __global__ void __launch_bounds__(MXQ_WARPS * 32) ep_mx_quant_rows_kernel(const 
     const int r = mx_out_row(row, p.interleave);
     const T* x = (const T*)p.x + mat * p.batch + row * p.stride;
     uint8_t* codes = p.codes + ((long long)mat * p.out_rows + r) * p.code_bytes;
+    uint32_t* scales = mx_scale_row(p, mat, r, lane & 15);       // of this lane's phase, if it has one
     for (int c0 = blockIdx.y * 256 * MXQ_DEPTH; c0 < p.cols; c0 += gridDim.y * 256 * MXQ_DEPTH) {
-      MxVec<T> raw[MXQ_DEPTH];
+      MxEight<T> raw[MXQ_DEPTH];
 #pragma unroll
       for (int i = 0; i < MXQ_DEPTH; ++i) raw[i] = mx_load8<T, VEC>(x, c0 + i * 256 + lane * 8, p.cols);
 #pragma unroll
       for (int i = 0; i < MXQ_DEPTH; ++i) {
         if (c0 + i * 256 >= p.cols) break;          // (the same for the whole warp)
         const int c = c0 + i * 256 + lane * 8;
-        float v[8];
-        mx_unpack<T>(raw[i], v);
-        uint32_t a = 0u;
+        MxMax<T> m;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) a = max(a, mx_abs(v[e]));
+        for (int e = 0; e < 4; ++e) m.add(raw[i].p[e]);
+        uint32_t a = max(m.left(), m.right());
         a = max(a, __shfl_xor_sync(0xffffffffu, a, 1));
         a = max(a, __shfl_xor_sync(0xffffffffu, a, 2));
         const uint32_t b = mx_scale(a);
         const float inv = mx_inverse(b);
-        // (a NaN scale: zeros, whatever inf * 0 would give)
+        float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= inv;
+        for (int e = 0; e < 4; ++e) *reinterpret_cast<float2*>(v + 2 * e) = mx_times(raw[i].p[e], inv, inv);
+        // (a NaN scale: zeros, whatever inf * 0 would give)
         const uint32_t q = b == 255u ? 0u : mx_codes(v);
         if (c < 2 * p.code_bytes) *reinterpret_cast<uint32_t*>(codes + c / 2) = q;
         // bytes of lanes 0, 4, 8, 12 (16, ...) to their sixteen lanes
         uint32_t w = b | (__shfl_xor_sync(0xffffffffu, b, 4) << 8);
         w = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 8), 0x5410);
         w = __shfl_sync(0xffffffffu, w, lane & 16);
-        mx_store_scales(p, mat, r, c >> 7, lane & 15, w);
+        if (scales != nullptr && c < p.k_atoms * MX_ATOM_K) scales[(long long)(c >> 7) * (MX_ATOM_BYTES / 4)] = w;
       }
     }
   }
 }
 
-// Along the columns: the output is the transpose.  A block takes 256 rows x 64 columns of x, a warp one block of 32 rows,
-// a lane two columns of it; the codes of a column meet in shared memory and leave as 128-byte rows.
-constexpr int MXT_COLS = 64, MXT_ROWS = 256;
-
-template <class T> struct __align__(2 * sizeof(T)) MxPair { T e[2]; };
+// Along the columns: the output is the transpose.  A block takes 256 rows of x, a warp one block of 32 rows, a lane four
+// columns of it (two of fp32): 256-byte pieces of x's rows.  (With 128-byte pieces of bf16 rows 3.8 TB/s; 32 x 7168 x 2048
+// 314 us.)  The codes of a column meet in shared memory and leave as 128-byte rows.
+constexpr int MXT_ROWS = 256;
+template <class T> constexpr int mxt_pairs() { return sizeof(T) == 2 ? 2 : 1; }
 
 template <class T, bool VEC>
-__global__ void __launch_bounds__(256) ep_mx_quant_cols_kernel(const __grid_constant__ MxQuantParams p) {
-  __shared__ __align__(16) uint8_t s_codes[MXT_COLS * 128];
-  __shared__ __align__(4) uint8_t s_scale[MXT_COLS][8];
+__global__ void __launch_bounds__(256, 2) ep_mx_quant_cols_kernel(const __grid_constant__ MxQuantParams p) {
+  constexpr int NP = mxt_pairs<T>(), COLS = 64 * NP;
+  struct __align__(8) Piece { MxPair<T> p[NP]; };
+  __shared__ __align__(16) uint8_t s_codes[COLS * 128];
+  __shared__ __align__(4) uint8_t s_scale[COLS][8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int r0 = blockIdx.y * MXT_ROWS, c0 = blockIdx.x * MXT_COLS;
+  const int r0 = blockIdx.y * MXT_ROWS, c0 = blockIdx.x * COLS;
   for (int m = blockIdx.z; m < p.mats; m += gridDim.z) {
-    const int c = c0 + 2 * lane, rw = r0 + warp * MX_BLOCK;
+    const int c = c0 + 2 * NP * lane, rw = r0 + warp * MX_BLOCK;
     const T* x = (const T*)p.x + m * p.batch + (long long)rw * p.stride + c;
-    MxPair<T> raw[MX_BLOCK];
+    Piece raw[MX_BLOCK];
 #pragma unroll
     for (int i = 0; i < MX_BLOCK; ++i) {
       const T* e = x + i * p.stride;
-      if constexpr (VEC) {             // (an even number of columns)
-        raw[i] = rw + i < p.rows && c < p.cols ? *reinterpret_cast<const MxPair<T>*>(e) : MxPair<T>{T(0.f), T(0.f)};
+      if constexpr (VEC) {             // (the number of columns is a multiple of a lane's)
+        const uint2 q = rw + i < p.rows && c < p.cols ? __ldcs(reinterpret_cast<const uint2*>(e)) : make_uint2(0, 0);
+        raw[i] = *reinterpret_cast<const Piece*>(&q);
       } else {
-        raw[i].e[0] = rw + i < p.rows && c < p.cols ? e[0] : T(0.f);
-        raw[i].e[1] = rw + i < p.rows && c + 1 < p.cols ? e[1] : T(0.f);
+#pragma unroll
+        for (int j = 0; j < 2 * NP; ++j) raw[i].p[j / 2].e[j % 2] = rw + i < p.rows && c + j < p.cols ? e[j] : T(0.f);
       }
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t a = 0u;
-      float v[MX_BLOCK];
+    for (int h = 0; h < NP; ++h) {
+      MxMax<T> top;
 #pragma unroll
-      for (int i = 0; i < MX_BLOCK; ++i) { v[i] = mx_float(raw[i].e[h]); a = max(a, mx_abs(v[i])); }
-      const uint32_t b = mx_scale(a);
-      const float inv = mx_inverse(b);
+      for (int i = 0; i < MX_BLOCK; ++i) top.add(raw[i].p[h]);
+      const uint32_t b0 = mx_scale(top.left()), b1 = mx_scale(top.right());
+      const float inv0 = mx_inverse(b0), inv1 = mx_inverse(b1);
+      uint32_t q[2][4];
 #pragma unroll
-      for (int i = 0; i < MX_BLOCK; ++i) v[i] *= inv;
-      uint4 q = make_uint4(0, 0, 0, 0);
-      if (b != 255u) { q.x = mx_codes(v); q.y = mx_codes(v + 8); q.z = mx_codes(v + 16); q.w = mx_codes(v + 24); }
+      for (int j = 0; j < 4; ++j) {
+        float u[8], v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 f = mx_times(raw[8 * j + i].p[h], inv0, inv1);
+          u[i] = f.x; v[i] = f.y;
+        }
+        q[0][j] = b0 == 255u ? 0u : mx_codes(u);
+        q[1][j] = b1 == 255u ? 0u : mx_codes(v);
+      }
       // (16-byte pieces of a row in an order by column: neighbouring lanes' fall into different banks)
-      *reinterpret_cast<uint4*>(s_codes + (2 * lane + h) * 128 + (warp ^ (lane & 7)) * 16) = q;
-      s_scale[2 * lane + h][warp] = (uint8_t)b;
+      const int n = 2 * NP * lane + 2 * h;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<uint4*>(s_codes + (n + i) * 128 + (warp ^ (lane & 7)) * 16) = make_uint4(q[i][0], q[i][1], q[i][2], q[i][3]);
+      s_scale[n][warp] = (uint8_t)b0;
+      s_scale[n + 1][warp] = (uint8_t)b1;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < MXT_COLS * 8; i += 256) {       // 16 bytes of a column's codes
+    for (int i = threadIdx.x; i < COLS * 8; i += 256) {       // 16 bytes of a column's codes
       const int n = i >> 3, k = r0 / 2 + (i & 7) * 16;
       if (c0 + n < p.cols && k < p.code_bytes)
         *reinterpret_cast<uint4*>(p.codes + ((long long)m * p.out_rows + mx_out_row(c0 + n, p.interleave)) * p.code_bytes + k) =
-            *reinterpret_cast<const uint4*>(s_codes + n * 128 + ((i & 7) ^ (n >> 1 & 7)) * 16);
+            *reinterpret_cast<const uint4*>(s_codes + n * 128 + ((i & 7) ^ (n / (2 * NP) & 7)) * 16);
     }
-    for (int i = threadIdx.x; i < 2 * MXT_COLS * p.phases; i += 256) {
-      const int n = (i >> 1) % MXT_COLS, h = i & 1;
-      if (c0 + n < p.cols)
-        mx_store_scales(p, m, mx_out_row(c0 + n, p.interleave), r0 / MX_ATOM_K + h, i / (2 * MXT_COLS),
-                        *reinterpret_cast<const uint32_t*>(&s_scale[n][4 * h]));
+    for (int i = threadIdx.x; i < 2 * COLS * p.phases; i += 256) {
+      const int n = (i >> 1) % COLS, ka = r0 / MX_ATOM_K + (i & 1);
+      uint32_t* scales = c0 + n < p.cols && ka < p.k_atoms ? mx_scale_row(p, m, mx_out_row(c0 + n, p.interleave), i / (2 * COLS)) : nullptr;
+      if (scales != nullptr) scales[(long long)ka * (MX_ATOM_BYTES / 4)] = *reinterpret_cast<const uint32_t*>(&s_scale[n][4 * (i & 1)]);
     }
     __syncthreads();
   }
@@ -202,6 +238,29 @@ __global__ void __launch_bounds__(MXQ_WARPS * 32) ep_mx_dequant_kernel(const __g
     const uint8_t* codes = p.codes + ((long long)mat * p.in_rows + r) * p.code_bytes;
     const uint8_t* scales = p.scales + (long long)mat * p.row_atoms * p.k_atoms * MX_ATOM_BYTES + mx_scale_offset(r, 0, p.k_atoms);
     T* out = (T*)p.out + ((long long)mat * p.rows + row) * p.cols;
+    if constexpr (!VEC) {        // rows start anywhere: neighbouring lanes take neighbouring elements
+      for (int c0 = blockIdx.y * 256 * MXD_DEPTH + lane; c0 < p.cols; c0 += gridDim.y * 256 * MXD_DEPTH) {
+#pragma unroll 2
+        for (int i = 0; i < 8 * MXD_DEPTH; i += 8) {
+          uint32_t code[8], b[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int c = c0 + (i + e) * 32;
+            code[e] = c < p.cols ? codes[c >> 1] >> (4 * (c & 1)) : 0u;
+            b[e] = c < p.cols ? scales[(long long)(c >> 7) * MX_ATOM_BYTES + (c >> 5 & 3)] : 0u;
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int c = c0 + (i + e) * 32;
+            if (c >= p.cols) break;
+            const float f = mx_element(code[e]) * mx_value(b[e]);
+            if constexpr (sizeof(T) == 2) out[c] = __float2bfloat16(f);
+            else out[c] = f;
+          }
+        }
+      }
+      continue;
+    }
     for (int c0 = blockIdx.y * 256 * MXD_DEPTH + lane * 8; c0 < p.cols; c0 += gridDim.y * 256 * MXD_DEPTH) {
       uint32_t code[MXD_DEPTH], b[MXD_DEPTH];
 #pragma unroll
@@ -222,13 +281,8 @@ __global__ void __launch_bounds__(MXQ_WARPS * 32) ep_mx_dequant_kernel(const __g
           if constexpr (sizeof(T) == 2) v[e] = __float2bfloat16(f);
           else v[e] = f;
         }
-        if constexpr (VEC) {
 #pragma unroll
-          for (int q = 0; q < (int)sizeof(T) / 2; ++q) __stcs(reinterpret_cast<uint4*>(out + c) + q, reinterpret_cast<const uint4*>(v)[q]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) if (c + e < p.cols) out[c + e] = v[e];
-        }
+        for (int q = 0; q < (int)sizeof(T) / 2; ++q) __stcs(reinterpret_cast<uint4*>(out + c) + q, reinterpret_cast<const uint4*>(v)[q]);
       }
     }
   }
@@ -247,12 +301,13 @@ static dim3 mx_grid(long long lines, int parts) {
 template <class T>
 static int mx_quant(const MxQuantParams& p, bool along_cols, cudaStream_t stream) {
   const bool rows16 = (uintptr_t)p.x % 16 == 0 && (p.stride * sizeof(T)) % 16 == 0 && (p.batch * sizeof(T)) % 16 == 0 && p.cols % 8 == 0;
-  const bool pairs = (uintptr_t)p.x % (2 * sizeof(T)) == 0 && p.stride % 2 == 0 && p.batch % 2 == 0 && p.cols % 2 == 0;
+  constexpr int lane_cols = 2 * mxt_pairs<T>(), block_cols = 32 * lane_cols;
+  const bool pieces = (uintptr_t)p.x % 8 == 0 && p.stride % lane_cols == 0 && p.batch % lane_cols == 0 && p.cols % lane_cols == 0;
   if (along_cols) {
-    const dim3 grid((unsigned)((p.cols + MXT_COLS - 1) / MXT_COLS), (unsigned)((p.rows + MXT_ROWS - 1) / MXT_ROWS),
+    const dim3 grid((unsigned)((p.cols + block_cols - 1) / block_cols), (unsigned)((p.rows + MXT_ROWS - 1) / MXT_ROWS),
                     (unsigned)(p.mats < 65535 ? p.mats : 65535));
     if (grid.y > 65535) return fail(-5, "mx quantise: %d rows are too many along the last but one axis", p.rows);
-    if (pairs) ep_mx_quant_cols_kernel<T, true><<<grid, 256, 0, stream>>>(p);
+    if (pieces) ep_mx_quant_cols_kernel<T, true><<<grid, 256, 0, stream>>>(p);
     else ep_mx_quant_cols_kernel<T, false><<<grid, 256, 0, stream>>>(p);
   } else {
     const dim3 grid = mx_grid((long long)p.mats * p.rows, (p.k_atoms * MX_ATOM_K + 256 * MXQ_DEPTH - 1) / (256 * MXQ_DEPTH));
