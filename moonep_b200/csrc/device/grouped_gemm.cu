@@ -392,10 +392,15 @@ static int launch_dense_f32(const DenseParams& dp, cudaStream_t stream) {
   return 0;
 }
 
-template <int EPI>
+template <int EPI, int MAX_N>
 static int launch_mx(const MxParams& p, int grid, cudaStream_t stream) {
   static PairLaunch once;
-  return launch_pair((const void*)ep_mx_gemm_kernel<EPI>, once, p, grid, MXG_THREADS, MXG_SMEM, false, stream);
+  return launch_pair((const void*)ep_mx_gemm_kernel<EPI, MAX_N>, once, p, grid, MXG_THREADS,
+                     mxg_stages<EPI, MAX_N>() * mxg_stage(MAX_N) + 1024, false, stream);
+}
+template <int EPI>
+static int launch_mx(const MxParams& p, bool few, int grid, cudaStream_t stream) {
+  return few ? launch_mx<EPI, MXG_FEW_N>(p, grid, stream) : launch_mx<EPI, MXG_MAX_N>(p, grid, stream);
 }
 
 template <bool A_MN, int EPI, bool DISP>
@@ -610,9 +615,10 @@ int mep_mx_gemm_launch(const MxDesc* d, cudaStream_t stream) {
   int rc = 0;
   if ((rc = make_byte_map(&p.w, d->w_codes, (int64_t)d->ngroups * d->w_rows, k_bytes, 128))) return rc;
   if ((rc = make_byte_map(&p.ws, d->w_scales, (int64_t)d->ngroups * p.w_atoms, s_bytes, 0))) return rc;
-  for (int b = 0; b < 4; ++b)
-    if ((rc = make_byte_map(&p.tok[b], d->a_codes, d->rows, k_bytes, b < 3 ? 32 * (b + 1) : MXG_MAX_N / 2))) return rc;
+  for (int b = 0; b < MXG_BOXES; ++b)
+    if ((rc = make_byte_map(&p.tok[b], d->a_codes, d->rows, k_bytes, mxg_box_rows(b)))) return rc;
   if ((rc = make_byte_map(&p.ts, d->a_scales, (int64_t)MX_PHASES * p.t_atoms, s_bytes, 0))) return rc;
+  const bool few = d->rows <= MXG_FEW_N * (int64_t)d->ngroups;
   p.cu_seqlens = d->cu_seqlens; p.pads = d->pads; p.ngroups = d->ngroups; p.total_rows = d->rows; p.K = d->K; p.N = d->N;
   p.out = (__nv_bfloat16*)d->out; p.gate = (__nv_bfloat16*)d->gate; p.up = (__nv_bfloat16*)d->up;
   p.codes = (uint8_t*)d->codes; p.scales = (uint8_t*)d->scales;
@@ -624,9 +630,9 @@ int mep_mx_gemm_launch(const MxDesc* d, cudaStream_t stream) {
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (!d->gated) return launch_mx<MX_EPI_BF16>(p, sms, stream);
-  return p.gate != nullptr || p.up != nullptr ? launch_mx<MX_EPI_SWIGLU_SAVE>(p, sms, stream)
-                                              : launch_mx<MX_EPI_SWIGLU>(p, sms, stream);
+  if (!d->gated) return launch_mx<MX_EPI_BF16>(p, few, sms, stream);
+  return p.gate != nullptr || p.up != nullptr ? launch_mx<MX_EPI_SWIGLU_SAVE>(p, few, sms, stream)
+                                              : launch_mx<MX_EPI_SWIGLU>(p, few, sms, stream);
 }
 
 }  // extern "C"

@@ -29,24 +29,26 @@ namespace mep {
 
 enum { MX_EPI_BF16 = 0, MX_EPI_SWIGLU = 1, MX_EPI_SWIGLU_SAVE = 2 };
 
-constexpr int MXG_MAX_N = 224;                   // tokens of a tile
+constexpr int MXG_MAX_N = 224;                   // tokens of a tile, at most
+constexpr int MXG_FEW_N = 64;                    // the same where groups are short
 constexpr int MXG_BK = 256;                      // elements of a k-block: 128 bytes a row
-constexpr int MXG_STAGES = 5;
+constexpr int MXG_MAX_STAGES = 10;
 constexpr int MXG_W_BYTES = 128 * 128;
-constexpr int MXG_T_BYTES = MXG_MAX_N / 2 * 128;
 constexpr int MXG_S_BYTES = 2 * MX_ATOM_BYTES;   // scales of 128 rows and one k-block
-constexpr int MXG_STAGE = MXG_W_BYTES + MXG_T_BYTES + MXG_S_BYTES * 3;
 constexpr int MXG_SETS = 2;
 constexpr int MXG_THREADS = 64 + MXG_SETS * 128;
-constexpr int MXG_SMEM = MXG_STAGES * MXG_STAGE + 1024;
+constexpr int MXG_BOXES = 5;
+__host__ __device__ constexpr int mxg_box_rows(int b) { return b == 0 ? 16 : b == 4 ? MXG_MAX_N / 2 : 32 * b; }
+// Shared memory of a stage whose tiles have up to n tokens: weights, half of the tokens (in whole swizzle atoms), scales.
+__host__ __device__ constexpr int mxg_t_bytes(int n) { return (n / 2 * 128 + 1023) & ~1023; }
+__host__ __device__ constexpr int mxg_stage(int n) { return MXG_W_BYTES + mxg_t_bytes(n) + MXG_S_BYTES * (1 + (n + 127) / 128); }
 constexpr uint32_t MXG_SCALES_AT = 2 * MXG_MAX_N;
 constexpr uint32_t MXG_SCALE_COLS = 24;             // columns of tensor memory of a set: 8 of weights, 16 of tokens
 static_assert(MXG_SCALES_AT + 2 * MXG_SCALE_COLS <= 512, "tensor memory");
-static_assert(MXG_STAGE % 1024 == 0 && MXG_T_BYTES % 1024 == 0, "swizzle atoms");
 
 struct MxParams {
   CUtensorMap w, ws;               // weights' codes, 128-byte x 128-row boxes; scales, two atoms a box
-  CUtensorMap tok[4], ts;          // token rows in boxes of 32, 64, 96, 112 rows; scales
+  CUtensorMap tok[MXG_BOXES], ts;  // token rows in boxes of 16, 32, 64, 96, 112 rows; scales
   const int32_t* cu_seqlens;
   const int32_t* pads;
   int ngroups, total_rows, K;
@@ -63,6 +65,18 @@ struct MxParams {
   int32_t* status;
   unsigned long long timeout_ns;
 };
+
+// Shared memory that the kernel declares itself: staged tokens, group tables, scales of two tiles, barriers (rounded up).
+template <int EPI> constexpr int mxg_token_row() { return (EPI == MX_EPI_SWIGLU_SAVE ? 384 : EPI == MX_EPI_SWIGLU ? 128 : 256) + 16; }
+template <int EPI> constexpr int mxg_static_smem() {
+  return MXG_SETS * TG_CHUNK * mxg_token_row<EPI>() + (3 * MAX_GROUPS + 1) * 4 + (EPI == MX_EPI_BF16 ? 8 : 2 * MXG_MAX_N * 4) + 512;
+}
+
+// Slots of the ring: as many as the device's shared memory has room for beside these.
+template <int EPI, int MAX_N> constexpr int mxg_stages() {
+  const int n = (227 * 1024 - 1024 - mxg_static_smem<EPI>()) / mxg_stage(MAX_N);
+  return n < MXG_MAX_STAGES ? n : MXG_MAX_STAGES;
+}
 
 struct MxTile {
   int g, row0, n;          // first row (a multiple of 32), tokens computed (a multiple of 32)
@@ -96,12 +110,12 @@ __host__ __device__ constexpr uint32_t make_instr_desc_mxf4(int M, int N, int sc
          ((uint32_t)(M >> 4) << 24) | ((uint32_t)scale_byte << 29);
 }
 
-template <int EPI>
+template <int EPI, int MAX_N>
 __global__ void __launch_bounds__(MXG_THREADS, 1)
 ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
+  constexpr int NST = mxg_stages<EPI, MAX_N>(), STAGE = mxg_stage(MAX_N), T_BYTES = mxg_t_bytes(MAX_N);
   constexpr bool GATED = EPI != MX_EPI_BF16, SAVE = EPI == MX_EPI_SWIGLU_SAVE;
-  constexpr int NST = MXG_STAGES;
-  constexpr int TOK_ROW = (SAVE ? 384 : GATED ? 128 : 256) + 16;     // bytes of a staged token
+  constexpr int TOK_ROW = mxg_token_row<EPI>();     // bytes of a staged token
   const int crank = (int)cluster_cta_rank();
   const int work_id0 = (int)(blockIdx.x >> 1), work_stride = (int)(gridDim.x >> 1);
   extern __shared__ uint8_t smem_dyn[];
@@ -111,7 +125,7 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
   __shared__ __align__(8) uint64_t acc_empty[2];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
-  __shared__ int s_end[MAX_GROUPS];
+  __shared__ int s_end[MAX_GROUPS], s_span[MAX_GROUPS];
   __shared__ int s_prefix[MAX_GROUPS + 1];
   __shared__ __align__(128) uint8_t s_stage[MXG_SETS][TG_CHUNK * TOK_ROW];
   __shared__ float s_scale[GATED ? 2 : 1][GATED ? MXG_MAX_N : 1];
@@ -120,28 +134,33 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
   uint8_t* stages = (uint8_t*)(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
   volatile int* abortp = &s_abort;
 
-  if (tid == 0) {
-    // both CTAs' loads count on the leader's full barrier, on which only its producer arrives
-    for (int s = 0; s < NST; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int a = 0; a < 2; ++a) { mbar_init(&acc_full[a], 1); mbar_init(&acc_empty[a], 8 * MXG_SETS); }
-    mbar_fence_init();
-    s_abort = 0;
+  if (warp == 0) {
+    if (lane == 0) {
+      // both CTAs' loads count on the leader's full barrier, on which only its producer arrives
+      for (int s = 0; s < NST; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+      for (int a = 0; a < 2; ++a) { mbar_init(&acc_full[a], 1); mbar_init(&acc_empty[a], 8 * MXG_SETS); }
+      mbar_fence_init();
+      s_abort = 0;
+    }
+    if (lane == 1) { tma_prefetch_desc(&p.w); tma_prefetch_desc(&p.ws); }
+    if (lane == 2) { tma_prefetch_desc(&p.ts); tma_prefetch_desc(&p.tok[0]); }
   }
+  // Group tables: ends, and rows with tokens counted from the multiple of 32 at or before the first.  (One round of loads
+  // for all groups, 1 us; the padding ranges looked up in the scan below and again for every tile cost 2 - 4 us a launch.)
   for (int g = tid; g < p.ngroups; g += MXG_THREADS) {
-    const int end = p.cu_seqlens != nullptr ? p.cu_seqlens[g] : p.total_rows;
-    s_end[g] = min(max(end, 0), p.total_rows);      // (no row outside the tensors is stored, whatever cu_seqlens says)
+    // (no row outside the tensors is stored, whatever cu_seqlens says)
+    auto clamped = [&](int end) { return min(max(end, 0), p.total_rows); };
+    const int start = g == 0 || p.cu_seqlens == nullptr ? 0 : clamped(p.cu_seqlens[g - 1]);
+    const int end = clamped(p.cu_seqlens != nullptr ? p.cu_seqlens[g] : p.total_rows);
+    s_end[g] = end;
+    s_span[g] = end > start ? (start & 31) + group_valid(p, g, start, end) : 0;
   }
   __syncthreads();
-  // rows of the group with tokens, from the multiple of 32 at or before its first
-  auto span = [&](int g) {
-    const int start = g == 0 ? 0 : s_end[g - 1], end = s_end[g];
-    return end > start ? (start & 31) + group_valid(p, g, start, end) : 0;
-  };
   if (warp == 0) {      // exclusive prefix of token tiles per group
     int run = 0;
     for (int g0 = 0; g0 < p.ngroups; g0 += 32) {
       const int g = g0 + lane;
-      const int nt = g < p.ngroups ? (span(g) + MXG_MAX_N - 1) / MXG_MAX_N : 0;
+      const int nt = g < p.ngroups ? (s_span[g] + MAX_N - 1) / MAX_N : 0;
       int incl = nt;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -161,19 +180,21 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
 
   const int m_tiles = (p.w_rows + 255) / 256;
   const long long total_tiles = (long long)s_prefix[p.ngroups] * m_tiles;
-  auto get = [&](long long id) {
-    MxTile t;
-    int lo = 0, hi = p.ngroups - 1;      // largest g with prefix[g] * m_tiles <= id
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if ((long long)s_prefix[mid] * m_tiles <= id) lo = mid; else hi = mid - 1;
+  // Tile `id`, for a whole warp; ids only grow, and g is where the warp's last tile was.
+  auto get = [&](long long id, int& g) {
+    while (true) {      // the first group behind g that starts beyond id, 32 at a time
+      const int i = g + 1 + lane;
+      const uint32_t beyond = __ballot_sync(0xffffffffu, i >= p.ngroups || (long long)s_prefix[i] * m_tiles > id);
+      if (beyond != 0u) { g += __ffs(beyond) - 1; break; }
+      g += 32;
     }
-    t.g = lo;
-    const int nt = s_prefix[lo + 1] - s_prefix[lo];
-    const int local = (int)(id - (long long)s_prefix[lo] * m_tiles);
+    MxTile t;
+    t.g = g;
+    const int nt = s_prefix[g + 1] - s_prefix[g];
+    const int local = (int)(id - (long long)s_prefix[g] * m_tiles);
     const int mi = local / nt, ti = local - mi * nt;       // tiles that share weights are neighbours
-    const int start = lo == 0 ? 0 : s_end[lo - 1], end = s_end[lo];
-    const int length = span(lo), valid = start + length - (start & 31);
+    const int start = g == 0 ? 0 : s_end[g - 1], end = s_end[g];
+    const int length = s_span[g], valid = start + length - (start & 31);
     t.n = ((length + nt - 1) / nt + 31) & ~31;
     t.row0 = (start & ~31) + ti * t.n;
     t.lo = max(t.row0, start);
@@ -192,16 +213,16 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
   if (warp == 0) {
     // ================= TMA producer =================
     const bool issue = elect_one();
-    if (issue) { tma_prefetch_desc(&p.w); tma_prefetch_desc(&p.ws); tma_prefetch_desc(&p.ts); }
+    int at = 0;
     RingSlot st;
     bool ok = true;
     for (long long id = work_id0; id < total_tiles && ok; id += work_stride) {
-      const MxTile t = get(id);
+      const MxTile t = get(id, at);
       const int n = uniform(t.n), row0 = uniform(t.row0), g = uniform(t.g), m = uniform(t.m);
-      const int box = min(4, (n / 2 + 31) / 32);
+      const int box = n / 2 <= 16 ? 0 : (n / 2 + 31) / 32;
       const int atoms = (n + 127) / 128;       // row atoms that hold the tokens' scales
-      const CUtensorMap* tmap = &p.tok[0] + (box - 1);
-      const uint32_t bytes = 2u * (uint32_t)(MXG_W_BYTES + min(box * 32, MXG_MAX_N / 2) * 128 + (1 + atoms) * MXG_S_BYTES);
+      const CUtensorMap* tmap = &p.tok[0] + box;
+      const uint32_t bytes = 2u * (uint32_t)(MXG_W_BYTES + mxg_box_rows(box) * 128 + (1 + atoms) * MXG_S_BYTES);
       const int wrow = g * p.w_rows + m + 128 * crank, watom = g * p.w_atoms + m / 128 + crank;
       const int trow = row0 + crank * (n / 2), tatom = (row0 >> 5 & 3) * p.t_atoms + (row0 >> 7);
       for (int kb = 0; kb < num_kb; ++kb, st.next(NST)) {
@@ -209,8 +230,8 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
         ok = warp_wait(&empty[s], st.parity ^ 1u, 1);
         if (!ok) break;
         if (!issue) continue;
-        uint8_t* sw = stages + (size_t)s * MXG_STAGE;
-        uint8_t* ss = sw + MXG_W_BYTES + MXG_T_BYTES;
+        uint8_t* sw = stages + (size_t)s * STAGE;
+        uint8_t* ss = sw + MXG_W_BYTES + T_BYTES;
         const uint32_t bar = mapa_u32(&full[s], 0);
         if (crank == 0) mbar_expect_tx(&full[s], bytes);
         tma_load_2d_pair(sw, &p.w, kb * 128, wrow, bar);
@@ -225,40 +246,45 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
       const bool issue = elect_one();
       const uint64_t desc_w = make_smem_desc(smem_u32(stages), 16, 1024);
       const uint64_t desc_t = make_smem_desc(smem_u32(stages) + MXG_W_BYTES, 16, 1024);
-      const uint64_t desc_s = make_scale_desc(smem_u32(stages) + MXG_W_BYTES + MXG_T_BYTES);
+      const uint64_t desc_s = make_scale_desc(smem_u32(stages) + MXG_W_BYTES + T_BYTES);
       RingSlot st;
-      int tile_n = 0;
+      int tile_n = 0, at = 0;
       uint32_t set = 0;
       bool ok = true;
       for (long long id = work_id0; id < total_tiles && ok; id += work_stride, ++tile_n) {
-        const MxTile t = get(id);
-        const int n = uniform(t.n), atoms = (n + 127) / 128;
-        const uint32_t idesc = make_instr_desc_mxf4(256, n, 0);
+        const int n = uniform(get(id, at).n);
+        const uint32_t idesc0 = make_instr_desc_mxf4(256, n, 0), idesc2 = make_instr_desc_mxf4(256, n, 2);
         const int acc = tile_n & 1;
         if (!warp_wait(&acc_empty[acc], ((uint32_t)(tile_n >> 1) & 1u) ^ 1u, 2)) break;
         tc_fence_after();
         const uint32_t tacc = tmem_base + (uint32_t)acc * MXG_MAX_N;
+        uint32_t add = 0u;
         for (int kb = 0; kb < num_kb; ++kb, st.next(NST), set ^= MXG_SCALE_COLS) {
           const int s = st.slot;
           ok = warp_wait(&full[s], st.parity, 3);
           if (!ok) break;
           tc_fence_after();
           if (issue) {
-            const uint32_t at = (uint32_t)(s * (MXG_STAGE >> 4));
-            const uint64_t da = desc_w + at, db = desc_t + at, ds = desc_s + at;
+            const uint32_t off = (uint32_t)(s * (STAGE >> 4));
+            const uint64_t da = desc_w + off, db = desc_t + off, ds = desc_s + off;
             const uint32_t tsa = tmem_base + MXG_SCALES_AT + set, tsb = tsa + 8;
+            // (row atoms behind a short tile's tokens are copied as they lie there: nothing is multiplied by them.  With
+            // the number of atoms as the loop's bound the issuer was what the kernel waited for: 8192 x 7168 x 4096 90 us, 82)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {        // block atoms of the k-block
               tmem_cp_scales_2cta(tsa + 4 * j, ds + j * (MX_ATOM_BYTES >> 4));
-              for (int a = 0; a < atoms; ++a)
+#pragma unroll
+              for (int a = 0; a < (MAX_N + 127) / 128; ++a)
                 tmem_cp_scales_2cta(tsb + 8 * j + 4 * a, ds + (((1 + a) * MXG_S_BYTES + j * MX_ATOM_BYTES) >> 4));
             }
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)       // 64 elements: two of an atom row's four scales
-              umma_mxf4_2cta(tacc, da + kk * 2, db + kk * 2, idesc | ((uint32_t)(kk & 1) << 5) | ((uint32_t)(kk & 1) << 30),
-                             tsa + 4 * (kk >> 1), tsb + 8 * (kk >> 1), (kb > 0 || kk > 0) ? 1u : 0u);
+            // 64 elements each: two of an atom row's four scales
+            umma_mxf4_2cta(tacc, da, db, idesc0, tsa, tsb, add);
+            umma_mxf4_2cta(tacc, da + 2, db + 2, idesc2, tsa, tsb, 1u);
+            umma_mxf4_2cta(tacc, da + 4, db + 4, idesc0, tsa + 4, tsb + 8, 1u);
+            umma_mxf4_2cta(tacc, da + 6, db + 6, idesc2, tsa + 4, tsb + 8, 1u);
             umma_commit_2cta(&empty[s], 3);
           }
+          add = 1u;
         }
         if (!ok) break;
         if (issue) umma_commit_2cta(&acc_full[acc], 3);
@@ -268,17 +294,19 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
     // ========= epilogue: two sets of four warps, each warp one quarter of the CTA's weight rows =========
     const int q = warp & 3, set = (warp - 2) >> 2;
     const int te = tid - 64 - set * 128;                    // 0..127
-    const int first = set * TG_CHUNK, step = MXG_SETS * TG_CHUNK;
-    const int my_tok = (te >> 5) * step + first + (te & 31);
-    int tile_n = 0;
+    const int step = MXG_SETS * TG_CHUNK;
+    int tile_n = 0, at = 0;
     uint8_t* const sb = s_stage[set];
     // this thread's row of the matrices that its warp stores: token 8 (lane / 16) + lane % 8, columns 8 (lane / 8 % 2)
     const uint32_t st_addr = smem_u32(sb) + (uint32_t)((8 * (lane >> 4) + (lane & 7)) * TOK_ROW + q * (GATED ? 32 : 64) +
                                                        ((lane >> 3) & 1) * 16);
     const bool vec_ok = p.vec_out != 0;
     for (long long id = work_id0; id < total_tiles; id += work_stride, ++tile_n) {
-      const MxTile t = get(id);
+      const MxTile t = get(id, at);
       const int acc = tile_n & 1;
+      // this set's chunks start at tokens first, first + step, ...; the sets change places from tile to tile, so that
+      // tiles of up to 32 tokens keep both busy
+      const int first = ((set + tile_n) & 1) * TG_CHUNK, my_tok = (te >> 5) * step + first + (te & 31);
       if constexpr (GATED) {       // (published by the barriers below)
         for (int i = my_tok; i < t.n; i += 4 * step) {
           const int r = t.row0 + i;
