@@ -12,7 +12,7 @@
 //        SwiGLU, down, both dgrads, the pushed combine, the fused dispatch.
 //        Also large products with fp32 output.
 //   ep_dense_f32_kernel (dense_f32.cuh): one product with fp32 output (router logits).
-//   ep_weight_grad_kernel (weight_grad.cuh): weight grads, fp32 output or with the SGD step in the epilogue.
+//   ep_weight_grad_kernel (weight_grad.cuh): weight grads, fp32 or bf16 output or with the SGD step in the epilogue.
 //   ep_mx_gemm_kernel (mx_gemm.cuh): token-major products of microscaled 4-bit operands.
 // Group g < split reads/writes allocation 0 (local experts), g >= split allocation 1 (this
 // rank's prefetch / reduce slots): the [2*epn] compute view never has to be contiguous.
@@ -209,6 +209,8 @@ struct MxDesc {
   const int32_t* pads;
   const float* row_scale;
   void *out, *gate, *up, *codes, *scales;                // codes, scales: the activation, quantised along its columns
+  const float* d_act;                                    // gated, backward: gate and up are their gradients
+  float* d_scale;                                        // [2 * tiles of w_rows][rows], or null
   int64_t ldc;
   int32_t* status;
   int64_t timeout_ns;
@@ -455,7 +457,11 @@ int mep_gemm_launch(const GemmDesc* d, cudaStream_t stream) {
     // weight grad: A [a_rows][Mw] and B [a_rows][N], both read as MN-major 64x64 boxes
     if (d->Mw % BM != 0) return fail(-2, "wgrad: Mw=%d must be a multiple of %d", d->Mw, BM);
     if ((rc = make_map(&kp.a, d->a[0], d->a_rows, d->Mw, d->lda[0], 64, BK))) return rc;
-    if (d->epi != EPI_F32) return fail(-3, "wgrad writes fp32");
+    const bool bf16 = d->epi == EPI_BF16;
+    if (d->epi != EPI_F32 && !bf16) return fail(-3, "wgrad writes fp32 or bf16");
+    if (bf16 && (d->accumulate || d->sgd_w[0] != nullptr || d->ngroups > d->split || d->N % 8 != 0))
+      return fail(-16, "wgrad: bf16 grads are stored, of local groups, with N %% 8 == 0");
+    if (bf16) kp.vec32 = d->N % 16 == 0;
     kp.products = d->b[1][0] != nullptr ? 2 : 1;
     if (d->sgd_w[0] != nullptr) {
       if (d->accumulate) return fail(-13, "wgrad: the fused SGD step cannot accumulate into existing grads");
@@ -475,6 +481,7 @@ int mep_gemm_launch(const GemmDesc* d, cudaStream_t stream) {
       if (d->ngroups > d->split && d->out[2 * i + 1] == nullptr) return fail(-8, "wgrad: groups >= split need a slot grad tensor");
       if ((((uintptr_t)d->out[2 * i] | (uintptr_t)d->out[2 * i + 1]) & 15) != 0 || d->ldc % 4 != 0)
         return fail(-11, "weight-grad output must be 16-byte aligned with a 16-byte multiple row stride");
+      if (bf16) kp.vec32 = kp.vec32 && ((uintptr_t)d->out[2 * i] & 31) == 0;
       if (d->accumulate) {
         const int64_t n_local = d->split < d->ngroups ? d->split : d->ngroups;
         if ((rc = make_map<true>(&kp.b2[i][0], d->out[2 * i], n_local * d->Mw, d->N, d->ldc, 32, 32))) return rc;
@@ -486,12 +493,13 @@ int mep_gemm_launch(const GemmDesc* d, cudaStream_t stream) {
     wgrad_geometry(&kp, d->rows_used > 0 ? d->rows_used : d->total_rows, pair);
     kp.wg_select = kp.sgd_w[0] != nullptr ? d->wg_select : 0;
     if (kp.sgd_w[0] != nullptr) return launch_wgrad<WG_SGD>(kp, pair, grid, stream);
+    if (bf16) return launch_wgrad<WG_BF16>(kp, pair, grid, stream);
     return kp.accumulate ? launch_wgrad<WG_ADD>(kp, pair, grid, stream) : launch_wgrad<WG_STORE>(kp, pair, grid, stream);
   }
+  const bool dense_f32 = d->epi == EPI_F32 && d->ngroups == 1 && d->cu_seqlens == nullptr;
   if (d->epi == EPI_F32) {
-    // router logits: one group, one segment
-    if (d->ngroups != 1 || d->cu_seqlens != nullptr || d->nseg != 1 || d->accumulate)
-      return fail(-15, "gemm: fp32 output is one dense product");
+    // router logits, or the down-dgrad of groups whose SwiGLU backward wants it unrounded: one segment
+    if (d->nseg != 1 || d->accumulate || d->disp_mode != 0) return fail(-15, "gemm: fp32 output is one product");
     if (d->K % 8 != 0) return fail(-4, "gemm: K=%d must be a multiple of 8", d->K);
     if (d->total_rows < 1) return 0;
   }
@@ -500,7 +508,7 @@ int mep_gemm_launch(const GemmDesc* d, cudaStream_t stream) {
   // columns 237 -> 110 us, 16384 x 2048 -> 512 86 -> 46.  Up to 128 columns half of a pair's tile would be empty:
   // single CTAs, from twice as many tiles on (65536 x 512 -> 128 49 -> 34; 32768 x 2048 -> 128 48 either way).
   const long long dn_rows = ((long long)d->total_rows * ((d->N + BM - 1) / BM) + grid - 1) / grid;
-  if (d->epi == EPI_F32 && (dn_rows <= DN_MAX_TOK || (d->N <= BM && dn_rows <= 2 * DN_MAX_TOK))) {
+  if (dense_f32 && (dn_rows <= DN_MAX_TOK || (d->N <= BM && dn_rows <= 2 * DN_MAX_TOK))) {
     DenseParams dp;
     std::memset(&dp, 0, sizeof(dp));
     dp.out = (float*)d->out[0]; dp.ldc = d->ldc; dp.S = d->total_rows; dp.N = d->N;
@@ -603,6 +611,15 @@ int mep_gemm_launch(const GemmDesc* d, cudaStream_t stream) {
 
 int mep_mx_desc_bytes() { return (int)sizeof(MxDesc); }
 
+// sum[r] = parts[0][r] + parts[1][r] + ..., zero for the rows behind *rows_ptr.
+int mep_mx_sum_parts(const float* parts, int n, int rows, const int32_t* rows_ptr, float* sum, cudaStream_t stream) {
+  if (n < 1 || rows < 0) return fail(-1, "mx sum: %d x %d", n, rows);
+  if (rows == 0) return 0;
+  ep_mx_sum_parts_kernel<<<(rows + 255) / 256, 256, 0, stream>>>(parts, n, rows, rows_ptr, sum);
+  MEP_CUDA_OK(cudaGetLastError());
+  return 0;
+}
+
 int mep_mx_gemm_launch(const MxDesc* d, cudaStream_t stream) {
   if (d->ngroups < 1 || d->ngroups > MAX_GROUPS) return fail(-1, "mx product: ngroups=%d out of range", d->ngroups);
   if (d->rows < 0 || d->K < 1 || d->N < 1 || d->w_rows < 1) return fail(-2, "mx product: %d x %d x %d", d->rows, d->K, d->N);
@@ -615,10 +632,10 @@ int mep_mx_gemm_launch(const MxDesc* d, cudaStream_t stream) {
   int rc = 0;
   if ((rc = make_byte_map(&p.w, d->w_codes, (int64_t)d->ngroups * d->w_rows, k_bytes, 128))) return rc;
   if ((rc = make_byte_map(&p.ws, d->w_scales, (int64_t)d->ngroups * p.w_atoms, s_bytes, 0))) return rc;
-  for (int b = 0; b < MXG_BOXES; ++b)
+  const bool few = d->rows <= MXG_FEW_N * (int64_t)d->ngroups;
+  for (int b = 0; b < (few ? 2 : MXG_BOXES); ++b)       // (boxes of up to half a tile's tokens)
     if ((rc = make_byte_map(&p.tok[b], d->a_codes, d->rows, k_bytes, mxg_box_rows(b)))) return rc;
   if ((rc = make_byte_map(&p.ts, d->a_scales, (int64_t)MX_PHASES * p.t_atoms, s_bytes, 0))) return rc;
-  const bool few = d->rows <= MXG_FEW_N * (int64_t)d->ngroups;
   p.cu_seqlens = d->cu_seqlens; p.pads = d->pads; p.ngroups = d->ngroups; p.total_rows = d->rows; p.K = d->K; p.N = d->N;
   p.out = (__nv_bfloat16*)d->out; p.gate = (__nv_bfloat16*)d->gate; p.up = (__nv_bfloat16*)d->up;
   p.codes = (uint8_t*)d->codes; p.scales = (uint8_t*)d->scales;
@@ -630,6 +647,11 @@ int mep_mx_gemm_launch(const MxDesc* d, cudaStream_t stream) {
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  p.d_act = d->d_act; p.d_scale = d->d_scale;
+  if (d->d_act != nullptr) {
+    if (!d->gated || p.gate == nullptr || p.up == nullptr) return fail(-3, "mx product: the backward pass writes both gradients");
+    return launch_mx<MX_EPI_SWIGLU_BWD>(p, few, sms, stream);
+  }
   if (!d->gated) return launch_mx<MX_EPI_BF16>(p, few, sms, stream);
   return p.gate != nullptr || p.up != nullptr ? launch_mx<MX_EPI_SWIGLU_SAVE>(p, few, sms, stream)
                                               : launch_mx<MX_EPI_SWIGLU>(p, few, sms, stream);

@@ -21,13 +21,16 @@
 // SwiGLU: gate and up columns come packed in turns of 16 rows, so that a warp's 32 rows of tensor memory hold both of 16
 // activations: read as two fragments of 16 rows, gate and up of an element meet in one thread's registers, in fp32.
 // The activation is rounded to bf16 and, if it is the next product's operand, quantised while it is in shared memory.
+// Backward: the same product again, with the gradients of gate and up computed where the forward pass has the
+// activation.  Gate and up are then neither kept between the passes nor rounded: a quarter of a bf16 product's time for
+// four bytes an element of either.
 #pragma once
 
 #include "device/mx_format.cuh"
 
 namespace mep {
 
-enum { MX_EPI_BF16 = 0, MX_EPI_SWIGLU = 1, MX_EPI_SWIGLU_SAVE = 2 };
+enum { MX_EPI_BF16 = 0, MX_EPI_SWIGLU = 1, MX_EPI_SWIGLU_SAVE = 2, MX_EPI_SWIGLU_BWD = 3 };
 
 constexpr int MXG_MAX_N = 224;                   // tokens of a tile, at most
 constexpr int MXG_FEW_N = 64;                    // the same where groups are short
@@ -61,6 +64,8 @@ struct MxParams {
   int code_bytes, k_atoms, out_atoms;      // of act
   int vec_out;
   const float* row_scale;
+  const float* d_act;              // backward: gradient of the activation, [total_rows][N]
+  float* d_scale;                  // parts of the scales' gradients, [CTA's columns][total_rows], or null
   long long ldc;
   int32_t* status;
   unsigned long long timeout_ns;
@@ -69,7 +74,8 @@ struct MxParams {
 // Shared memory that the kernel declares itself: staged tokens, group tables, scales of two tiles, barriers (rounded up).
 template <int EPI> constexpr int mxg_token_row() { return (EPI == MX_EPI_SWIGLU_SAVE ? 384 : EPI == MX_EPI_SWIGLU ? 128 : 256) + 16; }
 template <int EPI> constexpr int mxg_static_smem() {
-  return MXG_SETS * TG_CHUNK * mxg_token_row<EPI>() + (3 * MAX_GROUPS + 1) * 4 + (EPI == MX_EPI_BF16 ? 8 : 2 * MXG_MAX_N * 4) + 512;
+  return MXG_SETS * TG_CHUNK * mxg_token_row<EPI>() + (3 * MAX_GROUPS + 1) * 4 + (EPI == MX_EPI_BF16 ? 8 : 2 * MXG_MAX_N * 4) +
+         (EPI == MX_EPI_SWIGLU_BWD ? MXG_SETS * 4 * TG_CHUNK * 4 : 0) + 512;
 }
 
 // Slots of the ring: as many as the device's shared memory has room for beside these.
@@ -114,7 +120,7 @@ template <int EPI, int MAX_N>
 __global__ void __launch_bounds__(MXG_THREADS, 1)
 ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
   constexpr int NST = mxg_stages<EPI, MAX_N>(), STAGE = mxg_stage(MAX_N), T_BYTES = mxg_t_bytes(MAX_N);
-  constexpr bool GATED = EPI != MX_EPI_BF16, SAVE = EPI == MX_EPI_SWIGLU_SAVE;
+  constexpr bool GATED = EPI != MX_EPI_BF16, SAVE = EPI == MX_EPI_SWIGLU_SAVE, BWD = EPI == MX_EPI_SWIGLU_BWD;
   constexpr int TOK_ROW = mxg_token_row<EPI>();     // bytes of a staged token
   const int crank = (int)cluster_cta_rank();
   const int work_id0 = (int)(blockIdx.x >> 1), work_stride = (int)(gridDim.x >> 1);
@@ -128,6 +134,7 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
   __shared__ int s_end[MAX_GROUPS], s_span[MAX_GROUPS];
   __shared__ int s_prefix[MAX_GROUPS + 1];
   __shared__ __align__(128) uint8_t s_stage[MXG_SETS][TG_CHUNK * TOK_ROW];
+  __shared__ float s_part[BWD ? MXG_SETS : 1][BWD ? 4 : 1][BWD ? TG_CHUNK : 1];     // sums over a quarter's columns
   __shared__ float s_scale[GATED ? 2 : 1][GATED ? MXG_MAX_N : 1];
 
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -313,6 +320,20 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
           s_scale[acc][i] = r >= t.lo && r < t.hi && p.row_scale != nullptr ? p.row_scale[r] : 1.f;
         }
       }
+      // the gradients that meet a chunk's fragments: columns 8 half + lane / 4 of the quarter, tokens 8 j + 2 (lane % 4)
+      // and the next at [4 j + 2 half]; on their way before the fragments are
+      float da[BWD ? 16 : 1];
+      auto load_gradients = [&](int c) {
+        if constexpr (BWD) {
+          const int col = t.m / 2 + 64 * crank + q * 16 + (lane >> 2);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int row = t.row0 + c + 8 * (i >> 2) + 2 * (lane & 3) + (i & 1), x = col + 8 * (i >> 1 & 1);
+            da[i] = row >= t.lo && row < t.hi && x < p.N ? __ldg(p.d_act + (long long)row * p.ldc + x) : 0.f;
+          }
+        }
+      };
+      if (first < t.n) load_gradients(first);
       const bool have = gemm_wait(&acc_full[acc], (uint32_t)(tile_n >> 1) & 1u, abortp, p, 4);
       __syncwarp();
       if (!epilogue_all(set, have)) break;
@@ -350,7 +371,37 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
           const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
           return *reinterpret_cast<const uint32_t*>(&h);
         };
-        if constexpr (GATED) {
+        if constexpr (BWD) {
+          const int col = t.m / 2 + 64 * crank + q * 16 + (lane >> 2);
+          float part[8];       // of token [2 j + e], over this thread's two columns
+#pragma unroll
+          for (int i = 0; i < 8; ++i) part[i] = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float dg[2], du[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float g = __uint_as_float(r[2 * i + e]), u = __uint_as_float(r[16 + 2 * i + e]);
+              const float sig = 1.f / (1.f + __expf(-g)), d = da[2 * i + e];
+              const float ds = d * s_scale[acc][c + 8 * (i >> 1) + 2 * (lane & 3) + e];
+              // (columns behind the last have whatever lies behind the weights)
+              part[2 * (i >> 1) + e] += col + 8 * (i & 1) < p.N ? d * (g * sig) * u : 0.f;
+              dg[e] = ds * u * (sig * (1.f + g * (1.f - sig)));
+              du[e] = ds * (g * sig);
+            }
+            pk[i] = pack(dg[0], dg[1]);
+            pk[8 + i] = pack(du[0], du[1]);
+          }
+          if (p.d_scale != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+#pragma unroll
+              for (int o = 4; o < 32; o <<= 1) part[i] += __shfl_xor_sync(0xffffffffu, part[i], o);
+              if (lane < 4) s_part[set][q][8 * (i >> 1) + 2 * lane + (i & 1)] = part[i];
+            }
+          }
+          if (c + step < t.n) load_gradients(c + step);
+        } else if constexpr (GATED) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             float a[2];
@@ -362,7 +413,7 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
             pa[i] = pack(a[0], a[1]);
           }
         }
-        if constexpr (!GATED || SAVE) {
+        if constexpr (EPI == MX_EPI_BF16 || SAVE) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) pk[i] = pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
         }
@@ -373,22 +424,38 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
           release_acc();
         }
         __syncwarp();
-        if constexpr (GATED) {
+        if constexpr (GATED && !BWD) {
 #pragma unroll
           for (int j = 0; j < 4; j += 2)
             stmatrix_x4_trans(st_addr + (uint32_t)(j * 8 * TOK_ROW), pa[2 * j], pa[2 * j + 1], pa[2 * j + 2], pa[2 * j + 3]);
         }
-        if constexpr (!GATED || SAVE) {
+        if constexpr (!GATED || SAVE || BWD) {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int j = 0; j < 4; j += 2)
-              stmatrix_x4_trans(st_addr + (uint32_t)(j * 8 * TOK_ROW + (SAVE ? 128 * (1 + h) : h * 32)),
+              stmatrix_x4_trans(st_addr + (uint32_t)(j * 8 * TOK_ROW + (SAVE ? 128 * (1 + h) : BWD ? 128 * h : h * 32)),
                                 pk[8 * h + 2 * j], pk[8 * h + 2 * j + 1], pk[8 * h + 2 * j + 2], pk[8 * h + 2 * j + 3]);
         }
         __syncwarp();
         epilogue_sync(set);
-        if constexpr (GATED) {
+        if constexpr (BWD) {
+          const int f = (te & 7) * 8, col0 = t.m / 2 + 64 * crank + f;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int k = (te >> 3) + 16 * i, row = t.row0 + c + k;
+            if (row < t.lo || row >= t.hi || col0 >= p.N) continue;
+            const long long off = (long long)row * p.ldc + col0;
+            store8(p.gate + off, *reinterpret_cast<const uint4*>(sb + k * TOK_ROW + f * 2), p.N - col0, vec_ok);
+            store8(p.up + off, *reinterpret_cast<const uint4*>(sb + k * TOK_ROW + 128 + f * 2), p.N - col0, vec_ok);
+          }
+          if (p.d_scale != nullptr && te < TG_CHUNK) {
+            const int row = t.row0 + c + te;
+            if (row >= t.lo && row < t.hi)
+              p.d_scale[(long long)(t.m / 128 + crank) * p.total_rows + row] =
+                  (s_part[set][0][te] + s_part[set][1][te]) + (s_part[set][2][te] + s_part[set][3][te]);
+          }
+        } else if constexpr (GATED) {
           const int f = (te & 7) * 8, col0 = t.m / 2 + 64 * crank + f;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -443,9 +510,12 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
         for (int row = t.hi + (te + 128 * set) / V; row < t.zero_to; row += 128 * MXG_SETS / V) {
           const uint4 zero = make_uint4(0, 0, 0, 0);
           const long long off = (long long)row * p.ldc + col0;
+          if constexpr (BWD) {
+            if (p.d_scale != nullptr && (te & 7) == 0) p.d_scale[(long long)(t.m / 128 + crank) * p.total_rows + row] = 0.f;
+          }
           if (col0 < p.N) {
             if (p.out) store8(p.out + off, zero, p.N - col0, vec_ok);
-            if constexpr (SAVE) {
+            if constexpr (SAVE || BWD) {
               if (p.gate) store8(p.gate + off, zero, p.N - col0, vec_ok);
               if (p.up) store8(p.up + off, zero, p.N - col0, vec_ok);
             }
@@ -472,6 +542,17 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
     tc_fence_after();
     tmem_dealloc2(tmem_base, 512);
   }
+}
+
+// Sums of the parts above, in their order.
+__global__ void __launch_bounds__(256) ep_mx_sum_parts_kernel(const float* __restrict__ parts, int n, int rows,
+                                                              const int32_t* __restrict__ rows_ptr, float* __restrict__ sum) {
+  const int r = blockIdx.x * 256 + threadIdx.x, used = rows_ptr ? min(*rows_ptr, rows) : rows;
+  if (r >= rows) return;
+  float s = 0.f;
+  if (r < used)
+    for (int i = 0; i < n; ++i) s += parts[(long long)i * rows + r];
+  sum[r] = s;
 }
 
 }  // namespace mep

@@ -1,5 +1,6 @@
 // Weight-grad GEMM (groups partition the REDUCTION dimension): D[g] (+)= A[rows of g]^T * B[rows of g], both
-// operands MN-major; fp32 output (stored, or added: WG_ADD), or WG_SGD, the optimizer step fused in: the accumulator is applied
+// operands MN-major; fp32 output (stored, or added: WG_ADD; WG_BF16: rounded to bf16 and stored, for leaves of
+// autograd), or WG_SGD, the optimizer step fused in: the accumulator is applied
 // straight to the bf16 weights, w = bf16(w - lr * acc), for every local expert that has no replica this step.
 //
 // A launch may compute the grads of two weights that share A (the gate and up projections): group by group, first
@@ -32,7 +33,7 @@
 
 namespace mep {
 
-enum { WG_STORE = 0, WG_SGD = 1, WG_ADD = 2 };        // what becomes of a tile (SGD: or stored, where it has replicas)
+enum { WG_STORE = 0, WG_SGD = 1, WG_ADD = 2, WG_BF16 = 3 };        // what becomes of a tile (SGD: or stored, where it has replicas)
 constexpr int WG_EPI_WARPS = 16;
 constexpr int WG_THREADS = 64 + WG_EPI_WARPS * 32;
 constexpr int WG_STEPS = 32 / WG_EPI_WARPS;           // 16-row x 64-column pieces of a tile that a warp takes
@@ -432,6 +433,24 @@ __global__ void __launch_bounds__(WG_THREADS, 1) ep_weight_grad_kernel(const __g
               quad_transpose(v + 4 * e, c);  // word c of the blocks 2b + e -> all words of block 2c + e
             }
             if (in_rows) wg_store16(dst + 8ll * h * p.N, p.N - col - 16 * c, vec32, v);
+          }
+        } else if (MODE == WG_BF16) {
+          // 16 columns of a row a thread, as with the weights: 32 contiguous bytes
+          __nv_bfloat16* dst = (__nv_bfloat16*)p.out[2 * t.prod] + row_of(t, k) * p.ldc + col + 16 * c;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t v[8];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+              for (int b = 0; b < 4; ++b) {
+                const uint32_t* gr = r + 4 * (2 * b + e) + 2 * h;
+                const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(gr[0]), __uint_as_float(gr[1]));
+                v[4 * e + b] = *reinterpret_cast<const uint32_t*>(&y);
+              }
+              quad_transpose(v + 4 * e, c);
+            }
+            if (in_rows) wg_store16(dst + 8ll * h * p.ldc, p.N - col - 16 * c, vec32, v);
           }
         } else {
           // threads 2i and 2i + 1 of a quad trade: 4 contiguous columns of an even block for one, of the next

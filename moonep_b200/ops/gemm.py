@@ -244,15 +244,19 @@ def down(act, wd, cu_seqlens, *, wd_slot=None, split=None, out=None, push=None, 
     return y
 
 
-def down_dgrad(dy, wd, cu_seqlens, *, wd_slot=None, split=None, out=None, g_begin=0, grid=0, dispatch=None, pads=None):
+def down_dgrad(dy, wd, cu_seqlens, *, wd_slot=None, split=None, out=None, g_begin=0, grid=0, dispatch=None, pads=None,
+               fp32=False):
     """``dact[rows,H'] = dy[rows,H] Wd[g]``.  ``out`` / ``g_begin`` / ``grid`` / ``dispatch`` as in
     :func:`gateup_swiglu`: the local experts and the prefetch slots may be two launches, and the
-    launch may carry the dispatch of ``dy`` itself."""
+    launch may carry the dispatch of ``dy`` itself.  ``fp32``: the sums unrounded (padding rows are left as they
+    are; not with ``dispatch``)."""
     rows, H = dy.shape
     Hp = wd.shape[2]
+    dtype = torch.float32 if fp32 else torch.bfloat16
     if out is None:
-        out = torch.empty(rows, Hp, dtype=torch.bfloat16, device=dy.device)
-    _tokens_gemm([dy], [wd], [wd_slot], cu_seqlens, split, Hp, H, H, True, EPI_BF16, [out], Hp,
+        out = torch.empty(rows, Hp, dtype=dtype, device=dy.device)
+    assert out.dtype == dtype and not (fp32 and dispatch is not None)
+    _tokens_gemm([dy], [wd], [wd_slot], cu_seqlens, split, Hp, H, H, True, EPI_F32 if fp32 else EPI_BF16, [out], Hp,
                  grid=grid, g_begin=g_begin, dispatch=dispatch, pads=pads)
     return out
 
@@ -294,6 +298,8 @@ def wgrad(a, b, cu_seqlens, grad_local, *, grad_slot=None, split=None, accumulat
     with ``select=0``.  The stored grads are the ones that ``reduce_grad`` has to move, so computing
     them first lets that transfer run beside the rest of the weight grad.
 
+    A bf16 ``grad_local`` takes the grads rounded (no slots, no ``accumulate``, no ``sgd``; N a multiple of 8).
+
     ``rows``: how many rows of ``a`` hold tokens, where the caller knows (a Buffer's ``N``; its row tensor has
     spare rows).  It changes no result, only how the launch is split."""
     assert select in (0, 1, 2) and (select == 0 or sgd is not None), "select splits a fused-SGD weight grad"
@@ -317,7 +323,9 @@ def _wgrads(a, products, cu_seqlens, split, accumulate, lr, keep, grid, select, 
     rows, M = a.shape
     N = products[0][0].shape[1]
     d = _GemmDesc()
-    d.mode, d.epi, d.b_mn, d.nseg = 1, EPI_F32, 1, 1
+    dtype = products[0][1].dtype
+    assert dtype in (torch.float32, torch.bfloat16)
+    d.mode, d.epi, d.b_mn, d.nseg = 1, EPI_F32 if dtype == torch.float32 else EPI_BF16, 1, 1
     cu_ptr, ngroups = _groups(cu_seqlens, rows)
     d.ngroups = ngroups
     d.split = ngroups if split is None else split
@@ -329,7 +337,7 @@ def _wgrads(a, products, cu_seqlens, split, accumulate, lr, keep, grid, select, 
     d.cu_seqlens = cu_ptr
     for i, (b, grad, slot, w) in enumerate(products):
         _bf16(b, "b")
-        assert b.shape[0] == rows and grad.dtype == torch.float32 and grad.is_contiguous()
+        assert b.shape[0] == rows and grad.dtype == dtype and grad.is_contiguous()
         assert grad.shape[1:] == (M, N)
         d.b[i][0], d.ldb = b.data_ptr(), b.stride(0)
         d.out[2 * i] = grad.data_ptr()

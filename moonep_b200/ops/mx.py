@@ -13,6 +13,7 @@ op                        math                            operands
 ``pack_gate_up``          Wg, Wu -> one ``MxTensor``      [G, H, H'] each, blocks along H
 ``matmul``                y = a W[g]^T                    a [rows,K] . W [G,N,K]
 ``gateup_swiglu``         act = silu(x Wg)*(x Wu)*w       x [rows,H] . packed Wg, Wu
+``gateup_swiglu_bwd``     d gate, d up, d w               fp32 d act [rows,H'] and the forward's
 ``expert_ffn``            y = act Wd^T, with gradients    bf16 x [rows,H], Wg/Wu/Wd [G,H,H']
 ========================  ==============================  =======================================
 
@@ -23,6 +24,8 @@ missing; there is no eager fallback.  Bounded waits that run out are reported by
 from __future__ import annotations
 
 import ctypes
+import math
+import struct
 from typing import Optional
 
 import torch
@@ -37,41 +40,36 @@ BLOCK = 32
 PHASES = 4
 
 
-class _MxDesc(ctypes.Structure):
-    _fields_ = [
-        ("a_codes", P), ("a_scales", P), ("w_codes", P), ("w_scales", P),
-        ("rows", ctypes.c_int32), ("K", ctypes.c_int32), ("ngroups", ctypes.c_int32),
-        ("w_rows", ctypes.c_int32), ("N", ctypes.c_int32), ("gated", ctypes.c_int32),
-        ("cu_seqlens", P), ("pads", P), ("row_scale", P),
-        ("out", P), ("gate", P), ("up", P), ("codes", P), ("scales", P),
-        ("ldc", ctypes.c_int64), ("status", P), ("timeout_ns", ctypes.c_int64),
-    ]
+# The product's descriptor, as the C side lays it out: four operand pointers; rows, K, groups, weight rows, N, gated; cu_seqlens,
+# pads, row_scale, out, gate, up, codes, scales, d_act, d_scale; ldc, status, timeout.  (Packed in one call: filling a ctypes structure
+# field by field took as long as the launch.)
+_DESC = struct.Struct("@4P6i10PqPq")
 
 
 nat.declare("mep_mx_quantize", I, [P, I, L, L, I, I, I, I, I, I, I, P, P, P, P])
 nat.declare("mep_mx_dequantize", I, [P, P, I, I, I, I, I, P, I, P, P])
 nat.declare("mep_mx_desc_bytes", I, [])
-nat.declare("mep_mx_gemm_launch", I, [ctypes.POINTER(_MxDesc), P])
+nat.declare("mep_mx_sum_parts", I, [P, I, I, P, P, P])
+nat.declare("mep_mx_gemm_launch", I, [ctypes.c_char_p, P])
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _MAX = 2 ** 31 - 1
 _checked_layout = False
 
 
-def _atoms(n: int) -> int:
-    return (n + 127) // 128
+_device = torch._C._cuda_getDevice       # (torch.cuda.current_device() without its check that CUDA is initialised)
 
 
 def _here(t: torch.Tensor, name: str) -> torch.Tensor:
     assert t.is_cuda, f"{name} must be a CUDA tensor"
-    assert t.device.index == torch.cuda.current_device(), f"{name} is on {t.device}, not on the current device"
+    assert t.get_device() == _device(), f"{name} is on {t.device}, not on the current device"
     return t
 
 
-def _rows_ptr(rows_ptr, device):
+def _rows_ptr(rows_ptr, index: int) -> int:
     if rows_ptr is None:
-        return None
-    assert rows_ptr.dtype == torch.int32 and rows_ptr.numel() == 1 and rows_ptr.device == device, \
+        return 0
+    assert rows_ptr.dtype == torch.int32 and rows_ptr.numel() == 1 and rows_ptr.get_device() == index, \
         "rows_ptr must be one int32 on the operand's device"
     return rows_ptr.data_ptr()
 
@@ -86,21 +84,54 @@ class MxTensor:
     K atoms, 512]``: the atoms of phase ``s`` begin at row ``32 s`` (row ``r`` is its row ``r - 32 s``), for the products'
     tiles of token rows, which start at any multiple of 32."""
 
-    __slots__ = ("codes", "scales", "shape")
+    __slots__ = ("shape", "_codes", "_scales", "_data", "_index", "_mats", "_rows", "_at")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape):
         shape = tuple(int(n) for n in shape)
         assert len(shape) in (2, 3, 4) and (len(shape) < 4 or shape[0] == 2), "[rows, K], [G, rows, K] or [2, G, rows, K]"
-        rows, K = _stored_rows(shape), shape[-1]
-        lead = shape[-3:-2]
         assert codes.dtype == torch.uint8 and scales.dtype == torch.uint8 and codes.device == scales.device
-        assert codes.is_contiguous() and tuple(codes.shape) == (*lead, rows, (K + BLOCK - 1) // BLOCK * (BLOCK // 2))
-        assert scales.is_contiguous() and tuple(scales.shape) == (*(lead or (PHASES,)), _atoms(rows), _atoms(K), 512)
-        self.codes, self.scales, self.shape = codes, scales, shape
+        sizes = _sizes(shape)
+        assert codes.is_contiguous() and scales.is_contiguous() and (tuple(codes.shape), tuple(scales.shape)) == sizes, \
+            f"a tensor of shape {shape} has codes and scales of {sizes}"
+        assert codes.data_ptr() % 16 == 0 and scales.data_ptr() % 16 == 0, "codes and scales must be 16-byte aligned"
+        self._codes, self._scales, self._data = codes, scales, codes
+        self._set(shape, sizes, (codes.data_ptr(), scales.data_ptr()))
+
+    def _set(self, shape, sizes, at):
+        self.shape, self._at = shape, at              # (addresses of codes and scales)
+        self._index = self._data.get_device()
+        self._mats, self._rows = (1 if len(shape) == 2 else shape[-3]), sizes[0][-2]
+        return self
+
+    @classmethod
+    def _empty(cls, shape, device, zero: bool = False) -> "MxTensor":
+        """A new one; codes and scales share an allocation, whose two views are made when somebody asks for them."""
+        sizes = _sizes(shape)
+        n = (math.prod(sizes[0]) + 511) // 512 * 512
+        self = cls.__new__(cls)
+        self._data = (torch.zeros if zero else torch.empty)(n + math.prod(sizes[1]), dtype=torch.uint8, device=device)
+        self._codes = self._scales = None
+        at = self._data.data_ptr()
+        return self._set(shape, sizes, (at, at + n))
+
+    def _views(self):
+        if self._codes is None:
+            codes, scales = _sizes(self.shape)
+            n, m = math.prod(codes), math.prod(scales)
+            self._codes, self._scales = self._data[:n].view(codes), self._data[self._data.numel() - m:].view(scales)
+        return self._codes, self._scales
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self._views()[0]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._views()[1]
 
     @property
     def device(self):
-        return self.codes.device
+        return self._data.device
 
     @property
     def nbytes(self) -> int:
@@ -113,46 +144,47 @@ class MxTensor:
         """The values, bf16 (exact down to 2^-133, the last bit of its subnormals) or fp32, of this tensor's shape;
         gate first, then up, for a packed pair.  ``rows_ptr`` as in :func:`quantize`."""
         assert dtype in (torch.bfloat16, torch.float32), "values are bf16 or fp32"
-        _here(self.codes, "the operand")
+        _here(self._data, "the operand")
         pair = len(self.shape) == 4
         assert rows_ptr is None or len(self.shape) == 2, "rows_ptr goes with one matrix"
-        mats = self.codes.shape[0] if self.codes.dim() == 3 else 1
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        out = torch.empty(self.shape, dtype=dtype, device=self._data.device)
         for i in range(2 if pair else 1):
-            dst = out[i] if pair else out
-            ew._rc(nat.call("mep_mx_dequantize", self.codes.data_ptr(), self.scales.data_ptr(), mats, self.shape[-2],
-                            self.shape[-1], i + 1 if pair else 0, self.codes.shape[-2], _rows_ptr(rows_ptr, self.device),
-                            int(dtype == torch.float32), dst.data_ptr(), nat.stream()), "mx dequantise")
+            ew._rc(nat.call("mep_mx_dequantize", *self._at, self._mats, self.shape[-2],
+                            self.shape[-1], i + 1 if pair else 0, self._rows, _rows_ptr(rows_ptr, self._index),
+                            int(dtype == torch.float32), (out[i] if pair else out).data_ptr(), nat.stream()), "mx dequantise")
         return out
 
 
-def _stored_rows(shape) -> int:
-    """Rows of a matrix of codes: for a pair the gate's and the up projection's in turns of 16."""
-    return shape[-2] if len(shape) < 4 else (shape[-2] + 15) // 16 * 32
-
-
-def _empty(shape, device, zero: bool = False) -> MxTensor:
-    rows, K, lead = _stored_rows(shape), shape[-1], shape[-3:-2]
-    make = torch.zeros if zero else torch.empty
-    codes = make(*lead, rows, (K + BLOCK - 1) // BLOCK * (BLOCK // 2), dtype=torch.uint8, device=device)
-    scales = make(*(lead or (PHASES,)), _atoms(rows), _atoms(K), 512, dtype=torch.uint8, device=device)
-    return MxTensor(codes, scales, shape)
+def _sizes(shape):
+    """Sizes of a tensor's codes and scales.  (The rows of a packed pair are the gate's and the up projection's in turns
+    of 16.)"""
+    rows, K = shape[-2:]
+    if len(shape) == 4:
+        rows = (rows + 15) // 16 * 32
+    code_bytes, atoms, k_atoms = (K + 31) // 32 * 16, (rows + 127) // 128, (K + 127) // 128
+    if len(shape) == 2:
+        return (rows, code_bytes), (PHASES, atoms, k_atoms, 512)
+    G = shape[-3]
+    return (G, rows, code_bytes), (G, atoms, k_atoms, 512)
 
 
 def _quantize_into(q: MxTensor, x: torch.Tensor, axis: int, interleave: int, rows_ptr) -> None:
-    mats, (rows, cols) = (x.shape[0] if x.dim() == 3 else 1), x.shape[-2:]
-    batch = x.stride(0) if x.dim() == 3 else 0
-    ew._rc(nat.call("mep_mx_quantize", x.data_ptr(), _TYPES[x.dtype], batch, x.stride(-2), mats, rows, cols, int(axis == -2),
-                    interleave, q.codes.shape[-2], PHASES if q.codes.dim() == 2 else 1, _rows_ptr(rows_ptr, x.device), q.codes.data_ptr(), q.scales.data_ptr(),
-                    nat.stream()), "mx quantise")
+    size, stride = x.shape, x.stride()
+    three = len(size) == 3
+    rc = nat.call("mep_mx_quantize", x.data_ptr(), _TYPES[x.dtype], stride[0] if three else 0, stride[-2], size[0] if three else 1,
+                  size[-2], size[-1], int(axis == -2), interleave, q._rows, 1 if len(q.shape) > 2 else PHASES,
+                  _rows_ptr(rows_ptr, q._index), *q._at, nat.stream())
+    if rc != 0:
+        ew._rc(rc, "mx quantise")
 
 
 def _operand(x: torch.Tensor, name: str) -> torch.Tensor:
     _here(x, name)
     assert x.dtype in _TYPES, f"{name} must be bf16, fp16 or fp32"
-    assert x.dim() in (2, 3), f"{name} must be [rows, K] or [G, rows, K]"
-    assert x.shape[-1] >= 1 and x.shape[-2] <= _MAX and x.shape[-1] <= _MAX
-    assert x.shape[-1] == 1 or x.stride(-1) == 1, f"{name} must be dense along its last axis"
+    size = x.shape
+    assert len(size) in (2, 3), f"{name} must be [rows, K] or [G, rows, K]"
+    assert size[-1] >= 1 and size[-2] <= _MAX and size[-1] <= _MAX
+    assert size[-1] == 1 or x.stride(-1) == 1, f"{name} must be dense along its last axis"
     return x
 
 
@@ -165,10 +197,9 @@ def quantize(x: torch.Tensor, axis: int = -1, *, rows_ptr: Optional[torch.Tensor
     _operand(x, "x")
     assert axis in (-1, -2), "axis must be -1 or -2"
     assert rows_ptr is None or (x.dim() == 2 and axis == -1), "rows_ptr goes with one matrix and axis=-1"
-    x = x.detach()
-    shape = x.shape if axis == -1 else (*x.shape[:-2], x.shape[-1], x.shape[-2])
+    shape = tuple(x.shape) if axis == -1 else (*x.shape[:-2], x.shape[-1], x.shape[-2])
     assert shape[-1] >= 1, "the reduction is empty"
-    q = _empty(shape, x.device)
+    q = MxTensor._empty(shape, x.device)
     _quantize_into(q, x, axis, 0, rows_ptr)
     return q
 
@@ -181,43 +212,45 @@ def pack_gate_up(wg: torch.Tensor, wu: torch.Tensor) -> MxTensor:
     assert wg.shape[-2] >= 1, "the reduction is empty"
     wg, wu = (w.detach() if w.dim() == 3 else w.detach()[None] for w in (wg, wu))
     G, H, Hp = wg.shape
-    q = _empty((2, G, Hp, H), wg.device, zero=Hp % 16 != 0)      # (the last turn of 16 is not full: zeros)
+    q = MxTensor._empty((2, G, Hp, H), wg.device, zero=Hp % 16 != 0)      # (the last turn of 16 is not full: zeros)
     _quantize_into(q, wg, -2, 1, None)
     _quantize_into(q, wu, -2, 2, None)
     return q
 
 
-def _launch(a: MxTensor, w: MxTensor, N: int, gated: bool, cu_seqlens, pads, row_scale, outs, ldc: int) -> None:
+def _launch(a: MxTensor, w: MxTensor, N: int, gated: int, cu_seqlens, pads, row_scale, out: int, gate: int, up: int, codes: int,
+            scales: int, ldc: int, d_act: int = 0, d_scale: int = 0) -> None:
     global _checked_layout
-    assert len(a.shape) == 2, "the rows' operand is one matrix"
-    _here(a.codes, "a")
-    assert w.device == a.device and w.shape[-1] == a.shape[-1], "operands do not go together"
-    ngroups = w.codes.shape[0] if w.codes.dim() == 3 else 1
-    assert 1 <= ngroups <= 1024, "1 to 1024 groups"
-    d = _MxDesc()
-    d.a_codes, d.a_scales, d.rows = a.codes.data_ptr(), a.scales.data_ptr(), a.shape[0]
-    d.w_codes, d.w_scales, d.w_rows = w.codes.data_ptr(), w.scales.data_ptr(), w.codes.shape[-2]
-    d.K, d.N, d.ngroups, d.gated = a.shape[1], N, ngroups, int(gated)
+    index, groups, (rows, K) = a._index, w._mats, a.shape
+    assert index == _device(), "the operands are not on the current device"
+    assert w._index == index and w.shape[-1] == K, "operands do not go together"
+    assert 1 <= groups <= 1024, "1 to 1024 groups"
+    cu = pad = scale = 0
     if cu_seqlens is None:
-        assert ngroups == 1, "several groups need cu_seqlens"
+        assert groups == 1, "several groups need cu_seqlens"
     else:
-        assert cu_seqlens.device == a.device and cu_seqlens.numel() == ngroups, "one entry of cu_seqlens a group"
-        d.cu_seqlens = gemm._groups(cu_seqlens, None)[0]
+        assert cu_seqlens.dtype == torch.int32 and cu_seqlens.get_device() == index and cu_seqlens.is_contiguous() \
+            and cu_seqlens.numel() == groups, "cu_seqlens must be int32, one entry a group"
+        cu = cu_seqlens.data_ptr()
         if pads is not None:
-            assert pads.device == a.device
-            d.pads = gemm._pads(pads, cu_seqlens)
+            assert pads.get_device() == index
+            pad = gemm._pads(pads, cu_seqlens)
     if row_scale is not None:
-        assert row_scale.dtype == torch.float32 and row_scale.device == a.device and row_scale.is_contiguous()
-        assert row_scale.dim() == 1 and row_scale.numel() >= a.shape[0], "one scale a row"
-        d.row_scale = row_scale.data_ptr()
-    for name, t in outs.items():
-        setattr(d, name, nat.ptr(t))
-    d.ldc = ldc
-    d.status = gemm.status_word(a.device).data_ptr()
+        assert row_scale.dtype == torch.float32 and row_scale.get_device() == index and row_scale.is_contiguous() \
+            and row_scale.dim() == 1 and row_scale.numel() >= rows, "row_scale must be fp32, one a row"
+        scale = row_scale.data_ptr()
+    status = gemm._status.get(index)
+    if status is None:
+        status = gemm.status_word(a.device)
     if not _checked_layout:
-        assert nat.call("mep_mx_desc_bytes") == ctypes.sizeof(_MxDesc), "MxDesc layout mismatch"
+        assert nat.call("mep_mx_desc_bytes") == _DESC.size, "MxDesc layout mismatch"
         _checked_layout = True
-    ew._rc(nat.call("mep_mx_gemm_launch", ctypes.byref(d), nat.stream()), "mx product")
+    rc = nat.call("mep_mx_gemm_launch",
+                  _DESC.pack(*a._at, *w._at, rows, K, groups, w._rows, N, gated, cu, pad, scale, out, gate, up, codes, scales,
+                             d_act, d_scale, ldc, status.data_ptr(), 0),
+                  nat.stream())
+    if rc != 0:
+        ew._rc(rc, "mx product")
 
 
 def matmul(a: MxTensor, w: MxTensor, cu_seqlens: Optional[torch.Tensor] = None, *, out: Optional[torch.Tensor] = None,
@@ -229,15 +262,18 @@ def matmul(a: MxTensor, w: MxTensor, cu_seqlens: Optional[torch.Tensor] = None, 
     are.  ``pads`` (a plan's ``zero_fill_ranges``): which rows of the groups are padding; they become zeros without
     being computed."""
     assert isinstance(a, MxTensor) and isinstance(w, MxTensor) and len(w.shape) < 4, "operands must be quantised"
-    N = w.shape[-2]
+    assert len(a.shape) == 2, "the rows' operand is one matrix"
+    rows, N = a.shape[0], w.shape[-2]
     if out is None:
-        out = torch.empty(a.shape[0], N, dtype=torch.bfloat16, device=a.device)
+        out = torch.empty((rows, N), dtype=torch.bfloat16, device=a._data.device)
+        ld = N
     else:
-        assert out.device == a.device and out.dtype == torch.bfloat16 and out.dim() == 2
-        assert out.shape[0] >= a.shape[0] and out.shape[1] == N and (N == 1 or out.stride(1) == 1)
-        assert out.shape[0] < 2 or out.stride(0) >= N, "rows of out overlap"
+        assert out.get_device() == a._index and out.dtype == torch.bfloat16 and out.dim() == 2
+        assert out.shape[0] >= rows and out.shape[1] == N and (N <= 1 or out.stride(1) == 1)
+        ld = out.stride(0)
+        assert out.shape[0] < 2 or ld >= N, "rows of out overlap"
     if N > 0:
-        _launch(a, w, N, False, cu_seqlens, pads, None, dict(out=out), out.stride(0) if out.shape[0] > 1 else max(N, out.stride(0)))
+        _launch(a, w, N, 0, cu_seqlens, pads, None, out.data_ptr(), 0, 0, 0, 0, ld)
     return out
 
 
@@ -251,13 +287,44 @@ def gateup_swiglu(a: MxTensor, wgu: MxTensor, cu_seqlens: Optional[torch.Tensor]
     ``save_gate_up``, else ``None``; the activation is computed from their fp32 sums.  Rows that belong to no group are
     undefined.  ``pads`` as in :func:`matmul`."""
     assert isinstance(a, MxTensor) and isinstance(wgu, MxTensor) and len(wgu.shape) == 4, "wgu must come from pack_gate_up"
-    rows, Hp = a.shape[0], wgu.shape[2]
-    new = lambda: torch.empty(rows, Hp, dtype=torch.bfloat16, device=a.device)
-    gate, up = (new(), new()) if save_gate_up else (None, None)
-    act = _empty((rows, Hp), a.device) if quantize else new()
-    outs = dict(gate=gate, up=up, **(dict(codes=act.codes, scales=act.scales) if quantize else dict(out=act)))
-    _launch(a, wgu, Hp, True, cu_seqlens, pads, row_scale, outs, Hp)
+    assert len(a.shape) == 2, "the rows' operand is one matrix"
+    rows, Hp, device = a.shape[0], wgu.shape[2], a._data.device
+    gate = up = None
+    if save_gate_up:
+        gate, up = (torch.empty((rows, Hp), dtype=torch.bfloat16, device=device) for _ in range(2))
+    if quantize:
+        act = MxTensor._empty((rows, Hp), device)
+        outs = 0, nat.ptr(gate), nat.ptr(up), *act._at
+    else:
+        act = torch.empty((rows, Hp), dtype=torch.bfloat16, device=device)
+        outs = act.data_ptr(), nat.ptr(gate), nat.ptr(up), 0, 0
+    if Hp > 0:
+        _launch(a, wgu, Hp, 1, cu_seqlens, pads, row_scale, *outs, Hp)
     return act, gate, up
+
+
+def gateup_swiglu_bwd(d_act: torch.Tensor, a: MxTensor, wgu: MxTensor, cu_seqlens: Optional[torch.Tensor] = None, *,
+                      row_scale: Optional[torch.Tensor] = None, want_dscale: bool = False, pads: Optional[torch.Tensor] = None):
+    """Backward of :func:`gateup_swiglu` up to the products: ``(d_gate, d_up, d_scale)`` from the gradient ``d_act``
+    ``[rows, H']`` (fp32) of the activation and the operands of the forward pass, whose product is computed again: gate
+    and up need not be kept.  ``d_gate`` and ``d_up`` are bf16; ``d_scale`` (fp32 ``[rows]``, with ``want_dscale``) is
+    summed in a fixed order and zero for the rows behind the last group."""
+    assert isinstance(a, MxTensor) and isinstance(wgu, MxTensor) and len(wgu.shape) == 4, "wgu must come from pack_gate_up"
+    assert len(a.shape) == 2, "the rows' operand is one matrix"
+    rows, Hp, device = a.shape[0], wgu.shape[2], a._data.device
+    assert d_act.dtype == torch.float32 and d_act.get_device() == a._index and d_act.is_contiguous() \
+        and tuple(d_act.shape) == (rows, Hp), "d_act must be fp32 [rows, H']"
+    d_gate, d_up = (torch.empty((rows, Hp), dtype=torch.bfloat16, device=device) for _ in range(2))
+    d_scale, n = None, (wgu._rows + 255) // 256 * 2
+    parts = torch.empty((n, rows), dtype=torch.float32, device=device) if want_dscale else None
+    if Hp > 0:
+        _launch(a, wgu, Hp, 1, cu_seqlens, pads, row_scale, 0, d_gate.data_ptr(), d_up.data_ptr(), 0, 0, Hp, d_act.data_ptr(),
+                nat.ptr(parts))
+    if want_dscale:
+        d_scale = torch.empty(rows, dtype=torch.float32, device=device)
+        end = 0 if cu_seqlens is None else cu_seqlens.data_ptr() + 4 * (cu_seqlens.numel() - 1)
+        ew._rc(nat.call("mep_mx_sum_parts", parts.data_ptr(), n, rows, end, d_scale.data_ptr(), nat.stream()), "mx sum")
+    return d_gate, d_up, d_scale
 
 
 def _pack(wg, wu, wd):
@@ -274,46 +341,41 @@ class _ExpertFFN(torch.autograd.Function):
         wgu, wdq = _pack(wg, wu, wd)
         keep = any(ctx.needs_input_grad)
         xq = quantize(x, rows_ptr=None if cu_seqlens is None else cu_seqlens[-1:])
-        act, gate, up = gateup_swiglu(xq, wgu, cu_seqlens, row_scale=row_scale, save_gate_up=keep, quantize=True, pads=pads)
+        act, _, _ = gateup_swiglu(xq, wgu, cu_seqlens, row_scale=row_scale, quantize=True, pads=pads)
         # (a pass over all rows leaves none; rows that belong to no group are zeros)
         new = torch.empty if cu_seqlens is None else torch.zeros
         y = matmul(act, wdq, cu_seqlens, pads=pads, out=new(x.shape, dtype=torch.bfloat16, device=x.device))
         if keep:
-            ctx.packed, ctx.frozen = (xq, act, wgu, wdq), isinstance(wg, MxTensor)
-            ctx.shapes = None if ctx.frozen else (wg.shape, wd.shape)
-            ctx.save_for_backward(gate, up, row_scale, cu_seqlens, pads)
+            ctx.packed, ctx.shapes = (xq, act, wgu, wdq), None if isinstance(wg, MxTensor) else (wg.shape, wd.shape)
+            ctx.save_for_backward(row_scale, cu_seqlens, pads)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         xq, act, wgu, wdq = ctx.packed
-        gate, up, row_scale, cu, pads = ctx.saved_tensors
+        row_scale, cu, pads = ctx.saved_tensors
         need_x, need_g, need_u, need_d, need_s = ctx.needs_input_grad[:5]
         dy = dy.contiguous()
-        G = wgu.shape[1]
-        rows_ptr = None if cu is None else cu[-1:]
-        H, Hp = xq.shape[1], wgu.shape[2]
+        (G, Hp, H), rows_ptr = wgu.shape[1:], None if cu is None else cu[-1:]
+        bf16 = dict(dtype=torch.bfloat16, device=dy.device)
         grads = [None] * 3
-        f32 = dict(dtype=torch.float32, device=dy.device)
         if need_d:
-            g = torch.empty(G, H, Hp, **f32)
-            gemm.wgrad(dy, act.dequantize(rows_ptr=rows_ptr), cu, g, pads=pads)
-            grads[2] = g.to(torch.bfloat16).view(ctx.shapes[1])
+            grads[2] = torch.empty(G, H, Hp, **bf16)
+            gemm.wgrad(dy, act.dequantize(rows_ptr=rows_ptr), cu, grads[2], pads=pads)
+            grads[2] = grads[2].view(ctx.shapes[1])
         dx = d_scale = None
         if need_x or need_g or need_u or need_s:
-            d_act = gemm.down_dgrad(dy, wdq.dequantize().view(G, H, Hp), cu, pads=pads)
-            d_gate, d_up, d_scale = ew.swiglu_bwd(d_act, gate, up, row_scale, rows_ptr=rows_ptr, want_dscale=need_s)
+            d_act = gemm.down_dgrad(dy, wdq.dequantize().view(G, H, Hp), cu, pads=pads, fp32=True)
+            d_gate, d_up, d_scale = gateup_swiglu_bwd(d_act, xq, wgu, cu, row_scale=row_scale, want_dscale=need_s, pads=pads)
             if need_x:
                 new = torch.empty if cu is None else torch.zeros
-                dx = new(dy.shape, dtype=torch.bfloat16, device=dy.device)
+                dx = new(dy.shape, **bf16)
                 w = wgu.dequantize()
                 gemm.gateup_dgrad(d_gate, d_up, w[0], w[1], cu, out=dx, pads=pads, transposed=True)
             if need_g or need_u:
-                xv = xq.dequantize(rows_ptr=rows_ptr)
-                out = torch.empty(2, G, H, Hp, **f32)
-                gemm.wgrad2(xv, (d_gate, d_up), cu, (out[0], out[1]), pads=pads)
-                out = out.to(torch.bfloat16)
+                out = torch.empty(2, G, H, Hp, **bf16)
+                gemm.wgrad2(xq.dequantize(rows_ptr=rows_ptr), (d_gate, d_up), cu, (out[0], out[1]), pads=pads)
                 grads[:2] = (out[i].view(ctx.shapes[0]) for i in range(2))
         return dx, grads[0], grads[1], grads[2], d_scale, None, None
 
@@ -328,7 +390,7 @@ def expert_ffn(x: torch.Tensor, wg, wu, wd, cu_seqlens: Optional[torch.Tensor] =
 
     The gradients are those of the formula with the quantised operands in it; the quantisation itself is passed
     straight through: ``d Wg = x^T d_gate`` has the quantised ``x``, ``d x`` the quantised weights.  What forward keeps
-    are the operands in 4 bits, gate and up in bf16.  Sums run in fp32; ``d act``, ``d gate`` and ``d up`` are
+    are the operands in 4 bits; backward computes gate and up again.  Sums run in fp32; ``d gate`` and ``d up`` are
     rounded to bf16, as operands of the bf16 products of :mod:`.gemm`, and the results once more.
 
     Rows that belong to no group get zeros, in ``y`` and in ``x``'s gradient.  For gradients H must be a multiple of 128

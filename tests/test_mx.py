@@ -282,6 +282,88 @@ def test_gateup_padding_rows():
     assert torch.equal(q.dequantize(), mx.quantize(plain[0]).dequantize())
 
 
+@gpu
+@pytest.mark.parametrize("H,Hp", [(256, 256), (64, 8), (1000, 515), (2048, 640)])
+@pytest.mark.parametrize("sizes", GROUPS)
+def test_gateup_swiglu_backward(sizes, H, Hp):
+    """d gate, d up and d scale against the formulas on the quantised operands in 64 bits.  Gate and up are fp32 sums, off
+    by dg and du; the formulas' slopes in them are at most 1.1 and 0.5 (silu and its derivative)."""
+    from moonep_b200.ops import mx
+    gen = _gen(17)
+    rows, G = sum(sizes), len(sizes)
+    x = torch.randn(rows, H, generator=gen).bfloat16()
+    wg, wu = ((torch.randn(G, H, Hp, generator=gen) * 2 * H ** -0.5).bfloat16() for _ in range(2))
+    scale, d_act = torch.rand(rows, generator=gen) + 0.1, torch.randn(rows, Hp, generator=gen)
+    ends = _ends(sizes)
+    gv, uv = (ox.quantise(w.transpose(1, 2).contiguous()) for w in (wg, wu))
+    _, gate, up, dg, du, _ = _gated_ref(ox.quantise(x), gv, uv, ends.tolist(), scale.double())
+    sig = torch.sigmoid(gate)
+    d = d_act.double()
+    want_s = d * gate * sig * up
+    ds = d * scale.double()[:, None]
+    want_g, want_u = ds * up * sig * (1 + gate * (1 - sig)), ds * gate * sig
+    slack = 1e-5 * (1 + gate.abs())              # exp, and a few fp32 steps
+    off_g = ds.abs() * (1.1 * du + 0.5 * up.abs() * dg + 0.5 * du * dg + up.abs() * 1.1 * slack)
+    off_u = ds.abs() * (1.1 * dg + slack * gate.abs())
+    off_s = (d.abs() * (1.1 * dg * up.abs() + (gate * sig).abs() * du + 1.1 * dg * du)).sum(1) \
+        + (want_s.abs() * (slack + Hp * 2.0 ** -24)).sum(1)
+    xq, w = mx.quantize(x.cuda()), mx.pack_gate_up(wg.cuda(), wu.cuda())
+    got = mx.gateup_swiglu_bwd(d_act.cuda(), xq, w, ends.cuda(), row_scale=scale.cuda(), want_dscale=True)
+    for y, ref, tol in zip(got, (want_g, want_u, want_s.sum(1)), (HALF * want_g.abs() + off_g, HALF * want_u.abs() + off_u, off_s)):
+        assert float(((y.cpu().double() - ref).abs() - tol).max()) <= 1e-30
+    again = mx.gateup_swiglu_bwd(d_act.cuda(), xq, w, ends.cuda(), row_scale=scale.cuda())
+    assert again[2] is None and torch.equal(again[0], got[0]) and torch.equal(again[1], got[1])
+
+
+@gpu
+def test_gateup_backward_padding_rows():
+    from moonep_b200.ops import mx
+    gen = _gen(18)
+    H, Hp, ends = 256, 160, _ends([128, 64, 192]).cuda()
+    pads = torch.tensor([[100, 28], [129, 63], [192, 0]], dtype=torch.int32).cuda()
+    x = torch.randn(384 + 30, H, generator=gen).bfloat16()
+    x[100:128], x[129:192] = 0, 0
+    d_act = torch.randn(384 + 30, Hp, generator=gen).cuda()
+    bad = d_act.clone()
+    bad[100:128], bad[129:192], bad[384:] = float("nan"), float("nan"), float("nan")
+    wg, wu = ((torch.randn(3, H, Hp, generator=gen) * H ** -0.5).bfloat16().cuda() for _ in range(2))
+    xq, w = mx.quantize(x.cuda()), mx.pack_gate_up(wg, wu)
+    plain = mx.gateup_swiglu_bwd(d_act, xq, w, ends, want_dscale=True)
+    padded = mx.gateup_swiglu_bwd(bad, xq, w, ends, want_dscale=True, pads=pads)
+    for a, b in zip(plain, padded):
+        assert torch.equal(a[:384], b[:384])
+    assert (padded[2][384:] == 0).all()
+
+
+# ---- the bf16 products that the FFN's backward pass needs ------------------------------------------
+@gpu
+@pytest.mark.parametrize("G,H,Hp", [(3, 256, 72), (2, 384, 256), (1, 128, 8)])
+def test_bf16_products_of_the_backward_pass(G, H, Hp):
+    from moonep_b200.ops import gemm
+    gen = _gen(19)
+    sizes = [64, 0, 192][:G] if G > 1 else [100]
+    ends, rows = _ends(sizes), sum(sizes)
+    dy, wd = torch.randn(rows, H, generator=gen).bfloat16(), torch.randn(G, H, Hp, generator=gen).bfloat16()
+    cu = None if G == 1 else ends.cuda()
+    got = gemm.down_dgrad(dy.cuda(), wd.cuda(), cu, fp32=True)
+    ref, mag = ox.product(dy.double(), wd.double().transpose(1, 2), ends.tolist())
+    assert got.dtype == torch.float32 and float(((got.cpu().double() - ref).abs() - (H + 2) * 2.0 ** -24 * mag).max()) <= 0
+    # gate and up weights stored [G, H', H]
+    d1, d2 = (torch.randn(rows, Hp, generator=gen).bfloat16().cuda() for _ in range(2))
+    w1, w2 = (torch.randn(G, H, Hp, generator=gen).bfloat16().cuda() for _ in range(2))
+    t = [w.transpose(1, 2).contiguous() for w in (w1, w2)]
+    assert torch.equal(gemm.gateup_dgrad(d1, d2, *t, cu, transposed=True), gemm.gateup_dgrad(d1, d2, w1, w2, cu))
+    # grads in bf16 are the fp32 ones rounded, those of empty groups zero
+    a = dy.cuda()
+    f32 = [torch.empty(G, H, Hp, device="cuda") for _ in range(3)]
+    b16 = [torch.full((G, H, Hp), 7.0, device="cuda", dtype=torch.bfloat16) for _ in range(3)]
+    for out in (f32, b16):
+        gemm.wgrad(a, d1, cu, out[0])
+        gemm.wgrad2(a, (d1, d2), cu, (out[1], out[2]))
+    for x, y in zip(f32, b16):
+        assert torch.equal(x.bfloat16(), y)
+
+
 # ---- the FFN -----------------------------------------------------------------------------------
 def _ffn_ref(x, wg, wu, wd, ends, scale, dy=None):
     """y, and with dy the gradients of x, wg, wu, wd, scale, by the formulas.  (The activation is rounded to bf16, then
@@ -315,7 +397,7 @@ def _near(got, ref, tol):
 # Independent roundings to bf16 are off by 2^-9 / sqrt(3) of a value in the mean square, at most 2^-8.  y has one; an
 # activation near a border may be quantised to either side (relative difference of the sums 2^-20, borders some 0.3
 # apart: one in 10^5, by a third of its value: 2^-10 in the norm).  A gradient of x passes the roundings of
-# d act, gate / up, d gate / d up, the bf16 weights exactly, and its own: four.
+# d act, gate / up, d gate / d up, the bf16 weights exactly, and its own: four.  (Now d act, gate and up are not rounded.)
 Y_TOL, GRAD_TOL = 2 * HALF, 4 * HALF
 
 
@@ -465,6 +547,9 @@ def test_refusals():
         lambda: mx.gateup_swiglu(q, qw, ends),
         lambda: mx.gateup_swiglu(q, gu, ends, row_scale=torch.ones(7, device="cuda")),
         lambda: mx.gateup_swiglu(q, gu, ends, row_scale=torch.ones(8, **bf)),
+        lambda: mx.gateup_swiglu_bwd(torch.zeros(8, 32, **bf), q, gu, ends),
+        lambda: mx.gateup_swiglu_bwd(torch.zeros(7, 32, device="cuda"), q, gu, ends),
+        lambda: mx.gateup_swiglu_bwd(torch.zeros(8, 32, device="cuda"), q, qw, ends),
         lambda: mx.expert_ffn(x.float(), w, w, w, ends),
         lambda: mx.expert_ffn(x, w, w, w, ends),
         lambda: mx.expert_ffn(x, gu, w, qw, ends),
