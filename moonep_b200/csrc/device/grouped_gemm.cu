@@ -397,7 +397,7 @@ static int launch_dense_f32(const DenseParams& dp, cudaStream_t stream) {
 template <int EPI, int MAX_N>
 static int launch_mx(const MxParams& p, int grid, cudaStream_t stream) {
   static PairLaunch once;
-  return launch_pair((const void*)ep_mx_gemm_kernel<EPI, MAX_N>, once, p, grid, MXG_THREADS,
+  return launch_pair((const void*)ep_mx_gemm_kernel<EPI, MAX_N>, once, p, grid, mxg_threads<EPI>(),
                      mxg_stages<EPI, MAX_N>() * mxg_stage(MAX_N) + 1024, false, stream);
 }
 template <int EPI>

@@ -16,7 +16,7 @@
 //
 //   warp 0  TMA producer
 //   warp 1  MMA issuer
-//   warps 2..5, 6..9 epilogue, two sets of four, as in ep_token_gemm_kernel
+//   warps 2..  epilogue, two or three sets of four, as in ep_token_gemm_kernel
 //
 // SwiGLU: gate and up columns come packed in turns of 16 rows, so that a warp's 32 rows of tensor memory hold both of 16
 // activations: read as two fragments of 16 rows, gate and up of an element meet in one thread's registers, in fp32.
@@ -38,8 +38,6 @@ constexpr int MXG_BK = 256;                      // elements of a k-block: 128 b
 constexpr int MXG_MAX_STAGES = 10;
 constexpr int MXG_W_BYTES = 128 * 128;
 constexpr int MXG_S_BYTES = 2 * MX_ATOM_BYTES;   // scales of 128 rows and one k-block
-constexpr int MXG_SETS = 2;
-constexpr int MXG_THREADS = 64 + MXG_SETS * 128;
 constexpr int MXG_BOXES = 5;
 __host__ __device__ constexpr int mxg_box_rows(int b) { return b == 0 ? 16 : b == 4 ? MXG_MAX_N / 2 : 32 * b; }
 // Shared memory of a stage whose tiles have up to n tokens: weights, half of the tokens (in whole swizzle atoms), scales.
@@ -71,11 +69,14 @@ struct MxParams {
   unsigned long long timeout_ns;
 };
 
+// Sets of four epilogue warps.
+template <int EPI> constexpr int mxg_sets() { return EPI == MX_EPI_SWIGLU || EPI == MX_EPI_SWIGLU_BWD ? 3 : 2; }
+template <int EPI> constexpr int mxg_threads() { return 64 + mxg_sets<EPI>() * 128; }
 // Shared memory that the kernel declares itself: staged tokens, group tables, scales of two tiles, barriers (rounded up).
 template <int EPI> constexpr int mxg_token_row() { return (EPI == MX_EPI_SWIGLU_SAVE ? 384 : EPI == MX_EPI_SWIGLU ? 128 : 256) + 16; }
 template <int EPI> constexpr int mxg_static_smem() {
-  return MXG_SETS * TG_CHUNK * mxg_token_row<EPI>() + (3 * MAX_GROUPS + 1) * 4 + (EPI == MX_EPI_BF16 ? 8 : 2 * MXG_MAX_N * 4) +
-         (EPI == MX_EPI_SWIGLU_BWD ? MXG_SETS * 4 * TG_CHUNK * 4 : 0) + 512;
+  return mxg_sets<EPI>() * TG_CHUNK * mxg_token_row<EPI>() + (3 * MAX_GROUPS + 1) * 4 + (EPI == MX_EPI_BF16 ? 8 : 2 * MXG_MAX_N * 4) +
+         (EPI == MX_EPI_SWIGLU_BWD ? mxg_sets<EPI>() * 4 * TG_CHUNK * 4 : 0) + 512;
 }
 
 // Slots of the ring: as many as the device's shared memory has room for beside these.
@@ -116,9 +117,18 @@ __host__ __device__ constexpr uint32_t make_instr_desc_mxf4(int M, int N, int sc
          ((uint32_t)(M >> 4) << 24) | ((uint32_t)scale_byte << 29);
 }
 
+// 1 / (1 + e^-x) to a few units in the last place.  (With the exact division gate and up of the decoder's experts, whose
+// epilogue is as long as their reduction, take 126 us, else MARK.)
+__device__ __forceinline__ float mx_sigmoid(float x) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-x)));
+  return r;
+}
+
 template <int EPI, int MAX_N>
-__global__ void __launch_bounds__(MXG_THREADS, 1)
+__global__ void __launch_bounds__(mxg_threads<EPI>(), 1)
 ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
+  constexpr int SETS = mxg_sets<EPI>();
   constexpr int NST = mxg_stages<EPI, MAX_N>(), STAGE = mxg_stage(MAX_N), T_BYTES = mxg_t_bytes(MAX_N);
   constexpr bool GATED = EPI != MX_EPI_BF16, SAVE = EPI == MX_EPI_SWIGLU_SAVE, BWD = EPI == MX_EPI_SWIGLU_BWD;
   constexpr int TOK_ROW = mxg_token_row<EPI>();     // bytes of a staged token
@@ -133,8 +143,8 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
   __shared__ int s_abort;
   __shared__ int s_end[MAX_GROUPS], s_span[MAX_GROUPS];
   __shared__ int s_prefix[MAX_GROUPS + 1];
-  __shared__ __align__(128) uint8_t s_stage[MXG_SETS][TG_CHUNK * TOK_ROW];
-  __shared__ float s_part[BWD ? MXG_SETS : 1][BWD ? 4 : 1][BWD ? TG_CHUNK : 1];     // sums over a quarter's columns
+  __shared__ __align__(128) uint8_t s_stage[SETS][TG_CHUNK * TOK_ROW];
+  __shared__ float s_part[BWD ? SETS : 1][BWD ? 4 : 1][BWD ? TG_CHUNK : 1];     // sums over a quarter's columns
   __shared__ float s_scale[GATED ? 2 : 1][GATED ? MXG_MAX_N : 1];
 
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -145,7 +155,7 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
     if (lane == 0) {
       // both CTAs' loads count on the leader's full barrier, on which only its producer arrives
       for (int s = 0; s < NST; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-      for (int a = 0; a < 2; ++a) { mbar_init(&acc_full[a], 1); mbar_init(&acc_empty[a], 8 * MXG_SETS); }
+      for (int a = 0; a < 2; ++a) { mbar_init(&acc_full[a], 1); mbar_init(&acc_empty[a], 8 * SETS); }
       mbar_fence_init();
       s_abort = 0;
     }
@@ -154,7 +164,7 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
   }
   // Group tables: ends, and rows with tokens counted from the multiple of 32 at or before the first.  (One round of loads
   // for all groups, 1 us; the padding ranges looked up in the scan below and again for every tile cost 2 - 4 us a launch.)
-  for (int g = tid; g < p.ngroups; g += MXG_THREADS) {
+  for (int g = tid; g < p.ngroups; g += mxg_threads<EPI>()) {
     // (no row outside the tensors is stored, whatever cu_seqlens says)
     auto clamped = [&](int end) { return min(max(end, 0), p.total_rows); };
     const int start = g == 0 || p.cu_seqlens == nullptr ? 0 : clamped(p.cu_seqlens[g - 1]);
@@ -298,10 +308,10 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
       }
     }
   } else {
-    // ========= epilogue: two sets of four warps, each warp one quarter of the CTA's weight rows =========
+    // ========= epilogue: sets of four warps, each warp one quarter of the CTA's weight rows =========
     const int q = warp & 3, set = (warp - 2) >> 2;
     const int te = tid - 64 - set * 128;                    // 0..127
-    const int step = MXG_SETS * TG_CHUNK;
+    const int step = SETS * TG_CHUNK;
     int tile_n = 0, at = 0;
     uint8_t* const sb = s_stage[set];
     // this thread's row of the matrices that its warp stores: token 8 (lane / 16) + lane % 8, columns 8 (lane / 8 % 2)
@@ -312,8 +322,8 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
       const MxTile t = get(id, at);
       const int acc = tile_n & 1;
       // this set's chunks start at tokens first, first + step, ...; the sets change places from tile to tile, so that
-      // tiles of up to 32 tokens keep both busy
-      const int first = ((set + tile_n) & 1) * TG_CHUNK, my_tok = (te >> 5) * step + first + (te & 31);
+      // tiles of few tokens keep all of them busy
+      const int first = (set + tile_n) % SETS * TG_CHUNK, my_tok = (te >> 5) * step + first + (te & 31);
       if constexpr (GATED) {       // (published by the barriers below)
         for (int i = my_tok; i < t.n; i += 4 * step) {
           const int r = t.row0 + i;
@@ -382,7 +392,7 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const float g = __uint_as_float(r[2 * i + e]), u = __uint_as_float(r[16 + 2 * i + e]);
-              const float sig = 1.f / (1.f + __expf(-g)), d = da[2 * i + e];
+              const float sig = mx_sigmoid(g), d = da[2 * i + e];
               const float ds = d * s_scale[acc][c + 8 * (i >> 1) + 2 * (lane & 3) + e];
               // (columns behind the last have whatever lies behind the weights)
               part[2 * (i >> 1) + e] += col + 8 * (i & 1) < p.N ? d * (g * sig) * u : 0.f;
@@ -408,7 +418,7 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const float g = __uint_as_float(r[2 * i + e]), u = __uint_as_float(r[16 + 2 * i + e]);
-              a[e] = g / (1.f + __expf(-g)) * u * s_scale[acc][c + 8 * (i >> 1) + 2 * (lane & 3) + e];
+              a[e] = g * mx_sigmoid(g) * u * s_scale[acc][c + 8 * (i >> 1) + 2 * (lane & 3) + e];
             }
             pa[i] = pack(a[0], a[1]);
           }
@@ -507,7 +517,7 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
       {      // padding rows that no tile computes
         constexpr int V = GATED ? 8 : 16;                    // vectors of this CTA's columns in a row
         const int f = (te & (V - 1)) * 8, col0 = (GATED ? t.m / 2 : t.m) + V * 8 * crank + f;
-        for (int row = t.hi + (te + 128 * set) / V; row < t.zero_to; row += 128 * MXG_SETS / V) {
+        for (int row = t.hi + (te + 128 * set) / V; row < t.zero_to; row += 128 * SETS / V) {
           const uint4 zero = make_uint4(0, 0, 0, 0);
           const long long off = (long long)row * p.ldc + col0;
           if constexpr (BWD) {
