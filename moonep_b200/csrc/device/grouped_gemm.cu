@@ -204,7 +204,7 @@ struct GemmDesc {
 // Product of microscaled 4-bit operands: tokens [rows][K], weights [ngroups][w_rows][K] (`gated`: gate and up packed).
 struct MxDesc {
   const void *a_codes, *a_scales, *w_codes, *w_scales;
-  int32_t rows, K, ngroups, w_rows, N, gated;
+  int32_t rows, K, ngroups, w_rows, N, gated, zero_tail, unused;
   const int32_t* cu_seqlens;
   const int32_t* pads;
   const float* row_scale;
@@ -611,6 +611,15 @@ int mep_gemm_launch(const GemmDesc* d, cudaStream_t stream) {
 
 int mep_mx_desc_bytes() { return (int)sizeof(MxDesc); }
 
+// Rows of `bytes` bytes of out [rows] from *rows_ptr on become zeros.
+int mep_mx_zero_tail(void* out, int rows, int64_t bytes, const int32_t* rows_ptr, cudaStream_t stream) {
+  if (rows < 0 || bytes < 0 || bytes % 16 != 0 || ((uintptr_t)out & 15) != 0) return fail(-1, "mx zero: %d rows", rows);
+  if (rows == 0 || bytes == 0) return 0;
+  ep_mx_zero_tail_kernel<<<148, 256, 0, stream>>>((uint8_t*)out, rows, bytes, rows_ptr);
+  MEP_CUDA_OK(cudaGetLastError());
+  return 0;
+}
+
 // sum[r] = parts[0][r] + parts[1][r] + ..., zero for the rows behind *rows_ptr.
 int mep_mx_sum_parts(const float* parts, int n, int rows, const int32_t* rows_ptr, float* sum, cudaStream_t stream) {
   if (n < 1 || rows < 0) return fail(-1, "mx sum: %d x %d", n, rows);
@@ -647,6 +656,7 @@ int mep_mx_gemm_launch(const MxDesc* d, cudaStream_t stream) {
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  p.zero_tail = d->zero_tail;
   p.d_act = d->d_act; p.d_scale = d->d_scale;
   if (d->d_act != nullptr) {
     if (!d->gated || p.gate == nullptr || p.up == nullptr) return fail(-3, "mx product: the backward pass writes both gradients");

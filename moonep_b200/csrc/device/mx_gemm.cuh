@@ -63,13 +63,16 @@ struct MxParams {
   int vec_out;
   const float* row_scale;
   const float* d_act;              // backward: gradient of the activation, [total_rows][N]
+  int zero_tail;                   // rows behind the last group become zeros
   float* d_scale;                  // parts of the scales' gradients, [CTA's columns][total_rows], or null
   long long ldc;
   int32_t* status;
   unsigned long long timeout_ns;
 };
 
-// Sets of four epilogue warps.
+// Sets of four epilogue warps.  (Gate and up of the decoder's experts, 32768 rows, 2048 -> 768: two sets 86 us, three 78;
+// backward 125, 117.  Four cost a slot of the ring: 32 x 1024 rows, 7168 -> 2048 324 us, 338.  Plain products, whose
+// epilogue is shorter: two 207 us, three 211.)
 template <int EPI> constexpr int mxg_sets() { return EPI == MX_EPI_SWIGLU || EPI == MX_EPI_SWIGLU_BWD ? 3 : 2; }
 template <int EPI> constexpr int mxg_threads() { return 64 + mxg_sets<EPI>() * 128; }
 // Shared memory that the kernel declares itself: staged tokens, group tables, scales of two tiles, barriers (rounded up).
@@ -118,7 +121,7 @@ __host__ __device__ constexpr uint32_t make_instr_desc_mxf4(int M, int N, int sc
 }
 
 // 1 / (1 + e^-x) to a few units in the last place.  (With the exact division gate and up of the decoder's experts, whose
-// epilogue is as long as their reduction, take 126 us, else MARK.)
+// epilogue is as long as their reduction, took 134 us, so 86.)
 __device__ __forceinline__ float mx_sigmoid(float x) {
   float r;
   asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-x)));
@@ -540,6 +543,13 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
       }
     }
   }
+  if constexpr (EPI == MX_EPI_BF16) {
+    if (p.zero_tail && warp >= 2) {      // a warp a row
+      const int warps = 4 * SETS;
+      for (int row = s_end[p.ngroups - 1] + (int)blockIdx.x * warps + warp - 2; row < p.total_rows; row += (int)gridDim.x * warps)
+        for (int c = lane * 8; c < p.N; c += 256) store8(p.out + (long long)row * p.ldc + c, make_uint4(0, 0, 0, 0), p.N - c, p.vec_out != 0);
+    }
+  }
   // ---- teardown: everything joins, in-flight work is given time to land on an abort ----------
   tc_fence_before();
   __syncthreads();
@@ -563,6 +573,14 @@ __global__ void __launch_bounds__(256) ep_mx_sum_parts_kernel(const float* __res
   if (r < used)
     for (int i = 0; i < n; ++i) s += parts[(long long)i * rows + r];
   sum[r] = s;
+}
+
+// Rows of `bytes` bytes (a multiple of 16) from *rows_ptr on become zeros.
+__global__ void __launch_bounds__(256) ep_mx_zero_tail_kernel(uint8_t* __restrict__ out, int rows, long long bytes,
+                                                              const int32_t* __restrict__ rows_ptr) {
+  const long long from = (long long)max(0, min(*rows_ptr, rows)) * bytes, to = rows * bytes, step = (long long)gridDim.x * 256 * 16;
+  for (long long i = from + ((long long)blockIdx.x * 256 + threadIdx.x) * 16; i < to; i += step)
+    *reinterpret_cast<uint4*>(out + i) = make_uint4(0, 0, 0, 0);
 }
 
 }  // namespace mep

@@ -49,13 +49,12 @@ __device__ __forceinline__ float2 mx_times(const MxPair<__nv_bfloat16>& x, float
   return __bfloat1622float2(y);
 }
 
-// Where row r of the output goes: as it is, or as gate (1) / up (2) column of the packed pair, sixteen of either in turn.
-__device__ __forceinline__ int mx_out_row(int r, int interleave) {
-  return interleave == 0 ? r : (r >> 4) * 32 + (r & 15) + (interleave == 2 ? 16 : 0);
-}
+// Row of a packed pair of a gate (up = 0) and an up projection: sixteen of either in turn.
+__device__ __forceinline__ int mx_pair_row(int r, int up) { return (r >> 4) * 32 + (r & 15) + 16 * up; }
 
 struct MxQuantParams {
   const void* x;
+  const void* x2;               // the up projection of a pair (x: gate), along the columns; or null
   long long batch, stride;      // elements between matrices, and between rows of x
   int mats, rows, cols;         // of x
   int out_rows;                 // rows of a matrix of the output (codes)
@@ -63,7 +62,6 @@ struct MxQuantParams {
   uint8_t* codes;
   uint8_t* scales;
   const int32_t* rows_ptr;      // rows of x that hold something, on the device; or null
-  int interleave;
   int phases;                   // 4: token rows, whose scales are stored at four phases
 };
 
@@ -105,10 +103,9 @@ __global__ void __launch_bounds__(MXQ_WARPS * 32) ep_mx_quant_rows_kernel(const 
   const unsigned lines = (unsigned)p.mats * (unsigned)rows;
   for (unsigned line = blockIdx.x * MXQ_WARPS + warp; line < lines; line += gridDim.x * MXQ_WARPS) {
     const int mat = p.mats > 1 ? (int)(line / (unsigned)rows) : 0, row = (int)(line - (unsigned)mat * (unsigned)rows);
-    const int r = mx_out_row(row, p.interleave);
     const T* x = (const T*)p.x + mat * p.batch + row * p.stride;
-    uint8_t* codes = p.codes + ((long long)mat * p.out_rows + r) * p.code_bytes;
-    uint32_t* scales = mx_scale_row(p, mat, r, lane & 15);       // of this lane's phase, if it has one
+    uint8_t* codes = p.codes + ((long long)mat * p.out_rows + row) * p.code_bytes;
+    uint32_t* scales = mx_scale_row(p, mat, row, lane & 15);       // of this lane's phase, if it has one
     for (int c0 = blockIdx.y * 256 * MXQ_DEPTH; c0 < p.cols; c0 += gridDim.y * 256 * MXQ_DEPTH) {
       MxEight<T> raw[MXQ_DEPTH];
 #pragma unroll
@@ -155,9 +152,14 @@ __global__ void __launch_bounds__(256, 2) ep_mx_quant_cols_kernel(const __grid_c
   __shared__ __align__(4) uint8_t s_scale[COLS][8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r0 = blockIdx.y * MXT_ROWS, c0 = blockIdx.x * COLS;
-  for (int m = blockIdx.z; m < p.mats; m += gridDim.z) {
+  // (a pair's last turn of sixteen is stored whole: zeros behind the last column)
+  const bool pair = p.x2 != nullptr;
+  const int cols = pair ? (p.cols + 15) & ~15 : p.cols;
+  for (int z = blockIdx.z; z < (pair ? 2 : 1) * p.mats; z += gridDim.z) {
+    const int up = z >= p.mats ? 1 : 0, m = z - up * p.mats;
     const int c = c0 + 2 * NP * lane, rw = r0 + warp * MX_BLOCK;
-    const T* x = (const T*)p.x + m * p.batch + (long long)rw * p.stride + c;
+    const T* x = (const T*)(up ? p.x2 : p.x) + m * p.batch + (long long)rw * p.stride + c;
+    auto out_row = [&](int n) { return pair ? mx_pair_row(c0 + n, up) : c0 + n; };
     Piece raw[MX_BLOCK];
 #pragma unroll
     for (int i = 0; i < MX_BLOCK; ++i) {
@@ -200,13 +202,13 @@ __global__ void __launch_bounds__(256, 2) ep_mx_quant_cols_kernel(const __grid_c
     __syncthreads();
     for (int i = threadIdx.x; i < COLS * 8; i += 256) {       // 16 bytes of a column's codes
       const int n = i >> 3, k = r0 / 2 + (i & 7) * 16;
-      if (c0 + n < p.cols && k < p.code_bytes)
-        *reinterpret_cast<uint4*>(p.codes + ((long long)m * p.out_rows + mx_out_row(c0 + n, p.interleave)) * p.code_bytes + k) =
+      if (c0 + n < cols && k < p.code_bytes)
+        *reinterpret_cast<uint4*>(p.codes + ((long long)m * p.out_rows + out_row(n)) * p.code_bytes + k) =
             *reinterpret_cast<const uint4*>(s_codes + n * 128 + ((i & 7) ^ (n / (2 * NP) & 7)) * 16);
     }
     for (int i = threadIdx.x; i < 2 * COLS * p.phases; i += 256) {
       const int n = (i >> 1) % COLS, ka = r0 / MX_ATOM_K + (i & 1);
-      uint32_t* scales = c0 + n < p.cols && ka < p.k_atoms ? mx_scale_row(p, m, mx_out_row(c0 + n, p.interleave), i / (2 * COLS)) : nullptr;
+      uint32_t* scales = c0 + n < cols && ka < p.k_atoms ? mx_scale_row(p, m, out_row(n), i / (2 * COLS)) : nullptr;
       if (scales != nullptr) scales[(long long)ka * (MX_ATOM_BYTES / 4)] = *reinterpret_cast<const uint32_t*>(&s_scale[n][4 * (i & 1)]);
     }
     __syncthreads();
@@ -216,11 +218,11 @@ __global__ void __launch_bounds__(256, 2) ep_mx_quant_cols_kernel(const __grid_c
 struct MxDequantParams {
   const uint8_t* codes;
   const uint8_t* scales;
-  int mats, rows, cols;         // of the values; `rows` of gate or up where they are a packed pair
+  int mats, rows, cols;         // of the values; `rows` of gate or up where they are a packed pair, which has both mats times
   int in_rows, code_bytes, k_atoms, row_atoms;
   void* out;                    // [mats][rows][cols]
   const int32_t* rows_ptr;
-  int interleave;
+  int pair;                     // the values of the gate projections, then of the up projections
 };
 
 // A lane takes eight values of a row, a warp MXD_DEPTH times 256.  (Exact in bf16 but for what a bf16 subnormal rounds,
@@ -231,13 +233,14 @@ template <class T, bool VEC>
 __global__ void __launch_bounds__(MXQ_WARPS * 32) ep_mx_dequant_kernel(const __grid_constant__ MxDequantParams p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rows = p.rows_ptr ? max(0, min(*p.rows_ptr, p.rows)) : p.rows;
-  const unsigned lines = (unsigned)p.mats * (unsigned)rows;
+  const unsigned lines = (unsigned)(p.pair ? 2 * p.mats : p.mats) * (unsigned)rows;
   for (unsigned line = blockIdx.x * MXQ_WARPS + warp; line < lines; line += gridDim.x * MXQ_WARPS) {
-    const int mat = p.mats > 1 ? (int)(line / (unsigned)rows) : 0, row = (int)(line - (unsigned)mat * (unsigned)rows);
-    const int r = mx_out_row(row, p.interleave);
+    const int out_mat = lines > (unsigned)rows ? (int)(line / (unsigned)rows) : 0, row = (int)(line - (unsigned)out_mat * (unsigned)rows);
+    const int up = out_mat >= p.mats ? 1 : 0, mat = out_mat - up * p.mats;
+    const int r = p.pair ? mx_pair_row(row, up) : row;
     const uint8_t* codes = p.codes + ((long long)mat * p.in_rows + r) * p.code_bytes;
     const uint8_t* scales = p.scales + (long long)mat * p.row_atoms * p.k_atoms * MX_ATOM_BYTES + mx_scale_offset(r, 0, p.k_atoms);
-    T* out = (T*)p.out + ((long long)mat * p.rows + row) * p.cols;
+    T* out = (T*)p.out + ((long long)out_mat * p.rows + row) * p.cols;
     if constexpr (!VEC) {        // rows start anywhere: neighbouring lanes take neighbouring elements
       for (int c0 = blockIdx.y * 256 * MXD_DEPTH + lane; c0 < p.cols; c0 += gridDim.y * 256 * MXD_DEPTH) {
 #pragma unroll 2
@@ -302,10 +305,10 @@ template <class T>
 static int mx_quant(const MxQuantParams& p, bool along_cols, cudaStream_t stream) {
   const bool rows16 = (uintptr_t)p.x % 16 == 0 && (p.stride * sizeof(T)) % 16 == 0 && (p.batch * sizeof(T)) % 16 == 0 && p.cols % 8 == 0;
   constexpr int lane_cols = 2 * mxt_pairs<T>(), block_cols = 32 * lane_cols;
-  const bool pieces = (uintptr_t)p.x % 8 == 0 && p.stride % lane_cols == 0 && p.batch % lane_cols == 0 && p.cols % lane_cols == 0;
+  const bool pieces = ((uintptr_t)p.x | (uintptr_t)p.x2) % 8 == 0 && p.stride % lane_cols == 0 && p.batch % lane_cols == 0 && p.cols % lane_cols == 0;
   if (along_cols) {
     const dim3 grid((unsigned)((p.cols + block_cols - 1) / block_cols), (unsigned)((p.rows + MXT_ROWS - 1) / MXT_ROWS),
-                    (unsigned)(p.mats < 65535 ? p.mats : 65535));
+                    (unsigned)(p.mats < 32767 ? (p.x2 ? 2 : 1) * p.mats : 65534));
     if (grid.y > 65535) return fail(-5, "mx quantise: %d rows are too many along the last but one axis", p.rows);
     if (pieces) ep_mx_quant_cols_kernel<T, true><<<grid, 256, 0, stream>>>(p);
     else ep_mx_quant_cols_kernel<T, false><<<grid, 256, 0, stream>>>(p);
@@ -326,38 +329,39 @@ extern "C" {
 
 // x [mats][rows][cols] of `type` (bf16, fp16, fp32), `batch` and `stride` elements apart.  along_cols = 0: blocks along the
 // columns, output rows are x's; 1: blocks along the rows, output rows are x's columns.  out_rows: rows of an output matrix.
-// phases = 4 (one matrix): scales for token rows, else 1.
-int mep_mx_quantize(const void* x, int type, int64_t batch, int64_t stride, int mats, int rows, int cols, int along_cols,
-                    int interleave, int out_rows, int phases, const int32_t* rows_ptr, void* codes, void* scales, cudaStream_t stream) {
+// phases = 4 (one matrix): scales for token rows, else 1.  x2 (along_cols = 1): the up projection packed with x, the gate.
+int mep_mx_quantize(const void* x, const void* x2, int type, int64_t batch, int64_t stride, int mats, int rows, int cols, int along_cols,
+                    int out_rows, int phases, const int32_t* rows_ptr, void* codes, void* scales, cudaStream_t stream) {
   if (mats < 0 || rows < 0 || cols < 0 || cols > 0x7F000000 || (int64_t)mats * rows > 0x7FFFFFFF)
     return fail(-1, "mx quantise: %d x %d x %d elements", mats, rows, cols);
+  if (x2 && (!along_cols || phases != 1)) return fail(-2, "mx quantise: a pair is packed along the columns");
   if (along_cols && rows_ptr) return fail(-2, "mx quantise: a device row count goes with blocks along the rows");
   if (phases != 1 && (phases != MX_PHASES || mats > 1)) return fail(-4, "mx quantise: %d phases of %d matrices", phases, mats);
   if (mats == 0 || rows == 0 || cols == 0) return 0;
   MxQuantParams p;
   const int K = along_cols ? rows : cols;
-  p.x = x; p.batch = batch; p.stride = stride; p.mats = mats; p.rows = rows; p.cols = cols;
+  p.x = x; p.x2 = x2; p.batch = batch; p.stride = stride; p.mats = mats; p.rows = rows; p.cols = cols;
   p.out_rows = out_rows; p.code_bytes = (K + MX_BLOCK - 1) / MX_BLOCK * (MX_BLOCK / 2);
   p.k_atoms = mx_atoms(K); p.row_atoms = mx_atoms(out_rows);
-  p.codes = (uint8_t*)codes; p.scales = (uint8_t*)scales; p.rows_ptr = rows_ptr; p.interleave = interleave; p.phases = phases;
+  p.codes = (uint8_t*)codes; p.scales = (uint8_t*)scales; p.rows_ptr = rows_ptr; p.phases = phases;
   if (type == MX_BF16) return mx_quant<__nv_bfloat16>(p, along_cols != 0, stream);
   if (type == MX_FP16) return mx_quant<__half>(p, along_cols != 0, stream);
   if (type == MX_FP32) return mx_quant<float>(p, along_cols != 0, stream);
   return fail(-3, "mx quantise: unknown type %d", type);
 }
 
-// The values [mats][rows][cols] in bf16, or fp32.
-int mep_mx_dequantize(const void* codes, const void* scales, int mats, int rows, int cols, int interleave, int in_rows,
+// The values [mats][rows][cols] in bf16, or fp32; of a pair [2][mats][rows][cols].
+int mep_mx_dequantize(const void* codes, const void* scales, int mats, int rows, int cols, int pair, int in_rows,
                       const int32_t* rows_ptr, int fp32, void* out, cudaStream_t stream) {
-  if (mats < 0 || rows < 0 || cols < 0 || cols > 0x7F000000 || (int64_t)mats * rows > 0x7FFFFFFF)
+  if (mats < 0 || rows < 0 || cols < 0 || cols > 0x7F000000 || (pair ? 2 : 1) * (int64_t)mats * rows > 0x7FFFFFFF)
     return fail(-1, "mx dequantise: %d x %d x %d elements", mats, rows, cols);
   if (mats == 0 || rows == 0 || cols == 0) return 0;
   MxDequantParams p;
   p.codes = (const uint8_t*)codes; p.scales = (const uint8_t*)scales; p.mats = mats; p.rows = rows; p.cols = cols;
   p.in_rows = in_rows; p.code_bytes = (cols + MX_BLOCK - 1) / MX_BLOCK * (MX_BLOCK / 2);
   p.k_atoms = mx_atoms(cols); p.row_atoms = mx_atoms(in_rows);
-  p.out = out; p.rows_ptr = rows_ptr; p.interleave = interleave;
-  const dim3 grid = mx_grid((long long)mats * rows, (cols + 256 * MXD_DEPTH - 1) / (256 * MXD_DEPTH));
+  p.out = out; p.rows_ptr = rows_ptr; p.pair = pair;
+  const dim3 grid = mx_grid((pair ? 2ll : 1ll) * mats * rows, (cols + 256 * MXD_DEPTH - 1) / (256 * MXD_DEPTH));
   const bool vec = cols % 8 == 0 && (uintptr_t)out % 16 == 0;
   if (fp32) {
     if (vec) ep_mx_dequant_kernel<float, true><<<grid, MXQ_WARPS * 32, 0, stream>>>(p);

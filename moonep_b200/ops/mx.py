@@ -40,15 +40,16 @@ BLOCK = 32
 PHASES = 4
 
 
-# The product's descriptor, as the C side lays it out: four operand pointers; rows, K, groups, weight rows, N, gated; cu_seqlens,
+# The product's descriptor, as the C side lays it out: four operand pointers; rows, K, groups, weight rows, N, gated, zero_tail, unused; cu_seqlens,
 # pads, row_scale, out, gate, up, codes, scales, d_act, d_scale; ldc, status, timeout.  (Packed in one call: filling a ctypes structure
 # field by field took as long as the launch.)
-_DESC = struct.Struct("@4P6i10PqPq")
+_DESC = struct.Struct("@4P8i10PqPq")
 
 
-nat.declare("mep_mx_quantize", I, [P, I, L, L, I, I, I, I, I, I, I, P, P, P, P])
+nat.declare("mep_mx_quantize", I, [P, P, I, L, L, I, I, I, I, I, I, P, P, P, P])
 nat.declare("mep_mx_dequantize", I, [P, P, I, I, I, I, I, P, I, P, P])
 nat.declare("mep_mx_desc_bytes", I, [])
+nat.declare("mep_mx_zero_tail", I, [P, I, L, P, P])
 nat.declare("mep_mx_sum_parts", I, [P, I, I, P, P, P])
 nat.declare("mep_mx_gemm_launch", I, [ctypes.c_char_p, P])
 
@@ -104,12 +105,12 @@ class MxTensor:
         return self
 
     @classmethod
-    def _empty(cls, shape, device, zero: bool = False) -> "MxTensor":
+    def _empty(cls, shape, device) -> "MxTensor":
         """A new one; codes and scales share an allocation, whose two views are made when somebody asks for them."""
         sizes = _sizes(shape)
         n = (math.prod(sizes[0]) + 511) // 512 * 512
         self = cls.__new__(cls)
-        self._data = (torch.zeros if zero else torch.empty)(n + math.prod(sizes[1]), dtype=torch.uint8, device=device)
+        self._data = torch.empty(n + math.prod(sizes[1]), dtype=torch.uint8, device=device)
         self._codes = self._scales = None
         at = self._data.data_ptr()
         return self._set(shape, sizes, (at, at + n))
@@ -148,10 +149,10 @@ class MxTensor:
         pair = len(self.shape) == 4
         assert rows_ptr is None or len(self.shape) == 2, "rows_ptr goes with one matrix"
         out = torch.empty(self.shape, dtype=dtype, device=self._data.device)
-        for i in range(2 if pair else 1):
-            ew._rc(nat.call("mep_mx_dequantize", *self._at, self._mats, self.shape[-2],
-                            self.shape[-1], i + 1 if pair else 0, self._rows, _rows_ptr(rows_ptr, self._index),
-                            int(dtype == torch.float32), (out[i] if pair else out).data_ptr(), nat.stream()), "mx dequantise")
+        rc = nat.call("mep_mx_dequantize", *self._at, self._mats, self.shape[-2], self.shape[-1], int(pair), self._rows,
+                      _rows_ptr(rows_ptr, self._index), int(dtype == torch.float32), out.data_ptr(), nat.stream())
+        if rc != 0:
+            ew._rc(rc, "mx dequantise")
         return out
 
 
@@ -168,11 +169,11 @@ def _sizes(shape):
     return (G, rows, code_bytes), (G, atoms, k_atoms, 512)
 
 
-def _quantize_into(q: MxTensor, x: torch.Tensor, axis: int, interleave: int, rows_ptr) -> None:
+def _quantize_into(q: MxTensor, x: torch.Tensor, axis: int, rows_ptr=None, up: int = 0) -> None:
     size, stride = x.shape, x.stride()
     three = len(size) == 3
-    rc = nat.call("mep_mx_quantize", x.data_ptr(), _TYPES[x.dtype], stride[0] if three else 0, stride[-2], size[0] if three else 1,
-                  size[-2], size[-1], int(axis == -2), interleave, q._rows, 1 if len(q.shape) > 2 else PHASES,
+    rc = nat.call("mep_mx_quantize", x.data_ptr(), up, _TYPES[x.dtype], stride[0] if three else 0, stride[-2], size[0] if three else 1,
+                  size[-2], size[-1], int(axis == -2), q._rows, 1 if len(q.shape) > 2 else PHASES,
                   _rows_ptr(rows_ptr, q._index), *q._at, nat.stream())
     if rc != 0:
         ew._rc(rc, "mx quantise")
@@ -200,7 +201,7 @@ def quantize(x: torch.Tensor, axis: int = -1, *, rows_ptr: Optional[torch.Tensor
     shape = tuple(x.shape) if axis == -1 else (*x.shape[:-2], x.shape[-1], x.shape[-2])
     assert shape[-1] >= 1, "the reduction is empty"
     q = MxTensor._empty(shape, x.device)
-    _quantize_into(q, x, axis, 0, rows_ptr)
+    _quantize_into(q, x, axis, rows_ptr)
     return q
 
 
@@ -210,16 +211,18 @@ def pack_gate_up(wg: torch.Tensor, wu: torch.Tensor) -> MxTensor:
     _operand(wg, "wg"), _operand(wu, "wu")
     assert wg.shape == wu.shape and wg.dtype == wu.dtype and wg.device == wu.device, "wg and wu must be alike"
     assert wg.shape[-2] >= 1, "the reduction is empty"
-    wg, wu = (w.detach() if w.dim() == 3 else w.detach()[None] for w in (wg, wu))
+    if wg.dim() == 2:
+        wg, wu = wg[None], wu[None]
+    if wg.stride() != wu.stride():
+        wg, wu = wg.contiguous(), wu.contiguous()
     G, H, Hp = wg.shape
-    q = MxTensor._empty((2, G, Hp, H), wg.device, zero=Hp % 16 != 0)      # (the last turn of 16 is not full: zeros)
-    _quantize_into(q, wg, -2, 1, None)
-    _quantize_into(q, wu, -2, 2, None)
+    q = MxTensor._empty((2, G, Hp, H), wg.device)
+    _quantize_into(q, wg, -2, up=wu.data_ptr())
     return q
 
 
 def _launch(a: MxTensor, w: MxTensor, N: int, gated: int, cu_seqlens, pads, row_scale, out: int, gate: int, up: int, codes: int,
-            scales: int, ldc: int, d_act: int = 0, d_scale: int = 0) -> None:
+            scales: int, ldc: int, d_act: int = 0, d_scale: int = 0, zero_tail: int = 0) -> None:
     global _checked_layout
     index, groups, (rows, K) = a._index, w._mats, a.shape
     assert index == _device(), "the operands are not on the current device"
@@ -246,7 +249,7 @@ def _launch(a: MxTensor, w: MxTensor, N: int, gated: int, cu_seqlens, pads, row_
         assert nat.call("mep_mx_desc_bytes") == _DESC.size, "MxDesc layout mismatch"
         _checked_layout = True
     rc = nat.call("mep_mx_gemm_launch",
-                  _DESC.pack(*a._at, *w._at, rows, K, groups, w._rows, N, gated, cu, pad, scale, out, gate, up, codes, scales,
+                  _DESC.pack(*a._at, *w._at, rows, K, groups, w._rows, N, gated, zero_tail, 0, cu, pad, scale, out, gate, up, codes, scales,
                              d_act, d_scale, ldc, status.data_ptr(), 0),
                   nat.stream())
     if rc != 0:
@@ -254,12 +257,12 @@ def _launch(a: MxTensor, w: MxTensor, N: int, gated: int, cu_seqlens, pads, row_
 
 
 def matmul(a: MxTensor, w: MxTensor, cu_seqlens: Optional[torch.Tensor] = None, *, out: Optional[torch.Tensor] = None,
-           pads: Optional[torch.Tensor] = None) -> torch.Tensor:
+           pads: Optional[torch.Tensor] = None, zero_tail: bool = False) -> torch.Tensor:
     """``y[rows of g] = a w[g]^T`` in bf16, summed in fp32: ``a`` ``[rows, K]``, ``w`` ``[G, N, K]`` with ``cu_seqlens``
     ``[G]``, or ``[N, K]`` for all rows.
 
     ``out`` ``[rows or more, N]`` (bf16, dense rows) takes the result; rows that belong to no group are left as they
-    are.  ``pads`` (a plan's ``zero_fill_ranges``): which rows of the groups are padding; they become zeros without
+    are, or with ``zero_tail`` become zeros where they are behind the last group.  ``pads`` (a plan's ``zero_fill_ranges``): which rows of the groups are padding; they become zeros without
     being computed."""
     assert isinstance(a, MxTensor) and isinstance(w, MxTensor) and len(w.shape) < 4, "operands must be quantised"
     assert len(a.shape) == 2, "the rows' operand is one matrix"
@@ -273,7 +276,7 @@ def matmul(a: MxTensor, w: MxTensor, cu_seqlens: Optional[torch.Tensor] = None, 
         ld = out.stride(0)
         assert out.shape[0] < 2 or ld >= N, "rows of out overlap"
     if N > 0:
-        _launch(a, w, N, 0, cu_seqlens, pads, None, out.data_ptr(), 0, 0, 0, 0, ld)
+        _launch(a, w, N, 0, cu_seqlens, pads, None, out.data_ptr(), 0, 0, 0, 0, ld, zero_tail=int(zero_tail))
     return out
 
 
@@ -342,9 +345,7 @@ class _ExpertFFN(torch.autograd.Function):
         keep = any(ctx.needs_input_grad)
         xq = quantize(x, rows_ptr=None if cu_seqlens is None else cu_seqlens[-1:])
         act, _, _ = gateup_swiglu(xq, wgu, cu_seqlens, row_scale=row_scale, quantize=True, pads=pads)
-        # (a pass over all rows leaves none; rows that belong to no group are zeros)
-        new = torch.empty if cu_seqlens is None else torch.zeros
-        y = matmul(act, wdq, cu_seqlens, pads=pads, out=new(x.shape, dtype=torch.bfloat16, device=x.device))
+        y = matmul(act, wdq, cu_seqlens, pads=pads, zero_tail=True)
         if keep:
             ctx.packed, ctx.shapes = (xq, act, wgu, wdq), None if isinstance(wg, MxTensor) else (wg.shape, wd.shape)
             ctx.save_for_backward(row_scale, cu_seqlens, pads)
@@ -369,10 +370,11 @@ class _ExpertFFN(torch.autograd.Function):
             d_act = gemm.down_dgrad(dy, wdq.dequantize().view(G, H, Hp), cu, pads=pads, fp32=True)
             d_gate, d_up, d_scale = gateup_swiglu_bwd(d_act, xq, wgu, cu, row_scale=row_scale, want_dscale=need_s, pads=pads)
             if need_x:
-                new = torch.empty if cu is None else torch.zeros
-                dx = new(dy.shape, **bf16)
                 w = wgu.dequantize()
-                gemm.gateup_dgrad(d_gate, d_up, w[0], w[1], cu, out=dx, pads=pads, transposed=True)
+                dx = gemm.gateup_dgrad(d_gate, d_up, w[0], w[1], cu, pads=pads, transposed=True)
+                if cu is not None:
+                    ew._rc(nat.call("mep_mx_zero_tail", dx.data_ptr(), dx.shape[0], 2 * H, rows_ptr.data_ptr(), nat.stream()),
+                           "mx rows behind the last group")
             if need_g or need_u:
                 out = torch.empty(2, G, H, Hp, **bf16)
                 gemm.wgrad2(xq.dequantize(rows_ptr=rows_ptr), (d_gate, d_up), cu, (out[0], out[1]), pads=pads)

@@ -125,6 +125,17 @@ def test_pack_gate_up(shape):
 
 
 @gpu
+def test_pack_gate_up_strides():
+    from moonep_b200.ops import mx
+    gen = _gen(20)
+    both = torch.randn(3, 96, 2 * 50, generator=gen).bfloat16().cuda()
+    wg, wu = both[:, :, :50], both[:, :, 50:]
+    want = mx.pack_gate_up(wg.contiguous(), wu.contiguous()).dequantize()
+    assert torch.equal(mx.pack_gate_up(wg, wu).dequantize(), want)
+    assert torch.equal(mx.pack_gate_up(wg, wu.contiguous()).dequantize(), want)
+
+
+@gpu
 def test_empty_operands():
     from moonep_b200.ops import mx
     q = mx.quantize(torch.empty(0, 64, device="cuda", dtype=torch.bfloat16))
@@ -202,6 +213,10 @@ def test_product_leaves_other_rows():
     assert (got[20:37, 8:8 + N] == 0).all() and (got[200:255, 8:8 + N] == 0).all()
     got[:255, 8:8 + N] = 7.0
     assert (got == 7.0).all()
+    mx.matmul(mx.quantize(more), mx.quantize(w.cuda()), ends.cuda(), out=out[:-20, 8:8 + N], zero_tail=True)
+    assert (out[255:-20, 8:8 + N] == 0).all() and (out[-20:] == 7).all() and (out[:, :8] == 7).all() and (out[:, 8 + N:] == 7).all()
+    mx.matmul(mx.quantize(more), mx.quantize(w.cuda()), torch.zeros_like(ends).cuda(), out=out[:-20, 8:8 + N], zero_tail=True)
+    assert (out[:-20, 8:8 + N] == 0).all() and (out[-20:] == 7).all()
 
 
 @gpu
