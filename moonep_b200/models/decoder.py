@@ -232,3 +232,5 @@ class MoEDecoder(nn.Module):
         for i, m in enumerate(self.moe_layers()):
             for k, v in (("router", m.w_router), ("gate", m.w_gate), ("up", m.w_up), ("down", m.w_down)):
                 v.copy_(sd[f"moe.{i}.{k}"].to(v.device))
+            if getattr(m, "expert_format", None) == "mxfp4" and not m.training:
+                m.pack_experts()

@@ -30,7 +30,7 @@ import torch.distributed as dist
 from .. import buffer as symm
 from ..api import Buffer
 from ..ops import elementwise as ew
-from ..ops import gemm
+from ..ops import gemm, mx
 from ..utils.trace import NULL_TRACER
 
 
@@ -115,6 +115,8 @@ class _MoEFn(torch.autograd.Function):
                                                    wu_slot=slots["u"], split=epn, row_scale=w_nvs,
                                                    save_gate_up=layer.training and keep, out=outs, g_begin=epn,
                                                    dispatch=wait_only, pads=plan.zero_fill_ranges)
+        elif layer.expert_format == "mxfp4":
+            return _MoEFn._forward_mx(ctx, layer, x, hidden, w_nvs, cu[:epn], plan, topk, w, keep)
         else:
             slots = dict(g=None, u=None, d=None)
             split, cu_use = None, cu[:epn]
@@ -145,11 +147,39 @@ class _MoEFn(torch.autograd.Function):
         return y
 
     @staticmethod
+    def _forward_mx(ctx, layer, x, hidden, w_nvs, cu, plan, topk, w, keep):
+        """The experts over microscaled 4-bit operands.  Of the rows only the quantised ones are kept for backward,
+        which computes gate and up again."""
+        buf, tr = layer.buf, layer.tracer
+        with tr.span("f.pack"):
+            wgu, wd = layer.packed_experts()
+        with tr.span("f.quantize"):
+            xq = mx.quantize(hidden, rows_ptr=cu[-1:])
+        with tr.span("f.gateup"):
+            act, _, _ = mx.gateup_swiglu(xq, wgu, cu, row_scale=w_nvs, quantize=True, pads=plan.zero_fill_ranges)
+        shard = buf.hidden_nvsh_buffer_view
+        with tr.span("f.down"):
+            mx.matmul(act, wd, cu, out=shard, pads=plan.zero_fill_ranges)
+        y, _, _ = buf.combine(plan, shard, None, zero_copy=True)
+        ctx.layer, ctx.plan, ctx.split = layer, plan, None
+        if keep:
+            ctx.packed = xq, act, wgu, wd
+        ctx.save_for_backward(x, None, w_nvs, cu, None, None, None, topk, w)
+        layer.last_plan = plan
+        return y
+
+    @staticmethod
     def backward(ctx, dy):
         layer, plan, split = ctx.layer, ctx.plan, ctx.split
         buf: Buffer = layer.buf
         pools = layer.pools
         x, hidden, w_nvs, cu, act, gate, up, topk, w = ctx.saved_tensors
+        w_gate, w_up, w_down = layer.w_gate, layer.w_up, layer.w_down
+        packed = getattr(ctx, "packed", None)
+        if packed is not None:      # straight through the quantisation: the products' own operands, in bf16
+            xq, act, wgu, wd = packed
+            hidden, act = xq.dequantize(rows_ptr=cu[-1:]), act.dequantize(rows_ptr=cu[-1:])
+            w_down = wd.dequantize()
         have_slots = split is not None
         slot = (lambda n: pools.slot(n)) if have_slots else (lambda n: None)
         gslot = (lambda n: pools.grad_slot(n)) if have_slots else (lambda n: None)
@@ -176,8 +206,8 @@ class _MoEFn(torch.autograd.Function):
                 ev_p = layer.prefetch(plan)
         with tr.span("b.down_dgrad"):
             if ev_p is None:
-                d_act = gemm.down_dgrad(d_out, layer.w_down, cu, wd_slot=slot("down"), split=split, dispatch=disp,
-                                        pads=pads)
+                d_act = gemm.down_dgrad(d_out, w_down, cu, wd_slot=slot("down"), split=split, dispatch=disp,
+                                        pads=pads, fp32=packed is not None)
             else:      # local experts first, next to the copy kernel; the slot groups once it is done
                 d_act = gemm.down_dgrad(d_out, layer.w_down, cu[:buf.epn], grid=layer.overlap_grid(),
                                         dispatch=disp, pads=pads)
@@ -209,7 +239,11 @@ class _MoEFn(torch.autograd.Function):
             gemm.wgrad(d_out, act, cu, layer.g_down, grad_slot=gslot("down"), split=split, accumulate=acc,
                        sgd=sgd(layer.w_down), pads=pads, rows=buf.N)
         with tr.span("b.swiglu_bwd"):
-            d_gate, d_up, d_scale = ew.swiglu_bwd(d_act, gate, up, w_nvs, rows_ptr=cu[-1:])
+            if packed is not None:
+                d_gate, d_up, d_scale = mx.gateup_swiglu_bwd(d_act, xq, wgu, cu, row_scale=w_nvs, want_dscale=True, pads=pads)
+                w_gate, w_up = wgu.dequantize()
+            else:
+                d_gate, d_up, d_scale = ew.swiglu_bwd(d_act, gate, up, w_nvs, rows_ptr=cu[-1:])
         ev_r = None
         zc = layer.accumulate_grads            # the slots are overwritten next step otherwise
         if fused_lr is None:
@@ -234,16 +268,17 @@ class _MoEFn(torch.autograd.Function):
         # dispatch backward = combine; the scalar path returns d(route weights) as [S, K]
         if layer.fused_combine:
             with tr.span("b.gateup_dgrad_push"):
-                gemm.gateup_dgrad(d_gate, d_up, layer.w_gate, layer.w_up, cu, wg_slot=slot("gate"),
+                gemm.gateup_dgrad(d_gate, d_up, w_gate, w_up, cu, wg_slot=slot("gate"),
                                   wu_slot=slot("up"), split=split, push=buf.push_target(plan), grid=grid,
-                                  pads=pads)
+                                  pads=pads, transposed=packed is not None)
             ev_r = _MoEFn._late_wgrads(layer, plan, hidden, d_gate, d_up, cu, gslot, split, ev_r, do_reduce, sgd)
             with tr.span("b.combine_pushed"):
                 dx, dw_sk = buf.combine_pushed(plan, d_scale)
         else:
             shard = buf.hidden_nvsh_buffer_view
-            gemm.gateup_dgrad(d_gate, d_up, layer.w_gate, layer.w_up, cu, wg_slot=slot("gate"),
-                              wu_slot=slot("up"), split=split, out=shard, grid=grid, pads=pads)
+            gemm.gateup_dgrad(d_gate, d_up, w_gate, w_up, cu, wg_slot=slot("gate"),
+                              wu_slot=slot("up"), split=split, out=shard, grid=grid, pads=pads,
+                              transposed=packed is not None)
             ev_r = _MoEFn._late_wgrads(layer, plan, hidden, d_gate, d_up, cu, gslot, split, ev_r, do_reduce, sgd)
             dx, dw_sk, _ = buf.combine(plan, shard, d_scale, zero_copy=True)
         # router backward
@@ -296,15 +331,27 @@ class _MoEFn(torch.autograd.Function):
 
 
 class MoELayer:
-    """One MoE layer of ``E`` SwiGLU experts sharded over the ``R`` ranks of ``buf``."""
+    """One MoE layer of ``E`` SwiGLU experts sharded over the ``R`` ranks of ``buf``.
+
+    ``expert_format="mxfp4"``: the experts' products run over microscaled 4-bit operands (:mod:`..ops.mx`): rows and
+    activations are quantised on the way, weights before.  A layer built with ``train=False`` quantises its weights once
+    (:meth:`pack_experts`, again after they were changed in place) and streams 17/64 of their bytes; one that trains does
+    it in every forward pass, and its gradients are those of the quantised operands, passed straight through to the bf16
+    weights and rows.  For a group of one rank, whose experts are all local; router and combine are as ever."""
 
     def __init__(self, buf: Buffer, Hp: int, pools: Optional[ExpertPools] = None, *, seed: int = 0,
                  router_bias: Optional[torch.Tensor] = None, init_std: float = 0.02,
                  train: bool = True, fused_combine: bool = True, hidden_in_place: bool = False,
-                 fused_dispatch: Optional[bool] = None):
+                 fused_dispatch: Optional[bool] = None, expert_format: str = "bf16"):
         assert not buf.virtual, "MoELayer runs one rank per process"
         assert buf.token_padding % 64 == 0, "the grouped GEMM needs token_padding % 64 == 0"
         assert buf.H % 128 == 0 and Hp % 64 == 0
+        assert expert_format in ("bf16", "mxfp4"), "expert_format is bf16 or mxfp4"
+        if expert_format == "mxfp4":
+            assert buf.R == 1, "4-bit experts need a group of one rank: prefetched weights are bf16"
+            assert not hidden_in_place, "4-bit experts keep quantised rows: there are none to keep in place"
+            assert not fused_dispatch, "a lone rank's rows are quantised between dispatch and product"
+        self.expert_format, self._packed = expert_format, None
         self.buf, self.pools, self.Hp = buf, pools, Hp
         self.training, self.accumulate_grads = train, False
         self.fused_combine = fused_combine
@@ -356,6 +403,21 @@ class MoELayer:
             self.g_router = z(1, H, E)
             self.g_gate, self.g_up, self.g_down = z(epn, H, Hp), z(epn, H, Hp), z(epn, H, Hp)
         self.last_plan = None
+        if expert_format == "mxfp4" and not train:
+            self.pack_experts()
+
+    def pack_experts(self) -> None:
+        """4-bit experts of a layer that does not train: quantise the weights as they are now.  Done when the layer is
+        built and by ``load_state_dict``; call it after changing them in place."""
+        assert self.expert_format == "mxfp4"
+        self._packed = mx.pack_gate_up(self.w_gate, self.w_up), mx.quantize(self.w_down)
+
+    def packed_experts(self):
+        """Gate and up projections, and the down projection, quantised: those kept by :meth:`pack_experts`, or while
+        training the present weights'."""
+        if self.training:
+            return mx.pack_gate_up(self.w_gate, self.w_up), mx.quantize(self.w_down)
+        return self._packed
 
     def prefetch(self, plan):
         """``prefetch_weight`` of this layer's experts for ``plan`` on the comm stream; returns the
@@ -416,3 +478,5 @@ class MoELayer:
     def load_state_dict(self, sd):
         for k, v in self.parameters().items():
             v.copy_(sd[k].to(v.device))
+        if self._packed is not None:
+            self.pack_experts()

@@ -10,7 +10,7 @@ def quantise(x):
     K = x.shape[-1]
     full = torch.zeros(*x.shape[:-1], (K + 31) // 32 * 32, dtype=torch.float64)
     full[..., :K] = x.double()
-    b = full.view(*x.shape[:-1], -1, 32)
+    b = full.view(*x.shape[:-1], full.shape[-1] // 32, 32)
     a = b.abs().amax(-1, keepdim=True)                     # (NaN if there is one)
     m, e = torch.frexp(torch.where(a.isfinite(), a, 1.0))  # a = m 2^e, m in [0.5, 1)
     e = torch.where(a > 0, e - 3, -127).clamp(-127, 127)
