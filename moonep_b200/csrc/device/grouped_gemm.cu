@@ -282,7 +282,7 @@ struct PairLaunch {
 };
 template <class Params>
 static int launch_pair(const void* kern, PairLaunch& once, const Params& kp, int grid, int threads, int smem, bool coop,
-                       cudaStream_t stream) {
+                       cudaStream_t stream, bool pdl = false) {
   MEP_CUDA_OK(raise_smem_limit(kern, once.raised));
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
@@ -290,7 +290,7 @@ static int launch_pair(const void* kern, PairLaunch& once, const Params& kp, int
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
+  cudaLaunchAttribute attr[3];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeCooperative;
@@ -319,6 +319,12 @@ static int launch_pair(const void* kern, PairLaunch& once, const Params& kp, int
     if (use < 1) use = 1;
   }
   if ((int)cfg.gridDim.x / 2 > use) cfg.gridDim = dim3((unsigned)(2 * use));
+  // a kernel that calls pdl_wait() may be put in place while its predecessor runs (not in a capture)
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  if (pdl && cudaStreamIsCapturing(stream, &cap) == cudaSuccess && cap == cudaStreamCaptureStatusNone) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
   void* args[] = {(void*)&kp};
   MEP_CUDA_OK(cudaLaunchKernelExC(&cfg, kern, args));
   return 0;
@@ -398,7 +404,7 @@ template <int EPI, int MAX_N>
 static int launch_mx(const MxParams& p, int grid, cudaStream_t stream) {
   static PairLaunch once;
   return launch_pair((const void*)ep_mx_gemm_kernel<EPI, MAX_N>, once, p, grid, mxg_threads<EPI>(),
-                     mxg_stages<EPI, MAX_N>() * mxg_stage(MAX_N) + 1024, false, stream);
+                     mxg_stages<EPI, MAX_N>() * mxg_stage(MAX_N) + 1024, false, stream, true);
 }
 template <int EPI>
 static int launch_mx(const MxParams& p, bool few, int grid, cudaStream_t stream) {

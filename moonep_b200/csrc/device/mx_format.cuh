@@ -54,10 +54,20 @@ __device__ __forceinline__ uint32_t mx_codes(const float* x) {
       : "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]));
   return r;
 }
-// The value of a code times 1: sign, then 0 0.5 1 1.5 2 3 4 6.  As an fp32 number the code's exponent and mantissa are
-// put where fp32 has its own and rescaled by 2^126; 0.5, subnormal in either format, comes out right.
+// The value of a code (its low four bits): sign, then 0 0.5 1 1.5 2 3 4 6.  As an fp32 number the code's exponent and
+// mantissa are put where fp32 has its own and rescaled by 2^126; 0.5, subnormal in either format, comes out right.
 __device__ __forceinline__ float mx_element(uint32_t code) {
   return __uint_as_float(((code & 8u) << 28) | ((code & 7u) << 22)) * 0x1p126f;
+}
+// Four codes (the low 16 bits) as bf16, two a word: the magnitudes' bytes are looked up by byte permutations, then the
+// signs set.
+__device__ __forceinline__ uint2 mx_bf16x4(uint32_t codes) {
+  const uint32_t sel = codes & 0x7777u;
+  const uint32_t high = __byte_perm(0x3F3F3F00u, 0x40404040u, sel), low = __byte_perm(0xC0800000u, 0xC0804000u, sel);
+  uint2 r;
+  r.x = __byte_perm(low, high, 0x5140) | (codes << 12 & 0x8000u) | (codes << 24 & 0x80000000u);
+  r.y = __byte_perm(low, high, 0x7362) | (codes << 4 & 0x8000u) | (codes << 16 & 0x80000000u);
+  return r;
 }
 
 }  // namespace mep

@@ -165,6 +165,8 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
     if (lane == 1) { tma_prefetch_desc(&p.w); tma_prefetch_desc(&p.ws); }
     if (lane == 2) { tma_prefetch_desc(&p.ts); tma_prefetch_desc(&p.tok[0]); }
   }
+  if (warp == 1) { tmem_alloc2(&s_tmem, 512); tmem_relinquish2(); }
+  pdl_wait();               // nothing of this is read from memory; what follows is
   // Group tables: ends, and rows with tokens counted from the multiple of 32 at or before the first.  (One round of loads
   // for all groups, 1 us; the padding ranges looked up in the scan below and again for every tile cost 2 - 4 us a launch.)
   for (int g = tid; g < p.ngroups; g += mxg_threads<EPI>()) {
@@ -192,7 +194,6 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
     }
     if (lane == 0) s_prefix[p.ngroups] = run;
   }
-  if (warp == 1) { tmem_alloc2(&s_tmem, 512); tmem_relinquish2(); }
   tc_fence_before();
   cluster_sync_all();
   tc_fence_after();
@@ -550,6 +551,7 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
         for (int c = lane * 8; c < p.N; c += 256) store8(p.out + (long long)row * p.ldc + c, make_uint4(0, 0, 0, 0), p.N - c, p.vec_out != 0);
     }
   }
+  pdl_launch_dependents();   // (a kernel that waits for this one may take what room there is beside the last tiles)
   // ---- teardown: everything joins, in-flight work is given time to land on an abort ----------
   tc_fence_before();
   __syncthreads();

@@ -1,5 +1,6 @@
 // Quantisation into microscaled 4-bit operands (mx_format.cuh) and back.  Both directions are bandwidth kernels: one
-// pass, every element read and written once.
+// pass, every element read and written once.  They are launched as programmatic dependents, as the product behind them
+// is: a chain's kernels are in place when their predecessor ends (three launches for a token: 6 us of gaps less).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -7,6 +8,7 @@
 #include <cstdint>
 
 #include "device/mx_format.cuh"
+#include "device/sync.cuh"
 #include "host/ctx.h"
 #include "host/errors.h"
 
@@ -93,11 +95,15 @@ __device__ __forceinline__ MxEight<T> mx_load8(const T* row, int c, int cols) {
 }
 
 // Along the rows.  A warp takes MXQ_DEPTH parts of 256 elements of a row, a lane eight of each: four lanes share a
-// block, sixteen the four scales of an atom's row, which leave as one word (a phase).
+// block, sixteen the four scales of an atom's row, which leave as one word (a phase).  Bound by HBM, and next to it by
+// issue: 8192 x 7168 in bf16 30 us, 5.0 TB/s; fp32 42 us, 6.3.  (Sixteen elements a lane are fewer instructions, but two
+// 16-byte accesses of a lane side by side: 14336 x 7168 51.6 us, 53.7; odd rows 48, 72; 32 x 7168 x 2048 215, 201.)
 constexpr int MXQ_WARPS = 8, MXQ_DEPTH = 4;
 
 template <class T, bool VEC>
 __global__ void __launch_bounds__(MXQ_WARPS * 32) ep_mx_quant_rows_kernel(const __grid_constant__ MxQuantParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rows = p.rows_ptr ? max(0, min(*p.rows_ptr, p.rows)) : p.rows;
   const unsigned lines = (unsigned)p.mats * (unsigned)rows;
@@ -146,6 +152,8 @@ template <class T> constexpr int mxt_pairs() { return sizeof(T) == 2 ? 2 : 1; }
 
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256, 2) ep_mx_quant_cols_kernel(const __grid_constant__ MxQuantParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
   constexpr int NP = mxt_pairs<T>(), COLS = 64 * NP;
   struct __align__(8) Piece { MxPair<T> p[NP]; };
   __shared__ __align__(16) uint8_t s_codes[COLS * 128];
@@ -225,12 +233,15 @@ struct MxDequantParams {
   int pair;                     // the values of the gate projections, then of the up projections
 };
 
-// A lane takes eight values of a row, a warp MXD_DEPTH times 256.  (Exact in bf16 but for what a bf16 subnormal rounds,
+// A lane takes eight values of a row, a warp MXD_DEPTH times 256.  Bound by HBM (6.0 TB/s); the values' bytes are looked
+// up, which takes half the instructions of computing them.  (Sixteen values a lane: 4.3 TB/s.)  (Exact in bf16 but for what a bf16 subnormal rounds,
 // fp32 always.)
 constexpr int MXD_DEPTH = 8;
 
 template <class T, bool VEC>
 __global__ void __launch_bounds__(MXQ_WARPS * 32) ep_mx_dequant_kernel(const __grid_constant__ MxDequantParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rows = p.rows_ptr ? max(0, min(*p.rows_ptr, p.rows)) : p.rows;
   const unsigned lines = (unsigned)(p.pair ? 2 * p.mats : p.mats) * (unsigned)rows;
@@ -262,8 +273,7 @@ __global__ void __launch_bounds__(MXQ_WARPS * 32) ep_mx_dequant_kernel(const __g
           }
         }
       }
-      continue;
-    }
+    } else
     for (int c0 = blockIdx.y * 256 * MXD_DEPTH + lane * 8; c0 < p.cols; c0 += gridDim.y * 256 * MXD_DEPTH) {
       uint32_t code[MXD_DEPTH], b[MXD_DEPTH];
 #pragma unroll
@@ -277,15 +287,22 @@ __global__ void __launch_bounds__(MXQ_WARPS * 32) ep_mx_dequant_kernel(const __g
         const int c = c0 + i * 256;
         if (c >= p.cols) break;
         const float s = mx_value(b[i]);
-        __align__(16) T v[8];
+        if constexpr (sizeof(T) == 2) {
+          const __nv_bfloat162 s2 = __float2bfloat162_rn(s);
+          const uint2 lo = mx_bf16x4(code[i]), hi = mx_bf16x4(code[i] >> 16);
+          uint4 q = make_uint4(lo.x, lo.y, hi.x, hi.y);
+          __nv_bfloat162* v = reinterpret_cast<__nv_bfloat162*>(&q);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float f = mx_element(code[i] >> (4 * e)) * s;
-          if constexpr (sizeof(T) == 2) v[e] = __float2bfloat16(f);
-          else v[e] = f;
+          for (int e = 0; e < 4; ++e) v[e] = __hmul2(v[e], s2);
+          __stcs(reinterpret_cast<uint4*>(out + c), q);
+        } else {
+          float4 v[2];
+          float* f = reinterpret_cast<float*>(v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] = mx_element(code[i] >> (4 * e)) * s;
+          __stcs(reinterpret_cast<float4*>(out + c), v[0]);
+          __stcs(reinterpret_cast<float4*>(out + c) + 1, v[1]);
         }
-#pragma unroll
-        for (int q = 0; q < (int)sizeof(T) / 2; ++q) __stcs(reinterpret_cast<uint4*>(out + c) + q, reinterpret_cast<const uint4*>(v)[q]);
       }
     }
   }
@@ -302,7 +319,7 @@ static dim3 mx_grid(long long lines, int parts) {
 }
 
 template <class T>
-static int mx_quant(const MxQuantParams& p, bool along_cols, cudaStream_t stream) {
+static int mx_quant(MxQuantParams& p, bool along_cols, cudaStream_t stream) {
   const bool rows16 = (uintptr_t)p.x % 16 == 0 && (p.stride * sizeof(T)) % 16 == 0 && (p.batch * sizeof(T)) % 16 == 0 && p.cols % 8 == 0;
   constexpr int lane_cols = 2 * mxt_pairs<T>(), block_cols = 32 * lane_cols;
   const bool pieces = ((uintptr_t)p.x | (uintptr_t)p.x2) % 8 == 0 && p.stride % lane_cols == 0 && p.batch % lane_cols == 0 && p.cols % lane_cols == 0;
@@ -310,14 +327,13 @@ static int mx_quant(const MxQuantParams& p, bool along_cols, cudaStream_t stream
     const dim3 grid((unsigned)((p.cols + block_cols - 1) / block_cols), (unsigned)((p.rows + MXT_ROWS - 1) / MXT_ROWS),
                     (unsigned)(p.mats < 32767 ? (p.x2 ? 2 : 1) * p.mats : 65534));
     if (grid.y > 65535) return fail(-5, "mx quantise: %d rows are too many along the last but one axis", p.rows);
-    if (pieces) ep_mx_quant_cols_kernel<T, true><<<grid, 256, 0, stream>>>(p);
-    else ep_mx_quant_cols_kernel<T, false><<<grid, 256, 0, stream>>>(p);
+    MEP_CUDA_OK(launch_chained(pieces ? (const void*)ep_mx_quant_cols_kernel<T, true> : (const void*)ep_mx_quant_cols_kernel<T, false>,
+                               grid, dim3(256), 0, stream, p, 0, 1));
   } else {
     const dim3 grid = mx_grid((long long)p.mats * p.rows, (p.k_atoms * MX_ATOM_K + 256 * MXQ_DEPTH - 1) / (256 * MXQ_DEPTH));
-    if (rows16) ep_mx_quant_rows_kernel<T, true><<<grid, MXQ_WARPS * 32, 0, stream>>>(p);
-    else ep_mx_quant_rows_kernel<T, false><<<grid, MXQ_WARPS * 32, 0, stream>>>(p);
+    MEP_CUDA_OK(launch_chained(rows16 ? (const void*)ep_mx_quant_rows_kernel<T, true> : (const void*)ep_mx_quant_rows_kernel<T, false>,
+                               grid, dim3(MXQ_WARPS * 32), 0, stream, p, 0, 1));
   }
-  MEP_CUDA_OK(cudaGetLastError());
   return 0;
 }
 
@@ -363,14 +379,9 @@ int mep_mx_dequantize(const void* codes, const void* scales, int mats, int rows,
   p.out = out; p.rows_ptr = rows_ptr; p.pair = pair;
   const dim3 grid = mx_grid((pair ? 2ll : 1ll) * mats * rows, (cols + 256 * MXD_DEPTH - 1) / (256 * MXD_DEPTH));
   const bool vec = cols % 8 == 0 && (uintptr_t)out % 16 == 0;
-  if (fp32) {
-    if (vec) ep_mx_dequant_kernel<float, true><<<grid, MXQ_WARPS * 32, 0, stream>>>(p);
-    else ep_mx_dequant_kernel<float, false><<<grid, MXQ_WARPS * 32, 0, stream>>>(p);
-  } else {
-    if (vec) ep_mx_dequant_kernel<__nv_bfloat16, true><<<grid, MXQ_WARPS * 32, 0, stream>>>(p);
-    else ep_mx_dequant_kernel<__nv_bfloat16, false><<<grid, MXQ_WARPS * 32, 0, stream>>>(p);
-  }
-  MEP_CUDA_OK(cudaGetLastError());
+  const void* kern = fp32 ? (vec ? (const void*)ep_mx_dequant_kernel<float, true> : (const void*)ep_mx_dequant_kernel<float, false>)
+                          : (vec ? (const void*)ep_mx_dequant_kernel<__nv_bfloat16, true> : (const void*)ep_mx_dequant_kernel<__nv_bfloat16, false>);
+  MEP_CUDA_OK(launch_chained(kern, grid, dim3(MXQ_WARPS * 32), 0, stream, p, 0, 1));
   return 0;
 }
 
