@@ -204,7 +204,7 @@ struct GemmDesc {
 // Product of microscaled 4-bit operands: tokens [rows][K], weights [ngroups][w_rows][K] (`gated`: gate and up packed).
 struct MxDesc {
   const void *a_codes, *a_scales, *w_codes, *w_scales;
-  int32_t rows, K, ngroups, w_rows, N, gated, zero_tail, unused;
+  int32_t rows, K, ngroups, w_rows, N, gated, zero_tail, check_groups;
   const int32_t* cu_seqlens;
   const int32_t* pads;
   const float* row_scale;
@@ -637,7 +637,9 @@ int mep_mx_sum_parts(const float* parts, int n, int rows, const int32_t* rows_pt
 
 int mep_mx_gemm_launch(const MxDesc* d, cudaStream_t stream) {
   if (d->ngroups < 1 || d->ngroups > MAX_GROUPS) return fail(-1, "mx product: ngroups=%d out of range", d->ngroups);
-  if (d->rows < 0 || d->K < 1 || d->N < 1 || d->w_rows < 1) return fail(-2, "mx product: %d x %d x %d", d->rows, d->K, d->N);
+  if (d->rows < 0 || d->K < 1 || d->N < 1 || d->w_rows < 1 || d->K > 0x7F000000 || d->rows > 0x7F000000 ||
+      (int64_t)d->ngroups * d->w_rows > 0x7F000000)
+    return fail(-2, "mx product: %d x %d x %d with %d groups", d->rows, d->K, d->N, d->ngroups);
   if (d->rows == 0) return 0;
   MxParams p;
   std::memset(&p, 0, sizeof(p));
@@ -662,7 +664,7 @@ int mep_mx_gemm_launch(const MxDesc* d, cudaStream_t stream) {
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  p.zero_tail = d->zero_tail;
+  p.zero_tail = d->zero_tail; p.check_groups = d->check_groups;
   p.d_act = d->d_act; p.d_scale = d->d_scale;
   if (d->d_act != nullptr) {
     if (!d->gated || p.gate == nullptr || p.up == nullptr) return fail(-3, "mx product: the backward pass writes both gradients");

@@ -64,6 +64,7 @@ struct MxParams {
   const float* row_scale;
   const float* d_act;              // backward: gradient of the activation, [total_rows][N]
   int zero_tail;                   // rows behind the last group become zeros
+  int check_groups;                // a group whose rows are no multiple of 64 is recorded in `status`
   float* d_scale;                  // parts of the scales' gradients, [CTA's columns][total_rows], or null
   long long ldc;
   int32_t* status;
@@ -175,6 +176,15 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
     const int start = g == 0 || p.cu_seqlens == nullptr ? 0 : clamped(p.cu_seqlens[g - 1]);
     const int end = clamped(p.cu_seqlens != nullptr ? p.cu_seqlens[g] : p.total_rows);
     s_end[g] = end;
+    if constexpr (EPI == MX_EPI_BF16) {
+      // (one that ends where the tensors do has nothing behind it that the weight grads could read)
+      if (p.check_groups && blockIdx.x == 0 && (end - start) % 64 != 0 && end != p.total_rows && p.status != nullptr &&
+          atomicCAS(p.status, 0, (int)ST_BAD_INDEX) == 0) {
+        p.status[1] = KID_MX_GEMM;
+        p.status[4] = g;
+        p.status[5] = end - start;
+      }
+    }
     s_span[g] = end > start ? (start & 31) + group_valid(p, g, start, end) : 0;
   }
   __syncthreads();

@@ -40,7 +40,7 @@ BLOCK = 32
 PHASES = 4
 
 
-# The product's descriptor, as the C side lays it out: four operand pointers; rows, K, groups, weight rows, N, gated, zero_tail, unused; cu_seqlens,
+# The product's descriptor, as the C side lays it out: four operand pointers; rows, K, groups, weight rows, N, gated, zero_tail, check_groups; cu_seqlens,
 # pads, row_scale, out, gate, up, codes, scales, d_act, d_scale; ldc, status, timeout.  (Packed in one call: filling a ctypes structure
 # field by field took as long as the launch.)
 _DESC = struct.Struct("@4P8i10PqPq")
@@ -222,7 +222,7 @@ def pack_gate_up(wg: torch.Tensor, wu: torch.Tensor) -> MxTensor:
 
 
 def _launch(a: MxTensor, w: MxTensor, N: int, gated: int, cu_seqlens, pads, row_scale, out: int, gate: int, up: int, codes: int,
-            scales: int, ldc: int, d_act: int = 0, d_scale: int = 0, zero_tail: int = 0) -> None:
+            scales: int, ldc: int, d_act: int = 0, d_scale: int = 0, zero_tail: int = 0, check_groups: int = 0) -> None:
     global _checked_layout
     index, groups, (rows, K) = a._index, w._mats, a.shape
     assert index == _device(), "the operands are not on the current device"
@@ -249,7 +249,7 @@ def _launch(a: MxTensor, w: MxTensor, N: int, gated: int, cu_seqlens, pads, row_
         assert nat.call("mep_mx_desc_bytes") == _DESC.size, "MxDesc layout mismatch"
         _checked_layout = True
     rc = nat.call("mep_mx_gemm_launch",
-                  _DESC.pack(*a._at, *w._at, rows, K, groups, w._rows, N, gated, zero_tail, 0, cu, pad, scale, out, gate, up, codes, scales,
+                  _DESC.pack(*a._at, *w._at, rows, K, groups, w._rows, N, gated, zero_tail, check_groups, cu, pad, scale, out, gate, up, codes, scales,
                              d_act, d_scale, ldc, status.data_ptr(), 0),
                   nat.stream())
     if rc != 0:
@@ -345,7 +345,10 @@ class _ExpertFFN(torch.autograd.Function):
         keep = any(ctx.needs_input_grad)
         xq = quantize(x, rows_ptr=None if cu_seqlens is None else cu_seqlens[-1:])
         act, _, _ = gateup_swiglu(xq, wgu, cu_seqlens, row_scale=row_scale, quantize=True, pads=pads)
-        y = matmul(act, wdq, cu_seqlens, pads=pads, zero_tail=True)
+        y = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
+        H = x.shape[1]
+        _launch(act, wdq, H, 0, cu_seqlens, pads, None, y.data_ptr(), 0, 0, 0, 0, H, zero_tail=1,
+                check_groups=int(any(ctx.needs_input_grad[1:4])))
         if keep:
             ctx.packed, ctx.shapes = (xq, act, wgu, wdq), None if isinstance(wg, MxTensor) else (wg.shape, wd.shape)
             ctx.save_for_backward(row_scale, cu_seqlens, pads)
@@ -358,6 +361,8 @@ class _ExpertFFN(torch.autograd.Function):
         row_scale, cu, pads = ctx.saved_tensors
         need_x, need_g, need_u, need_d, need_s = ctx.needs_input_grad[:5]
         dy = dy.contiguous()
+        if dy.data_ptr() % 16 != 0:
+            dy = dy.clone()
         (G, Hp, H), rows_ptr = wgu.shape[1:], None if cu is None else cu[-1:]
         bf16 = dict(dtype=torch.bfloat16, device=dy.device)
         grads = [None] * 3
@@ -395,9 +400,9 @@ def expert_ffn(x: torch.Tensor, wg, wu, wd, cu_seqlens: Optional[torch.Tensor] =
     are the operands in 4 bits; backward computes gate and up again.  Sums run in fp32; ``d gate`` and ``d up`` are
     rounded to bf16, as operands of the bf16 products of :mod:`.gemm`, and the results once more.
 
-    Rows that belong to no group get zeros, in ``y`` and in ``x``'s gradient.  For gradients H must be a multiple of 128
-    and H' of 8, and with ``cu_seqlens`` every group's rows a multiple of 64, of which padding rows of ``x`` are zero
-    (what ``Buffer.dispatch`` gives)."""
+    Rows behind the last group get zeros, in ``y`` and in ``x``'s gradient.  For gradients H must be a multiple of 128
+    and H' of 8, and for the weights' every group's rows a multiple of 64, padding rows of ``x`` being zero (what
+    ``Buffer.dispatch`` gives), but for a group that ends with ``x`` itself; ``gemm.check_status`` reports others."""
     assert isinstance(x, torch.Tensor) and x.dim() == 2 and x.dtype == torch.bfloat16, "x must be bf16 [rows, H]"
     _operand(x, "x")
     H = x.shape[1]
@@ -415,7 +420,9 @@ def expert_ffn(x: torch.Tensor, wg, wu, wd, cu_seqlens: Optional[torch.Tensor] =
         assert wg.shape == wu.shape == wd.shape and wg.shape[-2] == H, "weights must be [G, H, H'] alike"
         Hp = wg.shape[-1]
     if row_scale is not None:
-        assert row_scale.dim() == 1 and row_scale.shape[0] == x.shape[0], "one scale a row"
+        assert row_scale.dtype == torch.float32 and row_scale.dim() == 1 and row_scale.shape[0] == x.shape[0], "one fp32 scale a row"
+        row_scale = row_scale.contiguous()
+    assert pads is None or cu_seqlens is not None, "padding ranges go with cu_seqlens"
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, *trained) + (() if row_scale is None else (row_scale,))):
         assert H % 128 == 0 and Hp % 8 == 0, "gradients need H % 128 == 0 and H' % 8 == 0"
     return _ExpertFFN.apply(x, wg, wu, wd, row_scale, cu_seqlens, pads)

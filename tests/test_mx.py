@@ -98,6 +98,21 @@ def test_quantise_extremes():
 
 
 @gpu
+@pytest.mark.parametrize("dtype,exp", [(torch.bfloat16, -126), (torch.float16, -14)])
+def test_quantise_subnormals(dtype, exp):
+    """Blocks of numbers below their type's smallest normal one, which is 2^exp."""
+    from moonep_b200.ops import mx
+    x = (torch.randn(4, 96, generator=_gen(22)) * 2.0 ** (exp + 2)).to(dtype)
+    x[1] *= 0.125
+    x[2] *= 2.0 ** -4
+    want = ox.quantise(x)
+    assert float(want[2].abs().max()) > 0
+    for q in (mx.quantize(x.cuda()), mx.quantize(x.t().contiguous().cuda(), axis=-2)):
+        _equal(q.dequantize(torch.float32), want)
+        _equal(q.dequantize(), want.float().bfloat16().double())
+
+
+@gpu
 def test_quantise_row_count_on_the_device():
     from moonep_b200.ops import mx
     x = torch.randn(300, 96, generator=_gen(5)).bfloat16()
@@ -487,6 +502,51 @@ def test_expert_ffn_packed_weights():
     assert torch.equal(ys[0], ys[1]) and torch.equal(gs[0], gs[1])
     assert (ys[0][192:] == 0).all() and (gs[0][192:] == 0).all()      # rows of no group
     assert float(gs[0][:192].float().abs().sum()) > 0
+
+
+@gpu
+def test_expert_ffn_group_that_weight_grads_cannot_take():
+    from moonep_b200.ops import gemm, mx
+    bf = dict(device="cuda", dtype=torch.bfloat16)
+    x, w = torch.randn(256, 128, **bf), [torch.randn(2, 128, 64, **bf).requires_grad_(True) for _ in range(3)]
+    ends = lambda *e: torch.tensor(e, dtype=torch.int32, device="cuda")
+    mx.expert_ffn(x, *w, ends(64, 256))
+    mx.expert_ffn(x, *w, ends(128, 256))
+    gemm.check_status()
+    mx.expert_ffn(x, *(t.detach() for t in w), ends(100, 200))      # no weight grads: rows may end anywhere
+    gemm.check_status()
+    for bad, rows in ((ends(100, 256), 100), (ends(64, 200), 136)):
+        mx.expert_ffn(x, *w, bad)
+        with pytest.raises(RuntimeError, match=f"{rows} rows"):
+            gemm.check_status()
+        gemm.reset_status()
+
+
+@gpu
+def test_expert_ffn_some_gradients_only():
+    """Each gradient alone is the one of them all; a leaf used twice gets both; rows broadcast from one."""
+    from moonep_b200.ops import mx
+    gen = _gen(21)
+    H, Hp, rows = 128, 64, 96
+    x = torch.randn(rows, H, generator=gen).bfloat16().cuda()
+    ws = [(torch.randn(H, Hp, generator=gen) * 0.2).bfloat16().cuda() for _ in range(3)]
+    scale, dy = torch.rand(rows, generator=gen).cuda() + 0.5, torch.randn(rows, H, generator=gen).bfloat16().cuda()
+    leaves = [t.clone().requires_grad_(True) for t in (x, *ws, scale)]
+    every = torch.autograd.grad(mx.expert_ffn(*leaves[:4], row_scale=leaves[4]), leaves, dy)
+    for i in range(5):
+        some = [t.clone().requires_grad_(i == j) for j, t in enumerate((x, *ws, scale))]
+        one, = torch.autograd.grad(mx.expert_ffn(*some[:4], row_scale=some[4]), some[i], dy)
+        assert torch.equal(one, every[i])
+    tied = ws[0].clone().requires_grad_(True)
+    g, = torch.autograd.grad(mx.expert_ffn(x, tied, tied, ws[2]), tied, dy)
+    a, b = ws[0].clone().requires_grad_(True), ws[0].clone().requires_grad_(True)
+    ga, gb = torch.autograd.grad(mx.expert_ffn(x, a, b, ws[2]), (a, b), dy)
+    assert torch.equal(g, ga + gb)
+    one = x[:1].clone().requires_grad_(True)
+    g, = torch.autograd.grad(mx.expert_ffn(one.expand(rows, H), *ws).sum(), one)
+    full = x[:1].repeat(rows, 1).requires_grad_(True)
+    gf, = torch.autograd.grad(mx.expert_ffn(full, *ws), full, torch.ones(rows, H, device="cuda", dtype=torch.bfloat16))
+    _near(g, gf.double().cpu().sum(0, keepdim=True), 2 * HALF)
 
 
 @gpu
