@@ -14,6 +14,11 @@
 // Token tiles start at multiples of 32 rows of the whole tensor, whatever row a group starts at: then a tile's scales
 // are whole atoms of one of their four phases.  Rows of a neighbouring group in a tile are computed and not stored.
 //
+// What bounds it: short groups the stream of the weights (16 tokens, 32 experts, 7168 -> 2 x 2048: 83 us, 6.0 TB/s; a launch has
+// 5 us before its first bytes and after its last), long ones the operand bytes that L2 and the SMs exchange, 11 - 13
+// TB/s, and in a long run the power cap (8192 x 7168 x 4096 82 us, 5.9 PFLOP/s; 91 at 1.3 - 1.6 GHz).  Measured and worse: two
+// token tiles that share staged weights, three quarters of the bytes, but weights that wait for the second tile are slots
+// with nothing in flight (118 us); weights in one contiguous piece a k-block (the same).
 //   warp 0  TMA producer
 //   warp 1  MMA issuer
 //   warps 2..  epilogue, two or three sets of four, as in ep_token_gemm_kernel
