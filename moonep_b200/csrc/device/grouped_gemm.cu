@@ -274,6 +274,18 @@ static bool fused_dispatch_cooperative() {
   return v != 0;
 }
 
+// SMs of the current device, asked once.
+static int device_sms() {
+  static std::atomic<int> known[64];
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  if (dev < 64 && (sms = known[dev].load(std::memory_order_relaxed)) > 0) return sms;
+  sms = 148;
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (dev < 64) known[dev].store(sms, std::memory_order_relaxed);
+  return sms;
+}
+
 // CTA-pair launch: clusters of two CTAs, one pair per two SMs.  `coop`: the whole grid must be
 // resident at once.
 struct PairLaunch {
@@ -312,9 +324,7 @@ static int launch_pair(const void* kern, PairLaunch& once, const Params& kp, int
     // a launch with a CTA limit shares the GPU with a copy kernel that is placed as SM pairs too:
     // leave it its pairs out of what the device can hold, or this persistent grid would need a
     // second wave
-    int dev = 0, sms = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const int sms = device_sms();
     if (grid < sms && most < (1 << 20)) use = most - (sms - grid + 1) / 2;
     if (use < 1) use = 1;
   }
@@ -661,9 +671,7 @@ int mep_mx_gemm_launch(const MxDesc* d, cudaStream_t stream) {
   p.vec_out = d->ldc % 8 == 0 && (((uintptr_t)d->out | (uintptr_t)d->gate | (uintptr_t)d->up) & 15) == 0;
   p.row_scale = d->row_scale; p.ldc = d->ldc; p.status = d->status;
   p.timeout_ns = (unsigned long long)(d->timeout_ns > 0 ? d->timeout_ns : 2000000000ll);
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int sms = device_sms();
   p.zero_tail = d->zero_tail; p.check_groups = d->check_groups;
   p.d_act = d->d_act; p.d_scale = d->d_scale;
   if (d->d_act != nullptr) {

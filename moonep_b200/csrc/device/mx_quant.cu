@@ -346,41 +346,58 @@ extern "C" {
 // x [mats][rows][cols] of `type` (bf16, fp16, fp32), `batch` and `stride` elements apart.  along_cols = 0: blocks along the
 // columns, output rows are x's; 1: blocks along the rows, output rows are x's columns.  out_rows: rows of an output matrix.
 // phases = 4 (one matrix): scales for token rows, else 1.  x2 (along_cols = 1): the up projection packed with x, the gate.
-int mep_mx_quantize(const void* x, const void* x2, int type, int64_t batch, int64_t stride, int mats, int rows, int cols, int along_cols,
-                    int out_rows, int phases, const int32_t* rows_ptr, void* codes, void* scales, cudaStream_t stream) {
-  if (mats < 0 || rows < 0 || cols < 0 || cols > 0x7F000000 || (int64_t)mats * rows > 0x7FFFFFFF)
-    return fail(-1, "mx quantise: %d x %d x %d elements", mats, rows, cols);
-  if (x2 && (!along_cols || phases != 1)) return fail(-2, "mx quantise: a pair is packed along the columns");
-  if (along_cols && rows_ptr) return fail(-2, "mx quantise: a device row count goes with blocks along the rows");
-  if (phases != 1 && (phases != MX_PHASES || mats > 1)) return fail(-4, "mx quantise: %d phases of %d matrices", phases, mats);
-  if (mats == 0 || rows == 0 || cols == 0) return 0;
+// rows_ptr: rows of x that hold something, on the device; or null.
+struct MxQuantDesc {
+  const void *x, *x2;
+  void *codes, *scales;
+  const int32_t* rows_ptr;
+  int64_t batch, stride;
+  int32_t type, mats, rows, cols, along_cols, out_rows, phases, unused;
+};
+// The values [mats][rows][cols] in bf16, or fp32; of a pair [2][mats][rows][cols].
+struct MxDequantDesc {
+  const void *codes, *scales;
+  void* out;
+  const int32_t* rows_ptr;
+  int32_t mats, rows, cols, pair, in_rows, fp32;
+};
+
+int mep_mx_quant_desc_bytes() { return (int)(sizeof(MxQuantDesc) << 16 | sizeof(MxDequantDesc)); }
+
+int mep_mx_quantize(const MxQuantDesc* d, cudaStream_t stream) {
+  if (d->mats < 0 || d->rows < 0 || d->cols < 0 || d->cols > 0x7F000000 || (int64_t)d->mats * d->rows > 0x7FFFFFFF)
+    return fail(-1, "mx quantise: %d x %d x %d elements", d->mats, d->rows, d->cols);
+  const bool along_cols = d->along_cols != 0;
+  if (d->x2 && (!along_cols || d->phases != 1)) return fail(-2, "mx quantise: a pair is packed along the columns");
+  if (along_cols && d->rows_ptr) return fail(-2, "mx quantise: a device row count goes with blocks along the rows");
+  if (d->phases != 1 && (d->phases != MX_PHASES || d->mats > 1))
+    return fail(-4, "mx quantise: %d phases of %d matrices", d->phases, d->mats);
+  if (d->mats == 0 || d->rows == 0 || d->cols == 0) return 0;
   MxQuantParams p;
-  const int K = along_cols ? rows : cols;
-  p.x = x; p.x2 = x2; p.batch = batch; p.stride = stride; p.mats = mats; p.rows = rows; p.cols = cols;
-  p.out_rows = out_rows; p.code_bytes = (K + MX_BLOCK - 1) / MX_BLOCK * (MX_BLOCK / 2);
-  p.k_atoms = mx_atoms(K); p.row_atoms = mx_atoms(out_rows);
-  p.codes = (uint8_t*)codes; p.scales = (uint8_t*)scales; p.rows_ptr = rows_ptr; p.phases = phases;
-  if (type == MX_BF16) return mx_quant<__nv_bfloat16>(p, along_cols != 0, stream);
-  if (type == MX_FP16) return mx_quant<__half>(p, along_cols != 0, stream);
-  if (type == MX_FP32) return mx_quant<float>(p, along_cols != 0, stream);
-  return fail(-3, "mx quantise: unknown type %d", type);
+  const int K = along_cols ? d->rows : d->cols;
+  p.x = d->x; p.x2 = d->x2; p.batch = d->batch; p.stride = d->stride; p.mats = d->mats; p.rows = d->rows; p.cols = d->cols;
+  p.out_rows = d->out_rows; p.code_bytes = (K + MX_BLOCK - 1) / MX_BLOCK * (MX_BLOCK / 2);
+  p.k_atoms = mx_atoms(K); p.row_atoms = mx_atoms(d->out_rows);
+  p.codes = (uint8_t*)d->codes; p.scales = (uint8_t*)d->scales; p.rows_ptr = d->rows_ptr; p.phases = d->phases;
+  if (d->type == MX_BF16) return mx_quant<__nv_bfloat16>(p, along_cols, stream);
+  if (d->type == MX_FP16) return mx_quant<__half>(p, along_cols, stream);
+  if (d->type == MX_FP32) return mx_quant<float>(p, along_cols, stream);
+  return fail(-3, "mx quantise: unknown type %d", d->type);
 }
 
-// The values [mats][rows][cols] in bf16, or fp32; of a pair [2][mats][rows][cols].
-int mep_mx_dequantize(const void* codes, const void* scales, int mats, int rows, int cols, int pair, int in_rows,
-                      const int32_t* rows_ptr, int fp32, void* out, cudaStream_t stream) {
-  if (mats < 0 || rows < 0 || cols < 0 || cols > 0x7F000000 || (pair ? 2 : 1) * (int64_t)mats * rows > 0x7FFFFFFF)
-    return fail(-1, "mx dequantise: %d x %d x %d elements", mats, rows, cols);
-  if (mats == 0 || rows == 0 || cols == 0) return 0;
+int mep_mx_dequantize(const MxDequantDesc* d, cudaStream_t stream) {
+  if (d->mats < 0 || d->rows < 0 || d->cols < 0 || d->cols > 0x7F000000 || (d->pair ? 2 : 1) * (int64_t)d->mats * d->rows > 0x7FFFFFFF)
+    return fail(-1, "mx dequantise: %d x %d x %d elements", d->mats, d->rows, d->cols);
+  if (d->mats == 0 || d->rows == 0 || d->cols == 0) return 0;
   MxDequantParams p;
-  p.codes = (const uint8_t*)codes; p.scales = (const uint8_t*)scales; p.mats = mats; p.rows = rows; p.cols = cols;
-  p.in_rows = in_rows; p.code_bytes = (cols + MX_BLOCK - 1) / MX_BLOCK * (MX_BLOCK / 2);
-  p.k_atoms = mx_atoms(cols); p.row_atoms = mx_atoms(in_rows);
-  p.out = out; p.rows_ptr = rows_ptr; p.pair = pair;
-  const dim3 grid = mx_grid((pair ? 2ll : 1ll) * mats * rows, (cols + 256 * MXD_DEPTH - 1) / (256 * MXD_DEPTH));
-  const bool vec = cols % 8 == 0 && (uintptr_t)out % 16 == 0;
-  const void* kern = fp32 ? (vec ? (const void*)ep_mx_dequant_kernel<float, true> : (const void*)ep_mx_dequant_kernel<float, false>)
-                          : (vec ? (const void*)ep_mx_dequant_kernel<__nv_bfloat16, true> : (const void*)ep_mx_dequant_kernel<__nv_bfloat16, false>);
+  p.codes = (const uint8_t*)d->codes; p.scales = (const uint8_t*)d->scales; p.mats = d->mats; p.rows = d->rows; p.cols = d->cols;
+  p.in_rows = d->in_rows; p.code_bytes = (d->cols + MX_BLOCK - 1) / MX_BLOCK * (MX_BLOCK / 2);
+  p.k_atoms = mx_atoms(d->cols); p.row_atoms = mx_atoms(d->in_rows);
+  p.out = d->out; p.rows_ptr = d->rows_ptr; p.pair = d->pair;
+  const dim3 grid = mx_grid((d->pair ? 2ll : 1ll) * d->mats * d->rows, (d->cols + 256 * MXD_DEPTH - 1) / (256 * MXD_DEPTH));
+  const bool vec = d->cols % 8 == 0 && (uintptr_t)d->out % 16 == 0;
+  const void* kern = d->fp32 ? (vec ? (const void*)ep_mx_dequant_kernel<float, true> : (const void*)ep_mx_dequant_kernel<float, false>)
+                             : (vec ? (const void*)ep_mx_dequant_kernel<__nv_bfloat16, true> : (const void*)ep_mx_dequant_kernel<__nv_bfloat16, false>);
   MEP_CUDA_OK(launch_chained(kern, grid, dim3(MXQ_WARPS * 32), 0, stream, p, 0, 1));
   return 0;
 }

@@ -40,14 +40,19 @@ BLOCK = 32
 PHASES = 4
 
 
-# The product's descriptor, as the C side lays it out: four operand pointers; rows, K, groups, weight rows, N, gated, zero_tail, check_groups; cu_seqlens,
-# pads, row_scale, out, gate, up, codes, scales, d_act, d_scale; ldc, status, timeout.  (Packed in one call: filling a ctypes structure
-# field by field took as long as the launch.)
+# Descriptors, as the C side lays them out, packed in one call: filling a ctypes structure field by field, or converting as
+# many arguments, took as long as the launch.
+# product: four operand pointers; rows, K, groups, weight rows, N, gated, zero_tail, check_groups; cu_seqlens, pads,
+#   row_scale, out, gate, up, codes, scales, d_act, d_scale; ldc, status, timeout
+# quantise: x, x2, codes, scales, rows_ptr; batch, stride; type, mats, rows, cols, along_cols, out_rows, phases, unused
+# dequantise: codes, scales, out, rows_ptr; mats, rows, cols, pair, in_rows, fp32
 _DESC = struct.Struct("@4P8i10PqPq")
+_QUANT = struct.Struct("@5P2q8i")
+_DEQUANT = struct.Struct("@4P6i")
 
-
-nat.declare("mep_mx_quantize", I, [P, P, I, L, L, I, I, I, I, I, I, P, P, P, P])
-nat.declare("mep_mx_dequantize", I, [P, P, I, I, I, I, I, P, I, P, P])
+nat.declare("mep_mx_quant_desc_bytes", I, [])
+nat.declare("mep_mx_quantize", I, [ctypes.c_char_p, P])
+nat.declare("mep_mx_dequantize", I, [ctypes.c_char_p, P])
 nat.declare("mep_mx_desc_bytes", I, [])
 nat.declare("mep_mx_zero_tail", I, [P, I, L, P, P])
 nat.declare("mep_mx_sum_parts", I, [P, I, I, P, P, P])
@@ -58,12 +63,24 @@ _MAX = 2 ** 31 - 1
 _checked_layout = False
 
 
+def _launch_native(name: str, desc: bytes, what: str) -> None:
+    global _checked_layout
+    if not _checked_layout:
+        assert nat.call("mep_mx_desc_bytes") == _DESC.size, "MxDesc layout mismatch"
+        assert nat.call("mep_mx_quant_desc_bytes") == (_QUANT.size << 16 | _DEQUANT.size), "MxQuantDesc layout mismatch"
+        _checked_layout = True
+    rc = nat.call(name, desc, nat.stream())
+    if rc != 0:
+        ew._rc(rc, what)
+
+
 _device = torch._C._cuda_getDevice       # (torch.cuda.current_device() without its check that CUDA is initialised)
 
 
 def _here(t: torch.Tensor, name: str) -> torch.Tensor:
-    assert t.is_cuda, f"{name} must be a CUDA tensor"
-    assert t.get_device() == _device(), f"{name} is on {t.device}, not on the current device"
+    at = t.get_device()
+    assert at >= 0, f"{name} must be a CUDA tensor"
+    assert at == _device(), f"{name} is on {t.device}, not on the current device"
     return t
 
 
@@ -96,24 +113,30 @@ class MxTensor:
             f"a tensor of shape {shape} has codes and scales of {sizes}"
         assert codes.data_ptr() % 16 == 0 and scales.data_ptr() % 16 == 0, "codes and scales must be 16-byte aligned"
         self._codes, self._scales, self._data = codes, scales, codes
-        self._set(shape, sizes, (codes.data_ptr(), scales.data_ptr()))
+        self._set(shape, sizes[0][-2], codes.get_device(), (codes.data_ptr(), scales.data_ptr()))
 
-    def _set(self, shape, sizes, at):
-        self.shape, self._at = shape, at              # (addresses of codes and scales)
-        self._index = self._data.get_device()
-        self._mats, self._rows = (1 if len(shape) == 2 else shape[-3]), sizes[0][-2]
+    def _set(self, shape, rows: int, index: int, at):
+        self.shape, self._index, self._at = shape, index, at          # (addresses of codes and scales)
+        self._mats, self._rows = (1 if len(shape) == 2 else shape[-3]), rows
         return self
 
     @classmethod
-    def _empty(cls, shape, device) -> "MxTensor":
+    def _empty(cls, shape, device, index: int) -> "MxTensor":
         """A new one; codes and scales share an allocation, whose two views are made when somebody asks for them."""
-        sizes = _sizes(shape)
-        n = (math.prod(sizes[0]) + 511) // 512 * 512
+        rows, K = shape[-2], shape[-1]
+        copies = mats = 1
+        if len(shape) == 2:
+            copies = PHASES
+        else:
+            copies = mats = shape[-3]
+            if len(shape) == 4:
+                rows = (rows + 15) // 16 * 32
+        n = (mats * rows * ((K + 31) // 32 * 16) + 511) // 512 * 512
         self = cls.__new__(cls)
-        self._data = torch.empty(n + math.prod(sizes[1]), dtype=torch.uint8, device=device)
+        self._data = data = torch.empty(n + copies * ((rows + 127) // 128) * ((K + 127) // 128) * 512, dtype=torch.uint8, device=device)
         self._codes = self._scales = None
-        at = self._data.data_ptr()
-        return self._set(shape, sizes, (at, at + n))
+        at = data.data_ptr()
+        return self._set(shape, rows, index, (at, at + n))
 
     def _views(self):
         if self._codes is None:
@@ -149,10 +172,9 @@ class MxTensor:
         pair = len(self.shape) == 4
         assert rows_ptr is None or len(self.shape) == 2, "rows_ptr goes with one matrix"
         out = torch.empty(self.shape, dtype=dtype, device=self._data.device)
-        rc = nat.call("mep_mx_dequantize", *self._at, self._mats, self.shape[-2], self.shape[-1], int(pair), self._rows,
-                      _rows_ptr(rows_ptr, self._index), int(dtype == torch.float32), out.data_ptr(), nat.stream())
-        if rc != 0:
-            ew._rc(rc, "mx dequantise")
+        _launch_native("mep_mx_dequantize",
+                       _DEQUANT.pack(*self._at, out.data_ptr(), _rows_ptr(rows_ptr, self._index), self._mats, self.shape[-2],
+                                     self.shape[-1], pair, self._rows, dtype is torch.float32), "mx dequantise")
         return out
 
 
@@ -171,12 +193,10 @@ def _sizes(shape):
 
 def _quantize_into(q: MxTensor, x: torch.Tensor, axis: int, rows_ptr=None, up: int = 0) -> None:
     size, stride = x.shape, x.stride()
-    three = len(size) == 3
-    rc = nat.call("mep_mx_quantize", x.data_ptr(), up, _TYPES[x.dtype], stride[0] if three else 0, stride[-2], size[0] if three else 1,
-                  size[-2], size[-1], int(axis == -2), q._rows, 1 if len(q.shape) > 2 else PHASES,
-                  _rows_ptr(rows_ptr, q._index), *q._at, nat.stream())
-    if rc != 0:
-        ew._rc(rc, "mx quantise")
+    batch, mats = (stride[0], size[0]) if len(size) == 3 else (0, 1)
+    _launch_native("mep_mx_quantize",
+                   _QUANT.pack(x.data_ptr(), up, *q._at, _rows_ptr(rows_ptr, q._index), batch, stride[-2], _TYPES[x.dtype], mats,
+                               size[-2], size[-1], axis == -2, q._rows, PHASES if len(q.shape) == 2 else 1, 0), "mx quantise")
 
 
 def _operand(x: torch.Tensor, name: str) -> torch.Tensor:
@@ -198,9 +218,11 @@ def quantize(x: torch.Tensor, axis: int = -1, *, rows_ptr: Optional[torch.Tensor
     _operand(x, "x")
     assert axis in (-1, -2), "axis must be -1 or -2"
     assert rows_ptr is None or (x.dim() == 2 and axis == -1), "rows_ptr goes with one matrix and axis=-1"
-    shape = tuple(x.shape) if axis == -1 else (*x.shape[:-2], x.shape[-1], x.shape[-2])
-    assert shape[-1] >= 1, "the reduction is empty"
-    q = MxTensor._empty(shape, x.device)
+    shape = tuple(x.shape)
+    if axis == -2:
+        shape = (*shape[:-2], shape[-1], shape[-2])
+        assert shape[-1] >= 1, "the reduction is empty"
+    q = MxTensor._empty(shape, x.device, x.get_device())
     _quantize_into(q, x, axis, rows_ptr)
     return q
 
@@ -216,14 +238,13 @@ def pack_gate_up(wg: torch.Tensor, wu: torch.Tensor) -> MxTensor:
     if wg.stride() != wu.stride():
         wg, wu = wg.contiguous(), wu.contiguous()
     G, H, Hp = wg.shape
-    q = MxTensor._empty((2, G, Hp, H), wg.device)
+    q = MxTensor._empty((2, G, Hp, H), wg.device, wg.get_device())
     _quantize_into(q, wg, -2, up=wu.data_ptr())
     return q
 
 
 def _launch(a: MxTensor, w: MxTensor, N: int, gated: int, cu_seqlens, pads, row_scale, out: int, gate: int, up: int, codes: int,
             scales: int, ldc: int, d_act: int = 0, d_scale: int = 0, zero_tail: int = 0, check_groups: int = 0) -> None:
-    global _checked_layout
     index, groups, (rows, K) = a._index, w._mats, a.shape
     assert index == _device(), "the operands are not on the current device"
     assert w._index == index and w.shape[-1] == K, "operands do not go together"
@@ -232,28 +253,23 @@ def _launch(a: MxTensor, w: MxTensor, N: int, gated: int, cu_seqlens, pads, row_
     if cu_seqlens is None:
         assert groups == 1, "several groups need cu_seqlens"
     else:
-        assert cu_seqlens.dtype == torch.int32 and cu_seqlens.get_device() == index and cu_seqlens.is_contiguous() \
+        assert cu_seqlens.dtype is torch.int32 and cu_seqlens.get_device() == index and cu_seqlens.is_contiguous() \
             and cu_seqlens.numel() == groups, "cu_seqlens must be int32, one entry a group"
         cu = cu_seqlens.data_ptr()
         if pads is not None:
-            assert pads.get_device() == index
-            pad = gemm._pads(pads, cu_seqlens)
+            assert pads.dtype is torch.int32 and pads.get_device() == index and pads.is_contiguous() and pads.dim() == 2 \
+                and pads.shape[1] == 2 and pads.shape[0] >= groups, "pads must be int32 [groups, 2]"
+            pad = pads.data_ptr()
     if row_scale is not None:
-        assert row_scale.dtype == torch.float32 and row_scale.get_device() == index and row_scale.is_contiguous() \
+        assert row_scale.dtype is torch.float32 and row_scale.get_device() == index and row_scale.is_contiguous() \
             and row_scale.dim() == 1 and row_scale.numel() >= rows, "row_scale must be fp32, one a row"
         scale = row_scale.data_ptr()
     status = gemm._status.get(index)
     if status is None:
         status = gemm.status_word(a.device)
-    if not _checked_layout:
-        assert nat.call("mep_mx_desc_bytes") == _DESC.size, "MxDesc layout mismatch"
-        _checked_layout = True
-    rc = nat.call("mep_mx_gemm_launch",
-                  _DESC.pack(*a._at, *w._at, rows, K, groups, w._rows, N, gated, zero_tail, check_groups, cu, pad, scale, out, gate, up, codes, scales,
-                             d_act, d_scale, ldc, status.data_ptr(), 0),
-                  nat.stream())
-    if rc != 0:
-        ew._rc(rc, "mx product")
+    _launch_native("mep_mx_gemm_launch",
+                   _DESC.pack(*a._at, *w._at, rows, K, groups, w._rows, N, gated, zero_tail, check_groups, cu, pad, scale, out, gate,
+                              up, codes, scales, d_act, d_scale, ldc, status.data_ptr(), 0), "mx product")
 
 
 def matmul(a: MxTensor, w: MxTensor, cu_seqlens: Optional[torch.Tensor] = None, *, out: Optional[torch.Tensor] = None,
@@ -296,7 +312,7 @@ def gateup_swiglu(a: MxTensor, wgu: MxTensor, cu_seqlens: Optional[torch.Tensor]
     if save_gate_up:
         gate, up = (torch.empty((rows, Hp), dtype=torch.bfloat16, device=device) for _ in range(2))
     if quantize:
-        act = MxTensor._empty((rows, Hp), device)
+        act = MxTensor._empty((rows, Hp), device, a._index)
         outs = 0, nat.ptr(gate), nat.ptr(up), *act._at
     else:
         act = torch.empty((rows, Hp), dtype=torch.bfloat16, device=device)
