@@ -95,9 +95,9 @@ __device__ __forceinline__ MxEight<T> mx_load8(const T* row, int c, int cols) {
 }
 
 // Along the rows.  A warp takes MXQ_DEPTH parts of 256 elements of a row, a lane eight of each: four lanes share a
-// block, sixteen the four scales of an atom's row, which leave as one word (a phase).  Bound by HBM, and next to it by
-// issue: 8192 x 7168 in bf16 30 us, 5.0 TB/s; fp32 42 us, 6.3.  (Sixteen elements a lane are fewer instructions, but two
-// 16-byte accesses of a lane side by side: 14336 x 7168 51.6 us, 53.7; odd rows 48, 72; 32 x 7168 x 2048 215, 201.)
+// block and store its scale, a phase each.  Bound by HBM: 8192 x 7168 in bf16 30 us, 5.0 TB/s with the launch, fp32 42 us,
+// 6.3.  (Sixteen elements a lane are fewer instructions, but two 16-byte accesses of a lane side by side: 14336 x 7168
+// 51.6 us, 53.7; odd rows 48, 72; 32 x 7168 x 2048 215, 201.)
 constexpr int MXQ_WARPS = 8, MXQ_DEPTH = 4;
 
 template <class T, bool VEC>
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(MXQ_WARPS * 32) ep_mx_quant_rows_kernel(const 
     const int mat = p.mats > 1 ? (int)(line / (unsigned)rows) : 0, row = (int)(line - (unsigned)mat * (unsigned)rows);
     const T* x = (const T*)p.x + mat * p.batch + row * p.stride;
     uint8_t* codes = p.codes + ((long long)mat * p.out_rows + row) * p.code_bytes;
-    uint32_t* scales = mx_scale_row(p, mat, row, lane & 15);       // of this lane's phase, if it has one
+    uint8_t* scales = reinterpret_cast<uint8_t*>(mx_scale_row(p, mat, row, lane & 3));    // of this lane's phase, if it has one
     for (int c0 = blockIdx.y * 256 * MXQ_DEPTH; c0 < p.cols; c0 += gridDim.y * 256 * MXQ_DEPTH) {
       MxEight<T> raw[MXQ_DEPTH];
 #pragma unroll
@@ -134,11 +134,7 @@ __global__ void __launch_bounds__(MXQ_WARPS * 32) ep_mx_quant_rows_kernel(const 
         // (a NaN scale: zeros, whatever inf * 0 would give)
         const uint32_t q = b == 255u ? 0u : mx_codes(v);
         if (c < 2 * p.code_bytes) *reinterpret_cast<uint32_t*>(codes + c / 2) = q;
-        // bytes of lanes 0, 4, 8, 12 (16, ...) to their sixteen lanes
-        uint32_t w = b | (__shfl_xor_sync(0xffffffffu, b, 4) << 8);
-        w = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 8), 0x5410);
-        w = __shfl_sync(0xffffffffu, w, lane & 16);
-        if (scales != nullptr && c < p.k_atoms * MX_ATOM_K) scales[(long long)(c >> 7) * (MX_ATOM_BYTES / 4)] = w;
+        if (scales != nullptr && c < p.k_atoms * MX_ATOM_K) scales[(c >> 7) * (long long)MX_ATOM_BYTES + (c >> 5 & 3)] = (uint8_t)b;
       }
     }
   }
