@@ -63,12 +63,16 @@ _MAX = 2 ** 31 - 1
 _checked_layout = False
 
 
-def _launch_native(name: str, desc: bytes, what: str) -> None:
+def _check_layouts() -> None:
     global _checked_layout
+    assert nat.call("mep_mx_desc_bytes") == _DESC.size, "MxDesc layout mismatch"
+    assert nat.call("mep_mx_quant_desc_bytes") == (_QUANT.size << 16 | _DEQUANT.size), "MxQuantDesc layout mismatch"
+    _checked_layout = True
+
+
+def _launch_native(name: str, desc: bytes, what: str) -> None:
     if not _checked_layout:
-        assert nat.call("mep_mx_desc_bytes") == _DESC.size, "MxDesc layout mismatch"
-        assert nat.call("mep_mx_quant_desc_bytes") == (_QUANT.size << 16 | _DEQUANT.size), "MxQuantDesc layout mismatch"
-        _checked_layout = True
+        _check_layouts()
     rc = nat.call(name, desc, nat.stream())
     if rc != 0:
         ew._rc(rc, what)
@@ -77,11 +81,12 @@ def _launch_native(name: str, desc: bytes, what: str) -> None:
 _device = torch._C._cuda_getDevice       # (torch.cuda.current_device() without its check that CUDA is initialised)
 
 
-def _here(t: torch.Tensor, name: str) -> torch.Tensor:
+def _here(t: torch.Tensor, name: str) -> int:
+    """Index of the current device, which ``t`` has to be on."""
     at = t.get_device()
     assert at >= 0, f"{name} must be a CUDA tensor"
     assert at == _device(), f"{name} is on {t.device}, not on the current device"
-    return t
+    return at
 
 
 def _rows_ptr(rows_ptr, index: int) -> int:
@@ -113,30 +118,27 @@ class MxTensor:
             f"a tensor of shape {shape} has codes and scales of {sizes}"
         assert codes.data_ptr() % 16 == 0 and scales.data_ptr() % 16 == 0, "codes and scales must be 16-byte aligned"
         self._codes, self._scales, self._data = codes, scales, codes
-        self._set(shape, sizes[0][-2], codes.get_device(), (codes.data_ptr(), scales.data_ptr()))
-
-    def _set(self, shape, rows: int, index: int, at):
-        self.shape, self._index, self._at = shape, index, at          # (addresses of codes and scales)
-        self._mats, self._rows = (1 if len(shape) == 2 else shape[-3]), rows
-        return self
+        self.shape, self._index = shape, codes.get_device()
+        self._at = codes.data_ptr(), scales.data_ptr()
+        self._mats, self._rows = (1 if len(shape) == 2 else shape[-3]), sizes[0][-2]
 
     @classmethod
     def _empty(cls, shape, device, index: int) -> "MxTensor":
         """A new one; codes and scales share an allocation, whose two views are made when somebody asks for them."""
         rows, K = shape[-2], shape[-1]
-        copies = mats = 1
         if len(shape) == 2:
-            copies = PHASES
+            mats, copies = 1, PHASES
         else:
-            copies = mats = shape[-3]
+            mats = copies = shape[-3]
             if len(shape) == 4:
                 rows = (rows + 15) // 16 * 32
-        n = (mats * rows * ((K + 31) // 32 * 16) + 511) // 512 * 512
+        n = (mats * rows * ((K + 31) // 32) + 31) // 32 * 512
         self = cls.__new__(cls)
         self._data = data = torch.empty(n + copies * ((rows + 127) // 128) * ((K + 127) // 128) * 512, dtype=torch.uint8, device=device)
         self._codes = self._scales = None
         at = data.data_ptr()
-        return self._set(shape, rows, index, (at, at + n))
+        self.shape, self._index, self._mats, self._rows, self._at = shape, index, mats, rows, (at, at + n)
+        return self
 
     def _views(self):
         if self._codes is None:
@@ -167,14 +169,17 @@ class MxTensor:
     def dequantize(self, dtype: torch.dtype = torch.bfloat16, *, rows_ptr: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The values, bf16 (exact down to 2^-133, the last bit of its subnormals) or fp32, of this tensor's shape;
         gate first, then up, for a packed pair.  ``rows_ptr`` as in :func:`quantize`."""
-        assert dtype in (torch.bfloat16, torch.float32), "values are bf16 or fp32"
-        _here(self._data, "the operand")
-        pair = len(self.shape) == 4
-        assert rows_ptr is None or len(self.shape) == 2, "rows_ptr goes with one matrix"
-        out = torch.empty(self.shape, dtype=dtype, device=self._data.device)
+        assert dtype is torch.bfloat16 or dtype is torch.float32, "values are bf16 or fp32"
+        data, shape = self._data, self.shape
+        index = _here(data, "the operand")
+        count = 0
+        if rows_ptr is not None:
+            assert len(shape) == 2, "rows_ptr goes with one matrix"
+            count = _rows_ptr(rows_ptr, index)
+        out = torch.empty(shape, dtype=dtype, device=data.device)
         _launch_native("mep_mx_dequantize",
-                       _DEQUANT.pack(*self._at, out.data_ptr(), _rows_ptr(rows_ptr, self._index), self._mats, self.shape[-2],
-                                     self.shape[-1], pair, self._rows, dtype is torch.float32), "mx dequantise")
+                       _DEQUANT.pack(*self._at, out.data_ptr(), count, self._mats, shape[-2], shape[-1], len(shape) == 4, self._rows,
+                                     dtype is torch.float32), "mx dequantise")
         return out
 
 
@@ -191,22 +196,16 @@ def _sizes(shape):
     return (G, rows, code_bytes), (G, atoms, k_atoms, 512)
 
 
-def _quantize_into(q: MxTensor, x: torch.Tensor, axis: int, rows_ptr=None, up: int = 0) -> None:
-    size, stride = x.shape, x.stride()
-    batch, mats = (stride[0], size[0]) if len(size) == 3 else (0, 1)
-    _launch_native("mep_mx_quantize",
-                   _QUANT.pack(x.data_ptr(), up, *q._at, _rows_ptr(rows_ptr, q._index), batch, stride[-2], _TYPES[x.dtype], mats,
-                               size[-2], size[-1], axis == -2, q._rows, PHASES if len(q.shape) == 2 else 1, 0), "mx quantise")
-
-
-def _operand(x: torch.Tensor, name: str) -> torch.Tensor:
-    _here(x, name)
-    assert x.dtype in _TYPES, f"{name} must be bf16, fp16 or fp32"
-    size = x.shape
-    assert len(size) in (2, 3), f"{name} must be [rows, K] or [G, rows, K]"
-    assert size[-1] >= 1 and size[-2] <= _MAX and size[-1] <= _MAX
-    assert size[-1] == 1 or x.stride(-1) == 1, f"{name} must be dense along its last axis"
-    return x
+def _operand(x: torch.Tensor, name: str):
+    """Device, sizes, strides and type of what is to be quantised."""
+    index = _here(x, name)
+    size, stride, kind = x.shape, x.stride(), _TYPES.get(x.dtype)
+    assert kind is not None, f"{name} must be bf16, fp16 or fp32"
+    assert len(size) == 2 or len(size) == 3, f"{name} must be [rows, K] or [G, rows, K]"
+    cols = size[-1]
+    assert 1 <= cols <= _MAX and size[-2] <= _MAX, f"{name} has no columns, or too many rows"
+    assert cols == 1 or stride[-1] == 1, f"{name} must be dense along its last axis"
+    return index, size, stride, kind
 
 
 def quantize(x: torch.Tensor, axis: int = -1, *, rows_ptr: Optional[torch.Tensor] = None) -> MxTensor:
@@ -215,38 +214,49 @@ def quantize(x: torch.Tensor, axis: int = -1, *, rows_ptr: Optional[torch.Tensor
 
     ``rows_ptr`` (device int32, one matrix, ``axis=-1``) bounds the rows that are read without a host sync; the others'
     codes and scales are left undefined.  No gradient passes (see :func:`expert_ffn`)."""
-    _operand(x, "x")
-    assert axis in (-1, -2), "axis must be -1 or -2"
-    assert rows_ptr is None or (x.dim() == 2 and axis == -1), "rows_ptr goes with one matrix and axis=-1"
-    shape = tuple(x.shape)
-    if axis == -2:
-        shape = (*shape[:-2], shape[-1], shape[-2])
-        assert shape[-1] >= 1, "the reduction is empty"
-    q = MxTensor._empty(shape, x.device, x.get_device())
-    _quantize_into(q, x, axis, rows_ptr)
+    index, size, stride, kind = _operand(x, "x")
+    assert axis == -1 or axis == -2, "axis must be -1 or -2"
+    rows, cols = size[-2], size[-1]
+    mats, batch = (size[0], stride[0]) if len(size) == 3 else (1, 0)
+    count, one = 0, len(size) == 2
+    if rows_ptr is not None:
+        assert one and axis == -1, "rows_ptr goes with one matrix and axis=-1"
+        count = _rows_ptr(rows_ptr, index)
+    if axis == -1:
+        n, k = rows, cols
+    else:
+        n, k = cols, rows
+        assert k >= 1, "the reduction is empty"
+    q = MxTensor._empty((n, k) if one else (mats, n, k), x.device, index)
+    _launch_native("mep_mx_quantize",
+                   _QUANT.pack(x.data_ptr(), 0, *q._at, count, batch, stride[-2], kind, mats, rows, cols, axis == -2, n,
+                               PHASES if one else 1, 0), "mx quantise")
     return q
 
 
 def pack_gate_up(wg: torch.Tensor, wu: torch.Tensor) -> MxTensor:
     """Gate and up projections ``[G, H, H']`` (or one expert's ``[H, H']``), quantised along H, as the one operand of
     :func:`gateup_swiglu`; its ``shape`` is ``[2, G, H', H]``."""
-    _operand(wg, "wg"), _operand(wu, "wu")
-    assert wg.shape == wu.shape and wg.dtype == wu.dtype and wg.device == wu.device, "wg and wu must be alike"
-    assert wg.shape[-2] >= 1, "the reduction is empty"
-    if wg.dim() == 2:
-        wg, wu = wg[None], wu[None]
-    if wg.stride() != wu.stride():
+    index, size, stride, kind = _operand(wg, "wg")
+    _operand(wu, "wu")
+    assert size == wu.shape and wg.dtype == wu.dtype, "wg and wu must be alike"
+    assert size[-2] >= 1, "the reduction is empty"
+    if stride != wu.stride():
         wg, wu = wg.contiguous(), wu.contiguous()
-    G, H, Hp = wg.shape
-    q = MxTensor._empty((2, G, Hp, H), wg.device, wg.get_device())
-    _quantize_into(q, wg, -2, up=wu.data_ptr())
+        stride = wg.stride()
+    G, batch = (size[0], stride[0]) if len(size) == 3 else (1, 0)
+    H, Hp = size[-2], size[-1]
+    q = MxTensor._empty((2, G, Hp, H), wg.device, index)
+    _launch_native("mep_mx_quantize",
+                   _QUANT.pack(wg.data_ptr(), wu.data_ptr(), *q._at, 0, batch, stride[-2], kind, G, H, Hp, 1, q._rows, 1, 0),
+                   "mx quantise")
     return q
 
 
 def _launch(a: MxTensor, w: MxTensor, N: int, gated: int, cu_seqlens, pads, row_scale, out: int, gate: int, up: int, codes: int,
             scales: int, ldc: int, d_act: int = 0, d_scale: int = 0, zero_tail: int = 0, check_groups: int = 0) -> None:
     index, groups, (rows, K) = a._index, w._mats, a.shape
-    assert index == _device(), "the operands are not on the current device"
+    assert index >= 0 and index == _device(), "the operands are not on the current device"
     assert w._index == index and w.shape[-1] == K, "operands do not go together"
     assert 1 <= groups <= 1024, "1 to 1024 groups"
     cu = pad = scale = 0
@@ -257,8 +267,9 @@ def _launch(a: MxTensor, w: MxTensor, N: int, gated: int, cu_seqlens, pads, row_
             and cu_seqlens.numel() == groups, "cu_seqlens must be int32, one entry a group"
         cu = cu_seqlens.data_ptr()
         if pads is not None:
-            assert pads.dtype is torch.int32 and pads.get_device() == index and pads.is_contiguous() and pads.dim() == 2 \
-                and pads.shape[1] == 2 and pads.shape[0] >= groups, "pads must be int32 [groups, 2]"
+            size = pads.shape
+            assert pads.dtype is torch.int32 and pads.get_device() == index and pads.is_contiguous() and len(size) == 2 \
+                and size[1] == 2 and size[0] >= groups, "pads must be int32 [groups, 2]"
             pad = pads.data_ptr()
     if row_scale is not None:
         assert row_scale.dtype is torch.float32 and row_scale.get_device() == index and row_scale.is_contiguous() \
@@ -432,7 +443,7 @@ def expert_ffn(x: torch.Tensor, wg, wu, wd, cu_seqlens: Optional[torch.Tensor] =
     else:
         trained = (wg, wu, wd)
         for name, w in zip(("wg", "wu", "wd"), trained):
-            assert _operand(w, name).dtype == torch.bfloat16, f"{name} must be bf16"
+            assert _operand(w, name)[3] == 0, f"{name} must be bf16"
         assert wg.shape == wu.shape == wd.shape and wg.shape[-2] == H, "weights must be [G, H, H'] alike"
         Hp = wg.shape[-1]
     if row_scale is not None:
