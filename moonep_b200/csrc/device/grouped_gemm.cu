@@ -14,6 +14,7 @@
 //   ep_dense_f32_kernel (dense_f32.cuh): one product with fp32 output (router logits).
 //   ep_weight_grad_kernel (weight_grad.cuh): weight grads, fp32 or bf16 output or with the SGD step in the epilogue.
 //   ep_mx_gemm_kernel (mx_gemm.cuh): token-major products of microscaled 4-bit operands.
+//   ep_mx_dgrad_kernel (mx_dgrad.cuh): bf16 rows times such weights, along their scales.
 // Group g < split reads/writes allocation 0 (local experts), g >= split allocation 1 (this
 // rank's prefetch / reduce slots): the [2*epn] compute view never has to be contiguous.
 // CTA pairs (template TWO, clusters of two CTAs, tcgen05 cta_group::2): the leader issues
@@ -158,6 +159,7 @@ __device__ __forceinline__ int group_valid(const Params& p, int g, int start, in
 #include "device/token_gemm.cuh"
 #include "device/weight_grad.cuh"
 #include "device/mx_gemm.cuh"
+#include "device/mx_dgrad.cuh"
 
 namespace mep {
 
@@ -216,6 +218,20 @@ struct MxDesc {
   int64_t timeout_ns;
 };
 
+// bf16 rows [rows][K] (two segments: with the gate's and the up projection's weights of a packed pair) times 4-bit
+// weights [ngroups][K][N] whose blocks lie along N.
+struct MxDgradDesc {
+  const void* a[2];
+  const void *w_codes, *w_scales;
+  void* out;
+  const int32_t* cu_seqlens;
+  const int32_t* pads;
+  int64_t lda, ldc;
+  int32_t rows, K, N, nseg, ngroups, w_rows, fp32, unused;
+  int32_t* status;
+  int64_t timeout_ns;
+};
+
 typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                              CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
@@ -242,20 +258,21 @@ static int make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols
   return 0;
 }
 
-// 2-D tensor [rows][cols] of bytes in 128-byte boxes with the 128-byte swizzle, or [rows][cols / 4] words in boxes of 256
-// words x 1 row, unswizzled.
-static int make_byte_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int box_rows) {
+// 2-D tensor [rows][cols] of bytes in 128-byte boxes with the 128-byte swizzle, or, unswizzled, (box_rows 0) [rows][cols / 4]
+// words in boxes of one row and box_words, or (box_rows -16) bytes in boxes of 64 x 16 rows.
+static int make_byte_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int box_rows, int box_words = 256) {
   EncodeFn enc = (EncodeFn)driver_tensor_map_encode();
   if (!enc) return fail(-10, "CUDA driver entry cuTensorMapEncodeTiled not available");
   if (((uintptr_t)base & 15) != 0 || cols % 16 != 0) return fail(-11, "mx operands must be 16-byte aligned");
   const bool words = box_rows == 0;
   cuuint64_t dims[2] = {(cuuint64_t)(words ? cols / 4 : cols), (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)cols};
-  cuuint32_t box[2] = {words ? 256u : 128u, words ? 1u : (cuuint32_t)box_rows};
+  const bool plain = box_rows < 0;
+  cuuint32_t box[2] = {words ? (cuuint32_t)box_words : plain ? 64u : 128u, words ? 1u : (cuuint32_t)(plain ? -box_rows : box_rows)};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = enc(m, words ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims,
                    strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   words ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   words || plain ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(-12, "cuTensorMapEncodeTiled failed with code %d", (int)r);
   return 0;
@@ -512,10 +529,10 @@ int mep_gemm_launch(const GemmDesc* d, cudaStream_t stream) {
     if (bf16) return launch_wgrad<WG_BF16>(kp, pair, grid, stream);
     return kp.accumulate ? launch_wgrad<WG_ADD>(kp, pair, grid, stream) : launch_wgrad<WG_STORE>(kp, pair, grid, stream);
   }
-  const bool dense_f32 = d->epi == EPI_F32 && d->ngroups == 1 && d->cu_seqlens == nullptr;
   if (d->epi == EPI_F32) {
-    // router logits, or the down-dgrad of groups whose SwiGLU backward wants it unrounded: one segment
-    if (d->nseg != 1 || d->accumulate || d->disp_mode != 0) return fail(-15, "gemm: fp32 output is one product");
+    // router logits: one group, one segment
+    if (d->ngroups != 1 || d->cu_seqlens != nullptr || d->nseg != 1 || d->accumulate)
+      return fail(-15, "gemm: fp32 output is one dense product");
     if (d->K % 8 != 0) return fail(-4, "gemm: K=%d must be a multiple of 8", d->K);
     if (d->total_rows < 1) return 0;
   }
@@ -524,7 +541,7 @@ int mep_gemm_launch(const GemmDesc* d, cudaStream_t stream) {
   // columns 237 -> 110 us, 16384 x 2048 -> 512 86 -> 46.  Up to 128 columns half of a pair's tile would be empty:
   // single CTAs, from twice as many tiles on (65536 x 512 -> 128 49 -> 34; 32768 x 2048 -> 128 48 either way).
   const long long dn_rows = ((long long)d->total_rows * ((d->N + BM - 1) / BM) + grid - 1) / grid;
-  if (dense_f32 && (dn_rows <= DN_MAX_TOK || (d->N <= BM && dn_rows <= 2 * DN_MAX_TOK))) {
+  if (d->epi == EPI_F32 && (dn_rows <= DN_MAX_TOK || (d->N <= BM && dn_rows <= 2 * DN_MAX_TOK))) {
     DenseParams dp;
     std::memset(&dp, 0, sizeof(dp));
     dp.out = (float*)d->out[0]; dp.ldc = d->ldc; dp.S = d->total_rows; dp.N = d->N;
@@ -625,16 +642,36 @@ int mep_gemm_launch(const GemmDesc* d, cudaStream_t stream) {
   return fail(-7, "gemm: unknown epilogue %d", d->epi);
 }
 
-int mep_mx_desc_bytes() { return (int)sizeof(MxDesc); }
+int mep_mx_dgrad_desc_bytes() { return (int)sizeof(MxDgradDesc); }
 
-// Rows of `bytes` bytes of out [rows] from *rows_ptr on become zeros.
-int mep_mx_zero_tail(void* out, int rows, int64_t bytes, const int32_t* rows_ptr, cudaStream_t stream) {
-  if (rows < 0 || bytes < 0 || bytes % 16 != 0 || ((uintptr_t)out & 15) != 0) return fail(-1, "mx zero: %d rows", rows);
-  if (rows == 0 || bytes == 0) return 0;
-  ep_mx_zero_tail_kernel<<<148, 256, 0, stream>>>((uint8_t*)out, rows, bytes, rows_ptr);
-  MEP_CUDA_OK(cudaGetLastError());
-  return 0;
+int mep_mx_dgrad_launch(const MxDgradDesc* d, cudaStream_t stream) {
+  if (d->ngroups < 1 || d->ngroups > MAX_GROUPS) return fail(-1, "mx dgrad: ngroups=%d out of range", d->ngroups);
+  if (d->rows < 0 || d->K < 1 || d->N < 1 || d->w_rows < 1 || d->nseg < 1 || d->nseg > 2 || d->K > 0x7F000000 || d->rows > 0x7F000000 ||
+      (int64_t)d->ngroups * d->w_rows > 0x7F000000)
+    return fail(-2, "mx dgrad: %d x %d x %d with %d groups", d->rows, d->K, d->N, d->ngroups);
+  if (d->rows == 0) return 0;
+  MxDgradParams p;
+  std::memset(&p, 0, sizeof(p));
+  int rc = 0;
+  for (int s = 0; s < d->nseg; ++s)
+    for (int b = 0; b < TG_BOXES; ++b)
+      if ((rc = make_map(&p.tok[s][b], d->a[s], d->rows, d->K, d->lda, BK, 32 * (b + 1)))) return rc;
+  const int64_t bytes = (int64_t)((d->N + MX_BLOCK - 1) / MX_BLOCK) * (MX_BLOCK / 2);
+  if ((rc = make_byte_map(&p.codes, d->w_codes, (int64_t)d->ngroups * d->w_rows, bytes, -16))) return rc;
+  p.row_atoms = mx_atoms(d->w_rows);
+  if ((rc = make_byte_map(&p.scales, d->w_scales, (int64_t)d->ngroups * p.row_atoms, (int64_t)mx_atoms(d->N) * MX_ATOM_BYTES, 0,
+                          MX_ATOM_BYTES / 4))) return rc;
+  p.cu_seqlens = d->cu_seqlens; p.pads = d->pads; p.ngroups = d->ngroups;
+  p.total_rows = d->rows; p.N = d->N; p.K = d->K; p.nseg = d->nseg; p.w_rows = d->w_rows;
+  p.out = d->out; p.ldc = d->ldc; p.vec_out = d->ldc % 8 == 0 && ((uintptr_t)d->out & 15) == 0;
+  p.status = d->status;
+  p.timeout_ns = (unsigned long long)(d->timeout_ns > 0 ? d->timeout_ns : 2000000000ll);
+  static PairLaunch once[2];
+  const void* kern = d->fp32 ? (const void*)ep_mx_dgrad_kernel<true> : (const void*)ep_mx_dgrad_kernel<false>;
+  return launch_pair(kern, once[d->fp32 ? 1 : 0], p, device_sms(), MXD_THREADS, MXD_SMEM, false, stream, true);
 }
+
+int mep_mx_desc_bytes() { return (int)sizeof(MxDesc); }
 
 // sum[r] = parts[0][r] + parts[1][r] + ..., zero for the rows behind *rows_ptr.
 int mep_mx_sum_parts(const float* parts, int n, int rows, const int32_t* rows_ptr, float* sum, cudaStream_t stream) {

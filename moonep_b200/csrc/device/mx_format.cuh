@@ -59,14 +59,14 @@ __device__ __forceinline__ uint32_t mx_codes(const float* x) {
 __device__ __forceinline__ float mx_element(uint32_t code) {
   return __uint_as_float(((code & 8u) << 28) | ((code & 7u) << 22)) * 0x1p126f;
 }
-// Four codes (the low 16 bits) as bf16, two a word: the magnitudes' bytes are looked up by byte permutations, then the
-// signs set.
+// Four codes (the low 16 bits) as bf16, two a word: the magnitudes' bytes are looked up by byte permutations; a product
+// moves the two signs of a word to bits 15 and 31.
 __device__ __forceinline__ uint2 mx_bf16x4(uint32_t codes) {
   const uint32_t sel = codes & 0x7777u;
   const uint32_t high = __byte_perm(0x3F3F3F00u, 0x40404040u, sel), low = __byte_perm(0xC0800000u, 0xC0804000u, sel);
   uint2 r;
-  r.x = __byte_perm(low, high, 0x5140) | (codes << 12 & 0x8000u) | (codes << 24 & 0x80000000u);
-  r.y = __byte_perm(low, high, 0x7362) | (codes << 4 & 0x8000u) | (codes << 16 & 0x80000000u);
+  r.x = __byte_perm(low, high, 0x5140) | ((codes & 0x88u) * 0x01001000u & 0x80008000u);
+  r.y = __byte_perm(low, high, 0x7362) | ((codes & 0x8800u) * 0x00010010u & 0x80008000u);
   return r;
 }
 

@@ -612,12 +612,4 @@ __global__ void __launch_bounds__(256) ep_mx_sum_parts_kernel(const float* __res
   sum[r] = s;
 }
 
-// Rows of `bytes` bytes (a multiple of 16) from *rows_ptr on become zeros.
-__global__ void __launch_bounds__(256) ep_mx_zero_tail_kernel(uint8_t* __restrict__ out, int rows, long long bytes,
-                                                              const int32_t* __restrict__ rows_ptr) {
-  const long long from = (long long)max(0, min(*rows_ptr, rows)) * bytes, to = rows * bytes, step = (long long)gridDim.x * 256 * 16;
-  for (long long i = from + ((long long)blockIdx.x * 256 + threadIdx.x) * 16; i < to; i += step)
-    *reinterpret_cast<uint4*>(out + i) = make_uint4(0, 0, 0, 0);
-}
-
 }  // namespace mep

@@ -174,12 +174,10 @@ class _MoEFn(torch.autograd.Function):
         buf: Buffer = layer.buf
         pools = layer.pools
         x, hidden, w_nvs, cu, act, gate, up, topk, w = ctx.saved_tensors
-        w_gate, w_up, w_down = layer.w_gate, layer.w_up, layer.w_down
         packed = getattr(ctx, "packed", None)
-        if packed is not None:      # straight through the quantisation: the products' own operands, in bf16
+        if packed is not None:      # straight through the quantisation: the products' own operands
             xq, act, wgu, wd = packed
             hidden, act = xq.dequantize(rows_ptr=cu[-1:]), act.dequantize(rows_ptr=cu[-1:])
-            w_down = wd.dequantize()
         have_slots = split is not None
         slot = (lambda n: pools.slot(n)) if have_slots else (lambda n: None)
         gslot = (lambda n: pools.grad_slot(n)) if have_slots else (lambda n: None)
@@ -205,9 +203,11 @@ class _MoEFn(torch.autograd.Function):
             with tr.span("b.reprefetch"):
                 ev_p = layer.prefetch(plan)
         with tr.span("b.down_dgrad"):
-            if ev_p is None:
-                d_act = gemm.down_dgrad(d_out, w_down, cu, wd_slot=slot("down"), split=split, dispatch=disp,
-                                        pads=pads, fp32=packed is not None)
+            if packed is not None:
+                d_act = mx.down_dgrad(d_out[:xq.shape[0]], wd, cu, pads=pads, fp32=True)
+            elif ev_p is None:
+                d_act = gemm.down_dgrad(d_out, layer.w_down, cu, wd_slot=slot("down"), split=split, dispatch=disp,
+                                        pads=pads)
             else:      # local experts first, next to the copy kernel; the slot groups once it is done
                 d_act = gemm.down_dgrad(d_out, layer.w_down, cu[:buf.epn], grid=layer.overlap_grid(),
                                         dispatch=disp, pads=pads)
@@ -241,7 +241,6 @@ class _MoEFn(torch.autograd.Function):
         with tr.span("b.swiglu_bwd"):
             if packed is not None:
                 d_gate, d_up, d_scale = mx.gateup_swiglu_bwd(d_act, xq, wgu, cu, row_scale=w_nvs, want_dscale=True, pads=pads)
-                w_gate, w_up = wgu.dequantize()
             else:
                 d_gate, d_up, d_scale = ew.swiglu_bwd(d_act, gate, up, w_nvs, rows_ptr=cu[-1:])
         ev_r = None
@@ -266,19 +265,21 @@ class _MoEFn(torch.autograd.Function):
                                            zero_consumed=zc)
         grid = layer.overlap_grid() if ev_r is not None else 0
         # dispatch backward = combine; the scalar path returns d(route weights) as [S, K]
-        if layer.fused_combine:
+        if layer.fused_combine and packed is None:
             with tr.span("b.gateup_dgrad_push"):
-                gemm.gateup_dgrad(d_gate, d_up, w_gate, w_up, cu, wg_slot=slot("gate"),
+                gemm.gateup_dgrad(d_gate, d_up, layer.w_gate, layer.w_up, cu, wg_slot=slot("gate"),
                                   wu_slot=slot("up"), split=split, push=buf.push_target(plan), grid=grid,
-                                  pads=pads, transposed=packed is not None)
+                                  pads=pads)
             ev_r = _MoEFn._late_wgrads(layer, plan, hidden, d_gate, d_up, cu, gslot, split, ev_r, do_reduce, sgd)
             with tr.span("b.combine_pushed"):
                 dx, dw_sk = buf.combine_pushed(plan, d_scale)
         else:
             shard = buf.hidden_nvsh_buffer_view
-            gemm.gateup_dgrad(d_gate, d_up, w_gate, w_up, cu, wg_slot=slot("gate"),
-                              wu_slot=slot("up"), split=split, out=shard, grid=grid, pads=pads,
-                              transposed=packed is not None)
+            if packed is not None:
+                mx.gateup_dgrad(d_gate, d_up, wgu, cu, pads=pads, out=shard)
+            else:
+                gemm.gateup_dgrad(d_gate, d_up, layer.w_gate, layer.w_up, cu, wg_slot=slot("gate"),
+                                  wu_slot=slot("up"), split=split, out=shard, grid=grid, pads=pads)
             ev_r = _MoEFn._late_wgrads(layer, plan, hidden, d_gate, d_up, cu, gslot, split, ev_r, do_reduce, sgd)
             dx, dw_sk, _ = buf.combine(plan, shard, d_scale, zero_copy=True)
         # router backward

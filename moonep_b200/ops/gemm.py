@@ -246,37 +246,31 @@ def down(act, wd, cu_seqlens, *, wd_slot=None, split=None, out=None, push=None, 
     return y
 
 
-def down_dgrad(dy, wd, cu_seqlens, *, wd_slot=None, split=None, out=None, g_begin=0, grid=0, dispatch=None, pads=None,
-               fp32=False):
+def down_dgrad(dy, wd, cu_seqlens, *, wd_slot=None, split=None, out=None, g_begin=0, grid=0, dispatch=None, pads=None):
     """``dact[rows,H'] = dy[rows,H] Wd[g]``.  ``out`` / ``g_begin`` / ``grid`` / ``dispatch`` as in
     :func:`gateup_swiglu`: the local experts and the prefetch slots may be two launches, and the
-    launch may carry the dispatch of ``dy`` itself.  ``fp32``: the sums unrounded (padding rows are left as they
-    are; not with ``dispatch``)."""
+    launch may carry the dispatch of ``dy`` itself."""
     rows, H = dy.shape
     Hp = wd.shape[2]
-    dtype = torch.float32 if fp32 else torch.bfloat16
     if out is None:
-        out = torch.empty(rows, Hp, dtype=dtype, device=dy.device)
-    assert out.dtype == dtype and not (fp32 and dispatch is not None)
-    _tokens_gemm([dy], [wd], [wd_slot], cu_seqlens, split, Hp, H, H, True, EPI_F32 if fp32 else EPI_BF16, [out], Hp,
+        out = torch.empty(rows, Hp, dtype=torch.bfloat16, device=dy.device)
+    _tokens_gemm([dy], [wd], [wd_slot], cu_seqlens, split, Hp, H, H, True, EPI_BF16, [out], Hp,
                  grid=grid, g_begin=g_begin, dispatch=dispatch, pads=pads)
     return out
 
 
 def gateup_dgrad(dg, du, wg, wu, cu_seqlens, *, wg_slot=None, wu_slot=None, split=None, out=None,
-                 push=None, grid=0, pads=None, transposed=False):
+                 push=None, grid=0, pads=None):
     """``dx[rows,H] = dg Wg[g]^T + du Wu[g]^T`` (two K segments into one accumulator); ``push`` as
-    in :func:`down`.  ``transposed``: the weights are stored ``[G, H', H]`` (:func:`.mx.pack_gate_up`'s values)."""
+    in :func:`down`."""
     rows, Hp = dg.shape
-    H = wg.shape[2 if transposed else 1]
-    assert wg.shape[1 if transposed else 2] == Hp and wu.shape == wg.shape
-    per_expert = wg.shape[1]
+    H = wg.shape[1]
     if push is not None:
-        _tokens_gemm([dg, du], [wg, wu], [wg_slot, wu_slot], cu_seqlens, split, H, Hp, per_expert, transposed,
+        _tokens_gemm([dg, du], [wg, wu], [wg_slot, wu_slot], cu_seqlens, split, H, Hp, H, False,
                      EPI_BF16, [], H, push=push, grid=grid, pads=pads)
         return None
     dx = torch.empty(rows, H, dtype=torch.bfloat16, device=dg.device) if out is None else out
-    _tokens_gemm([dg, du], [wg, wu], [wg_slot, wu_slot], cu_seqlens, split, H, Hp, per_expert, transposed,
+    _tokens_gemm([dg, du], [wg, wu], [wg_slot, wu_slot], cu_seqlens, split, H, Hp, H, False,
                  EPI_BF16, [dx], dx.stride(0), grid=grid, pads=pads)
     return dx
 

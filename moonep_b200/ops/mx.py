@@ -47,6 +47,8 @@ PHASES = 4
 # quantise: x, x2, codes, scales, rows_ptr; batch, stride; type, mats, rows, cols, along_cols, out_rows, phases, unused
 # dequantise: codes, scales, out, rows_ptr; mats, rows, cols, pair, in_rows, fp32
 _DESC = struct.Struct("@4P8i10PqPq")
+# dgrad: a[2], codes, scales, out, cu_seqlens, pads; lda, ldc; rows, K, N, nseg, groups, weight rows, fp32, unused; status, timeout
+_DGRAD = struct.Struct("@7P2q8iPq")
 _QUANT = struct.Struct("@5P2q8i")
 _DEQUANT = struct.Struct("@4P6i")
 
@@ -54,7 +56,8 @@ nat.declare("mep_mx_quant_desc_bytes", I, [])
 nat.declare("mep_mx_quantize", I, [ctypes.c_char_p, P])
 nat.declare("mep_mx_dequantize", I, [ctypes.c_char_p, P])
 nat.declare("mep_mx_desc_bytes", I, [])
-nat.declare("mep_mx_zero_tail", I, [P, I, L, P, P])
+nat.declare("mep_mx_dgrad_desc_bytes", I, [])
+nat.declare("mep_mx_dgrad_launch", I, [ctypes.c_char_p, P])
 nat.declare("mep_mx_sum_parts", I, [P, I, I, P, P, P])
 nat.declare("mep_mx_gemm_launch", I, [ctypes.c_char_p, P])
 
@@ -66,6 +69,7 @@ _checked_layout = False
 def _check_layouts() -> None:
     global _checked_layout
     assert nat.call("mep_mx_desc_bytes") == _DESC.size, "MxDesc layout mismatch"
+    assert nat.call("mep_mx_dgrad_desc_bytes") == _DGRAD.size, "MxDgradDesc layout mismatch"
     assert nat.call("mep_mx_quant_desc_bytes") == (_QUANT.size << 16 | _DEQUANT.size), "MxQuantDesc layout mismatch"
     _checked_layout = True
 
@@ -357,6 +361,51 @@ def gateup_swiglu_bwd(d_act: torch.Tensor, a: MxTensor, wgu: MxTensor, cu_seqlen
     return d_gate, d_up, d_scale
 
 
+def _dgrad(segs, w: MxTensor, cu_seqlens, pads, out: torch.Tensor) -> torch.Tensor:
+    a = segs[0]
+    index, K, N, groups = w._index, w.shape[-2], w.shape[-1], w._mats
+    assert index >= 0 and index == _device(), "the weights are not on the current device"
+    for t in segs:
+        gemm._bf16(t, "rows")
+        assert t.get_device() == index and t.dim() == 2 and t.shape == a.shape and t.stride(0) == a.stride(0)
+    assert a.shape[1] == K and K % 8 == 0, "rows must be [rows, K], K a multiple of 8"
+    assert 1 <= groups <= 1024, "1 to 1024 groups"
+    cu = pad = 0
+    if cu_seqlens is None:
+        assert groups == 1, "several groups need cu_seqlens"
+    else:
+        assert cu_seqlens.dtype is torch.int32 and cu_seqlens.get_device() == index and cu_seqlens.is_contiguous() \
+            and cu_seqlens.numel() == groups, "cu_seqlens must be int32, one entry a group"
+        cu, pad = cu_seqlens.data_ptr(), gemm._pads(pads, cu_seqlens) or 0
+    assert out.get_device() == index and out.dim() == 2 and out.shape[0] >= a.shape[0] and out.shape[1] == N and out.stride(1) == 1
+    _launch_native("mep_mx_dgrad_launch",
+                   _DGRAD.pack(a.data_ptr(), segs[-1].data_ptr(), *w._at, out.data_ptr(), cu, pad, a.stride(0), out.stride(0),
+                               a.shape[0], K, N, len(segs), groups, w._rows, out.dtype is torch.float32, 0,
+                               gemm.status_word(w.device).data_ptr(), 0), "mx dgrad")
+    return out
+
+
+def down_dgrad(dy: torch.Tensor, wd: MxTensor, cu_seqlens: Optional[torch.Tensor] = None, *, pads: Optional[torch.Tensor] = None,
+               fp32: bool = False) -> torch.Tensor:
+    """``d_act[rows,H'] = dy Wd[g]`` for bf16 ``dy`` ``[rows, H]`` and 4-bit ``wd`` ``[G, H, H']`` (or ``[H, H']``): the
+    gradient of :func:`matmul` with respect to the values of its rows.  bf16, or the ``fp32`` sums (padding rows and rows
+    of no group are undefined then; else zeros, padding and behind the last group)."""
+    assert isinstance(wd, MxTensor) and len(wd.shape) < 4, "wd must come from quantize"
+    out = torch.empty(dy.shape[0], wd.shape[-1], dtype=torch.float32 if fp32 else torch.bfloat16, device=wd.device)
+    return _dgrad((dy,), wd, cu_seqlens, pads, out)
+
+
+def gateup_dgrad(dg: torch.Tensor, du: torch.Tensor, wgu: MxTensor, cu_seqlens: Optional[torch.Tensor] = None, *,
+                 pads: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``dx[rows,H] = dg Wg[g]^T + du Wu[g]^T`` for bf16 ``dg``/``du`` ``[rows, H']`` and the packed weights of
+    :func:`gateup_swiglu`; zeros in padding rows and behind the last group.  ``out`` ``[rows or more, H]`` bf16 takes it."""
+    assert isinstance(wgu, MxTensor) and len(wgu.shape) == 4, "wgu must come from pack_gate_up"
+    if out is None:
+        out = torch.empty(dg.shape[0], wgu.shape[-1], dtype=torch.bfloat16, device=wgu.device)
+    assert out.dtype is torch.bfloat16, "dx is bf16"
+    return _dgrad((dg, du), wgu, cu_seqlens, pads, out)
+
+
 def _pack(wg, wu, wd):
     """``(wgu, wd)`` quantised: as they are if they are so already."""
     if isinstance(wg, MxTensor):
@@ -399,14 +448,10 @@ class _ExpertFFN(torch.autograd.Function):
             grads[2] = grads[2].view(ctx.shapes[1])
         dx = d_scale = None
         if need_x or need_g or need_u or need_s:
-            d_act = gemm.down_dgrad(dy, wdq.dequantize().view(G, H, Hp), cu, pads=pads, fp32=True)
+            d_act = down_dgrad(dy, wdq, cu, pads=pads, fp32=True)
             d_gate, d_up, d_scale = gateup_swiglu_bwd(d_act, xq, wgu, cu, row_scale=row_scale, want_dscale=need_s, pads=pads)
             if need_x:
-                w = wgu.dequantize()
-                dx = gemm.gateup_dgrad(d_gate, d_up, w[0], w[1], cu, pads=pads, transposed=True)
-                if cu is not None:
-                    ew._rc(nat.call("mep_mx_zero_tail", dx.data_ptr(), dx.shape[0], 2 * H, rows_ptr.data_ptr(), nat.stream()),
-                           "mx rows behind the last group")
+                dx = gateup_dgrad(d_gate, d_up, wgu, cu, pads=pads)
             if need_g or need_u:
                 out = torch.empty(2, G, H, Hp, **bf16)
                 gemm.wgrad2(xq.dequantize(rows_ptr=rows_ptr), (d_gate, d_up), cu, (out[0], out[1]), pads=pads)

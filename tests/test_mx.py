@@ -365,26 +365,72 @@ def test_gateup_backward_padding_rows():
     assert (padded[2][384:] == 0).all()
 
 
-# ---- the bf16 products that the FFN's backward pass needs ------------------------------------------
+@gpu
+@pytest.mark.parametrize("H,Hp", [(256, 256), (64, 8), (1000, 515), (2048, 640), (8, 1)])
+@pytest.mark.parametrize("sizes", GROUPS)
+def test_dgrads(sizes, H, Hp):
+    """bf16 rows times the values of quantised weights, along their scales: K sums in fp32, in bf16 half a step more."""
+    from moonep_b200.ops import mx
+    gen = _gen(23)
+    rows, G = sum(sizes), len(sizes)
+    ends = _ends(sizes)
+    dy = torch.randn(rows, H, generator=gen).bfloat16()
+    wd = _spread(gen, G, H, Hp).bfloat16() if H < 1000 else torch.randn(G, H, Hp, generator=gen).bfloat16()
+    q = mx.quantize(wd.cuda())
+    ref, mag = ox.product(dy.double(), ox.quantise(wd).transpose(1, 2), ends.tolist())
+    slack = (H + 2) * 2.0 ** -24 * mag
+    got = mx.down_dgrad(dy.cuda(), q, ends.cuda(), fp32=True)
+    assert got.dtype == torch.float32 and float(((got.cpu().double() - ref).abs() - slack).max()) <= 0
+    got = mx.down_dgrad(dy.cuda(), q, ends.cuda())
+    assert float(((got.cpu().double() - ref).abs() - slack - HALF * ref.abs()).max()) <= 0
+    if Hp % 8:
+        return
+    wg, wu = (torch.randn(G, H, Hp, generator=gen).bfloat16() for _ in range(2))
+    dg, du = (torch.randn(rows, Hp, generator=gen).bfloat16() for _ in range(2))
+    gv, uv = (ox.quantise(w.transpose(1, 2).contiguous()) for w in (wg, wu))        # [G, H', H]
+    got = mx.gateup_dgrad(dg.cuda(), du.cuda(), mx.pack_gate_up(wg.cuda(), wu.cuda()), ends.cuda())
+    (a, am), (b, bm) = (ox.product(d.double(), v.transpose(1, 2), ends.tolist()) for d, v in ((dg, gv), (du, uv)))
+    assert float(((got.cpu().double() - a - b).abs() - (2 * Hp + 2) * 2.0 ** -24 * (am + bm) - HALF * (a + b).abs()).max()) <= 0
+
+
+@gpu
+def test_dgrad_padding_and_other_rows():
+    from moonep_b200.ops import mx
+    gen = _gen(24)
+    H, Hp, ends = 256, 160, _ends([128, 64, 0, 192]).cuda()
+    pads = torch.tensor([[100, 28], [129, 63], [192, 0], [192, 0]], dtype=torch.int32).cuda()
+    dg, du = (torch.randn(384 + 40, Hp, generator=gen).bfloat16().cuda() for _ in range(2))
+    w = mx.pack_gate_up(*((torch.randn(4, H, Hp, generator=gen) * H ** -0.5).bfloat16().cuda() for _ in range(2)))
+    plain = mx.gateup_dgrad(dg, du, w, ends)
+    assert (plain[384:] == 0).all() and float(plain[:384].float().abs().min(1).values.max()) > 0
+    for d in (dg, du):
+        d[100:128], d[129:192] = 0, 0
+    want = mx.gateup_dgrad(dg, du, w, ends)
+    for d in (dg, du):
+        d[100:128], d[160:192], d[384:] = 0, float("nan"), float("nan")     # (a tile's own 32 rows are read)
+    out = torch.full((430, H), 7.0, device="cuda", dtype=torch.bfloat16)
+    got = mx.gateup_dgrad(dg, du, w, ends, pads=pads, out=out)
+    assert got.data_ptr() == out.data_ptr() and torch.equal(out[:424], want) and (out[424:] == 7).all()
+    # a NaN block of the weights reaches its columns' rows only
+    wd = torch.randn(2, 64, 96, generator=gen)
+    wd[1, 5, 40] = float("nan")
+    y = mx.down_dgrad(dg[:100, :64].contiguous(), mx.quantize(wd.cuda()), _ends([50, 50]).cuda())
+    bad = torch.zeros_like(y, dtype=torch.bool)
+    bad[50:, 32:64] = True
+    assert torch.equal(y.isnan(), bad)
+
+
 @gpu
 @pytest.mark.parametrize("G,H,Hp", [(3, 256, 72), (2, 384, 256), (1, 128, 8)])
-def test_bf16_products_of_the_backward_pass(G, H, Hp):
+def test_weight_grads_in_bf16(G, H, Hp):
+    """The fp32 grads rounded; those of empty groups zero."""
     from moonep_b200.ops import gemm
     gen = _gen(19)
     sizes = [64, 0, 192][:G] if G > 1 else [100]
-    ends, rows = _ends(sizes), sum(sizes)
-    dy, wd = torch.randn(rows, H, generator=gen).bfloat16(), torch.randn(G, H, Hp, generator=gen).bfloat16()
-    cu = None if G == 1 else ends.cuda()
-    got = gemm.down_dgrad(dy.cuda(), wd.cuda(), cu, fp32=True)
-    ref, mag = ox.product(dy.double(), wd.double().transpose(1, 2), ends.tolist())
-    assert got.dtype == torch.float32 and float(((got.cpu().double() - ref).abs() - (H + 2) * 2.0 ** -24 * mag).max()) <= 0
-    # gate and up weights stored [G, H', H]
+    rows = sum(sizes)
+    a = torch.randn(rows, H, generator=gen).bfloat16().cuda()
+    cu = None if G == 1 else _ends(sizes).cuda()
     d1, d2 = (torch.randn(rows, Hp, generator=gen).bfloat16().cuda() for _ in range(2))
-    w1, w2 = (torch.randn(G, H, Hp, generator=gen).bfloat16().cuda() for _ in range(2))
-    t = [w.transpose(1, 2).contiguous() for w in (w1, w2)]
-    assert torch.equal(gemm.gateup_dgrad(d1, d2, *t, cu, transposed=True), gemm.gateup_dgrad(d1, d2, w1, w2, cu))
-    # grads in bf16 are the fp32 ones rounded, those of empty groups zero
-    a = dy.cuda()
     f32 = [torch.empty(G, H, Hp, device="cuda") for _ in range(3)]
     b16 = [torch.full((G, H, Hp), 7.0, device="cuda", dtype=torch.bfloat16) for _ in range(3)]
     for out in (f32, b16):
@@ -622,6 +668,13 @@ def test_refusals():
         lambda: mx.gateup_swiglu(q, qw, ends),
         lambda: mx.gateup_swiglu(q, gu, ends, row_scale=torch.ones(7, device="cuda")),
         lambda: mx.gateup_swiglu(q, gu, ends, row_scale=torch.ones(8, **bf)),
+        lambda: mx.down_dgrad(x, gu, ends),
+        lambda: mx.down_dgrad(x.float(), mx.quantize(torch.randn(2, 64, 32, **bf)), ends),
+        lambda: mx.down_dgrad(x[:, :32].contiguous(), mx.quantize(torch.randn(2, 64, 32, **bf)), ends),
+        lambda: mx.down_dgrad(x, mx.quantize(torch.randn(2, 64, 32, **bf))),
+        lambda: mx.gateup_dgrad(x[:, :32].contiguous(), x[:4, :32].contiguous(), gu, ends),
+        lambda: mx.gateup_dgrad(x, x, gu, ends),
+        lambda: mx.gateup_dgrad(x, x, qw, ends),
         lambda: mx.gateup_swiglu_bwd(torch.zeros(8, 32, **bf), q, gu, ends),
         lambda: mx.gateup_swiglu_bwd(torch.zeros(7, 32, device="cuda"), q, gu, ends),
         lambda: mx.gateup_swiglu_bwd(torch.zeros(8, 32, device="cuda"), q, qw, ends),
