@@ -163,8 +163,7 @@ class _MoEFn(torch.autograd.Function):
         y, _, _ = buf.combine(plan, shard, None, zero_copy=True)
         ctx.layer, ctx.plan, ctx.split = layer, plan, None
         if keep:
-            ctx.packed = xq, act, wgu, wd
-        ctx.save_for_backward(x, None, w_nvs, cu, None, None, None, topk, w)
+            mx.save_operands(ctx, (xq, act, wgu, wd), x, None, w_nvs, cu, None, None, None, topk, w)
         layer.last_plan = plan
         return y
 
@@ -173,8 +172,8 @@ class _MoEFn(torch.autograd.Function):
         layer, plan, split = ctx.layer, ctx.plan, ctx.split
         buf: Buffer = layer.buf
         pools = layer.pools
-        x, hidden, w_nvs, cu, act, gate, up, topk, w = ctx.saved_tensors
-        packed = getattr(ctx, "packed", None)
+        packed, saved = mx.saved_operands(ctx) if hasattr(ctx, "mx_rest") else (None, ctx.saved_tensors)
+        x, hidden, w_nvs, cu, act, gate, up, topk, w = saved
         if packed is not None:      # straight through the quantisation: the products' own operands
             xq, act, wgu, wd = packed
             hidden, act = xq.dequantize(rows_ptr=cu[-1:]), act.dequantize(rows_ptr=cu[-1:])

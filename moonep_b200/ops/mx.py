@@ -144,6 +144,27 @@ class MxTensor:
         self.shape, self._index, self._mats, self._rows, self._at = shape, index, mats, rows, (at, at + n)
         return self
 
+    def _saved(self):
+        """``(tensors, rest)`` to save and to make it again from, for autograd's saved tensors: they are then freed, or moved
+        by hooks, as others are."""
+        own = self._data.dim() == 1
+        tensors = (self._data,) if own else (self._codes, self._scales)
+        return tensors, (self.shape, self._mats, self._rows, self._at[1] - self._at[0] if own else None)
+
+    @classmethod
+    def _again(cls, tensors, rest) -> "MxTensor":
+        self = cls.__new__(cls)
+        self.shape, self._mats, self._rows, scales_at = rest
+        self._data = data = tensors[0]
+        self._index, at = data.get_device(), data.data_ptr()
+        if scales_at is None:
+            self._codes, self._scales = tensors
+            self._at = at, tensors[1].data_ptr()
+        else:
+            self._codes = self._scales = None
+            self._at = at, at + scales_at
+        return self
+
     def _views(self):
         if self._codes is None:
             codes, scales = _sizes(self.shape)
@@ -293,8 +314,8 @@ def matmul(a: MxTensor, w: MxTensor, cu_seqlens: Optional[torch.Tensor] = None, 
     ``[G]``, or ``[N, K]`` for all rows.
 
     ``out`` ``[rows or more, N]`` (bf16, dense rows) takes the result; rows that belong to no group are left as they
-    are, or with ``zero_tail`` become zeros where they are behind the last group.  ``pads`` (a plan's ``zero_fill_ranges``): which rows of the groups are padding; they become zeros without
-    being computed."""
+    are, or with ``zero_tail`` become zeros where they are behind the last group.  ``pads`` (a plan's
+    ``zero_fill_ranges``): which rows of the groups are padding; they become zeros without being computed."""
     assert isinstance(a, MxTensor) and isinstance(w, MxTensor) and len(w.shape) < 4, "operands must be quantised"
     assert len(a.shape) == 2, "the rows' operand is one matrix"
     rows, N = a.shape[0], w.shape[-2]
@@ -377,7 +398,9 @@ def _dgrad(segs, w: MxTensor, cu_seqlens, pads, out: torch.Tensor) -> torch.Tens
         assert cu_seqlens.dtype is torch.int32 and cu_seqlens.get_device() == index and cu_seqlens.is_contiguous() \
             and cu_seqlens.numel() == groups, "cu_seqlens must be int32, one entry a group"
         cu, pad = cu_seqlens.data_ptr(), gemm._pads(pads, cu_seqlens) or 0
+        assert pads is None or pads.get_device() == index
     assert out.get_device() == index and out.dim() == 2 and out.shape[0] >= a.shape[0] and out.shape[1] == N and out.stride(1) == 1
+    assert out.shape[0] < 2 or out.stride(0) >= N, "rows of out overlap"
     _launch_native("mep_mx_dgrad_launch",
                    _DGRAD.pack(a.data_ptr(), segs[-1].data_ptr(), *w._at, out.data_ptr(), cu, pad, a.stride(0), out.stride(0),
                                a.shape[0], K, N, len(segs), groups, w._rows, out.dtype is torch.float32, 0,
@@ -406,6 +429,22 @@ def gateup_dgrad(dg: torch.Tensor, du: torch.Tensor, wgu: MxTensor, cu_seqlens: 
     return _dgrad((dg, du), wgu, cu_seqlens, pads, out)
 
 
+def save_operands(ctx, operands, *tensors) -> None:
+    """``ctx.save_for_backward`` of operands and tensors (or ``None``)."""
+    saved = [q._saved() for q in operands]
+    ctx.mx_rest = [(len(t), rest) for t, rest in saved]
+    ctx.save_for_backward(*(x for t, _ in saved for x in t), *tensors)
+
+
+def saved_operands(ctx):
+    """``(operands, tensors)`` saved by :func:`save_operands`."""
+    tensors, at, operands = ctx.saved_tensors, 0, []
+    for n, rest in ctx.mx_rest:
+        operands.append(MxTensor._again(tensors[at:at + n], rest))
+        at += n
+    return operands, tensors[at:]
+
+
 def _pack(wg, wu, wd):
     """``(wgu, wd)`` quantised: as they are if they are so already."""
     if isinstance(wg, MxTensor):
@@ -426,15 +465,14 @@ class _ExpertFFN(torch.autograd.Function):
         _launch(act, wdq, H, 0, cu_seqlens, pads, None, y.data_ptr(), 0, 0, 0, 0, H, zero_tail=1,
                 check_groups=int(any(ctx.needs_input_grad[1:4])))
         if keep:
-            ctx.packed, ctx.shapes = (xq, act, wgu, wdq), None if isinstance(wg, MxTensor) else (wg.shape, wd.shape)
-            ctx.save_for_backward(row_scale, cu_seqlens, pads)
+            ctx.shapes = None if isinstance(wg, MxTensor) else (wg.shape, wd.shape)
+            save_operands(ctx, (xq, act, wgu, wdq), row_scale, cu_seqlens, pads)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        xq, act, wgu, wdq = ctx.packed
-        row_scale, cu, pads = ctx.saved_tensors
+        (xq, act, wgu, wdq), (row_scale, cu, pads) = saved_operands(ctx)
         need_x, need_g, need_u, need_d, need_s = ctx.needs_input_grad[:5]
         dy = dy.contiguous()
         if dy.data_ptr() % 16 != 0:
@@ -442,6 +480,10 @@ class _ExpertFFN(torch.autograd.Function):
         (G, Hp, H), rows_ptr = wgu.shape[1:], None if cu is None else cu[-1:]
         bf16 = dict(dtype=torch.bfloat16, device=dy.device)
         grads = [None] * 3
+        if dy.shape[0] == 0:
+            zeros = lambda need, i: torch.zeros(ctx.shapes[i], **bf16) if need else None
+            return (torch.empty_like(dy) if need_x else None, zeros(need_g, 0), zeros(need_u, 0), zeros(need_d, 1),
+                    torch.empty_like(row_scale) if need_s else None, None, None)
         if need_d:
             grads[2] = torch.empty(G, H, Hp, **bf16)
             gemm.wgrad(dy, act.dequantize(rows_ptr=rows_ptr), cu, grads[2], pads=pads)

@@ -596,6 +596,49 @@ def test_expert_ffn_some_gradients_only():
 
 
 @gpu
+def test_expert_ffn_of_no_rows():
+    from moonep_b200.ops import mx
+    bf = dict(device="cuda", dtype=torch.bfloat16)
+    x, w = torch.empty(0, 128, **bf).requires_grad_(True), [torch.randn(2, 128, 64, **bf).requires_grad_(True) for _ in range(3)]
+    s = torch.empty(0, device="cuda").requires_grad_(True)
+    y = mx.expert_ffn(x, *w, torch.zeros(2, dtype=torch.int32, device="cuda"), row_scale=s)
+    grads = torch.autograd.grad(y, (x, *w, s), torch.empty(0, 128, **bf))
+    assert y.shape == (0, 128) and [g.shape for g in grads] == [t.shape for t in (x, *w, s)]
+    assert all((g == 0).all() for g in grads)
+    # rows, but no group has any
+    x = torch.randn(64, 128, **bf).requires_grad_(True)
+    y = mx.expert_ffn(x, *w, torch.zeros(2, dtype=torch.int32, device="cuda"))
+    grads = torch.autograd.grad(y, (x, *w), torch.ones(64, 128, **bf))
+    assert (y == 0).all() and all((g == 0).all() for g in grads)
+
+
+@gpu
+def test_expert_ffn_saved_operands():
+    """They go through hooks, are kept for a second backward pass on request and freed without."""
+    from moonep_b200.ops import mx
+    gen = _gen(25)
+    H, Hp, rows = 256, 128, 192
+    x, dy = (torch.randn(rows, H, generator=gen).bfloat16().cuda() for _ in range(2))
+    ws = [(torch.randn(H, Hp, generator=gen) * 0.1).bfloat16().cuda().requires_grad_(True) for _ in range(3)]
+    want = torch.autograd.grad(mx.expert_ffn(x, *ws), ws, dy)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda()):
+        y = mx.expert_ffn(x, *ws)
+    for a, b in zip(torch.autograd.grad(y, ws, dy), want):
+        assert torch.equal(a, b)
+    y = mx.expert_ffn(x, *ws)
+    for keep in (True, False):
+        for a, b in zip(torch.autograd.grad(y, ws, dy, retain_graph=keep), want):
+            assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, ws, dy)
+    frozen = mx.pack_gate_up(*ws[:2])
+    frozen = mx.MxTensor(frozen.codes.clone(), frozen.scales.clone(), frozen.shape), None, mx.quantize(ws[2])
+    xs = x.clone().requires_grad_(True)
+    g, = torch.autograd.grad(mx.expert_ffn(xs, *frozen), xs, dy)
+    assert torch.equal(g, torch.autograd.grad(mx.expert_ffn(xs, *ws), xs, dy)[0])
+
+
+@gpu
 def test_expert_ffn_captured():
     """One token, and a training step, captured and replayed on new inputs."""
     from moonep_b200.ops import mx
