@@ -741,3 +741,85 @@ def test_refusals_without_a_gpu():
         mx.pack_gate_up(torch.randn(1, 4, 32), torch.randn(1, 4, 32))
     with pytest.raises(AssertionError):
         mx.MxTensor(torch.zeros(4, 16, dtype=torch.uint8), torch.zeros(1, 1, 512, dtype=torch.uint8), (4, 32))
+
+
+# ---- sizes and use beside one another ------------------------------------------------------------
+@gpu
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements in what is quantised, read back, and written by each product; the far ends are compared."""
+    from moonep_b200.ops import mx
+    gen = torch.Generator(device="cuda").manual_seed(26)
+    bf = dict(device="cuda", dtype=torch.bfloat16)
+    w = torch.empty(1100, 2048, 1024, **bf)
+    assert w.numel() > 2 ** 31
+    w[:-1] = 1.0
+    w[-1] = torch.randn(2048, 1024, device="cuda", generator=gen)
+    for axis in (-1, -2):
+        v = mx.quantize(w, axis).dequantize()[-1].clone()
+        assert torch.equal(v, mx.quantize(w[-1], axis).dequantize())
+    del w, v
+    rows, K, N = 140_000, 64, 16_384
+    assert rows * N > 2 ** 31
+    x = torch.zeros(rows, K, **bf)
+    x[-300:] = torch.randn(300, K, device="cuda", generator=gen)
+    qw = mx.quantize(torch.randn(N, K, device="cuda", generator=gen))
+    qx = mx.quantize(x)
+    last = mx.quantize(x[-300:])                  # (the same tiles: their first row is a multiple of 32 before the end)
+    y = mx.matmul(qx, qw)
+    assert torch.equal(y[-300:], mx.matmul(last, qw)) and (y[0] == 0).all()
+    del y
+    gu = mx.pack_gate_up(*(torch.randn(K, N, generator=gen, **bf) for _ in range(2)))
+    act = mx.gateup_swiglu(qx, gu, quantize=True)[0]
+    assert torch.equal(act.dequantize()[-300:], mx.gateup_swiglu(last, gu, quantize=True)[0].dequantize())
+    del act
+    d = torch.randn(K, N, device="cuda", generator=gen)
+    wd = mx.quantize(d)                           # [K, N]: rows [rows, K] times it
+    y = mx.down_dgrad(x, wd)
+    assert torch.equal(y[-300:], mx.down_dgrad(x[-300:].contiguous(), wd))
+
+
+@gpu
+def test_two_streams_at_once():
+    """Calls on two streams that share weights, and a captured one beside an eager one."""
+    from moonep_b200.ops import mx
+    gen = _gen(27)
+    H, Hp = 512, 256
+    ends = _ends([100, 60, 0, 200]).cuda()
+    packed = mx.pack_gate_up(*((torch.randn(4, H, Hp, generator=gen) * 0.05).bfloat16().cuda() for _ in range(2))), None, \
+        mx.quantize((torch.randn(4, H, Hp, generator=gen) * 0.05).bfloat16().cuda())
+    xs = [torch.randn(360, H, generator=gen).bfloat16().cuda() for _ in range(2)]
+    with torch.no_grad():
+        want = [mx.expert_ffn(x, *packed, ends) for x in xs]
+        streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+        graph, static = torch.cuda.CUDAGraph(), xs[0].clone()
+        with torch.cuda.graph(graph):
+            out = mx.expert_ffn(static, *packed, ends)
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+        for _ in range(20):
+            for s, x, g in zip(streams, xs, got):
+                with torch.cuda.stream(s):
+                    g.append(mx.expert_ffn(x, *packed, ends))
+            graph.replay()
+        torch.cuda.synchronize()
+    assert torch.equal(out, want[0])
+    for g, w in zip(got, want):
+        assert all(torch.equal(y, w) for y in g)
+
+
+@gpu
+def test_repeated_calls_give_the_same_bits():
+    from moonep_b200.ops import mx
+    gen = _gen(28)
+    H, Hp, sizes = 1024, 512, [64, 448, 0, 128, 256]
+    ends, rows = _ends(sizes).cuda(), sum(sizes)
+    leaves = [torch.randn(rows, H, generator=gen).bfloat16().cuda()] + \
+        [(torch.randn(5, H, Hp, generator=gen) * 0.05).bfloat16().cuda() for _ in range(3)] + [torch.rand(rows, generator=gen).cuda()]
+    leaves = [t.requires_grad_(True) for t in leaves]
+    dy = torch.randn(rows, H, generator=gen).bfloat16().cuda()
+    runs = []
+    for _ in range(5):
+        y = mx.expert_ffn(*leaves[:4], ends, row_scale=leaves[4])
+        runs.append((y.detach(), *torch.autograd.grad(y, leaves, dy)))
+    for r in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(r, runs[0]))
