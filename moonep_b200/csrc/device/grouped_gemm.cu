@@ -427,15 +427,11 @@ static int launch_dense_f32(const DenseParams& dp, cudaStream_t stream) {
   return 0;
 }
 
-template <int EPI, int MAX_N>
+template <int EPI>
 static int launch_mx(const MxParams& p, int grid, cudaStream_t stream) {
   static PairLaunch once;
-  return launch_pair((const void*)ep_mx_gemm_kernel<EPI, MAX_N>, once, p, grid, mxg_threads<EPI>(),
-                     mxg_stages<EPI, MAX_N>() * mxg_stage(MAX_N) + 1024, false, stream, true);
-}
-template <int EPI>
-static int launch_mx(const MxParams& p, bool few, int grid, cudaStream_t stream) {
-  return few ? launch_mx<EPI, MXG_FEW_N>(p, grid, stream) : launch_mx<EPI, MXG_MAX_N>(p, grid, stream);
+  return launch_pair((const void*)ep_mx_gemm_kernel<EPI>, once, p, grid, mxg_threads<EPI>(), mxg_stages<EPI>() * MXG_STAGE + 1024, false,
+                     stream, true);
 }
 
 template <bool A_MN, int EPI, bool DISP>
@@ -696,8 +692,7 @@ int mep_mx_gemm_launch(const MxDesc* d, cudaStream_t stream) {
   int rc = 0;
   if ((rc = make_byte_map(&p.w, d->w_codes, (int64_t)d->ngroups * d->w_rows, k_bytes, 128))) return rc;
   if ((rc = make_byte_map(&p.ws, d->w_scales, (int64_t)d->ngroups * p.w_atoms, s_bytes, 0))) return rc;
-  const bool few = d->rows <= MXG_FEW_N * (int64_t)d->ngroups;
-  for (int b = 0; b < (few ? 2 : MXG_BOXES); ++b)       // (boxes of up to half a tile's tokens)
+  for (int b = 0; b < MXG_BOXES; ++b)
     if ((rc = make_byte_map(&p.tok[b], d->a_codes, d->rows, k_bytes, mxg_box_rows(b)))) return rc;
   if ((rc = make_byte_map(&p.ts, d->a_scales, (int64_t)MX_PHASES * p.t_atoms, s_bytes, 0))) return rc;
   p.cu_seqlens = d->cu_seqlens; p.pads = d->pads; p.ngroups = d->ngroups; p.total_rows = d->rows; p.K = d->K; p.N = d->N;
@@ -713,11 +708,11 @@ int mep_mx_gemm_launch(const MxDesc* d, cudaStream_t stream) {
   p.d_act = d->d_act; p.d_scale = d->d_scale;
   if (d->d_act != nullptr) {
     if (!d->gated || p.gate == nullptr || p.up == nullptr) return fail(-3, "mx product: the backward pass writes both gradients");
-    return launch_mx<MX_EPI_SWIGLU_BWD>(p, few, sms, stream);
+    return launch_mx<MX_EPI_SWIGLU_BWD>(p, sms, stream);
   }
-  if (!d->gated) return launch_mx<MX_EPI_BF16>(p, few, sms, stream);
-  return p.gate != nullptr || p.up != nullptr ? launch_mx<MX_EPI_SWIGLU_SAVE>(p, few, sms, stream)
-                                              : launch_mx<MX_EPI_SWIGLU>(p, few, sms, stream);
+  if (!d->gated) return launch_mx<MX_EPI_BF16>(p, sms, stream);
+  return p.gate != nullptr || p.up != nullptr ? launch_mx<MX_EPI_SWIGLU_SAVE>(p, sms, stream)
+                                              : launch_mx<MX_EPI_SWIGLU>(p, sms, stream);
 }
 
 }  // extern "C"

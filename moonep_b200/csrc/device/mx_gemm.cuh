@@ -38,16 +38,15 @@ namespace mep {
 enum { MX_EPI_BF16 = 0, MX_EPI_SWIGLU = 1, MX_EPI_SWIGLU_SAVE = 2, MX_EPI_SWIGLU_BWD = 3 };
 
 constexpr int MXG_MAX_N = 224;                   // tokens of a tile, at most
-constexpr int MXG_FEW_N = 64;                    // the same where groups are short
 constexpr int MXG_BK = 256;                      // elements of a k-block: 128 bytes a row
-constexpr int MXG_MAX_STAGES = 10;
 constexpr int MXG_W_BYTES = 128 * 128;
 constexpr int MXG_S_BYTES = 2 * MX_ATOM_BYTES;   // scales of 128 rows and one k-block
 constexpr int MXG_BOXES = 5;
 __host__ __device__ constexpr int mxg_box_rows(int b) { return b == 0 ? 16 : b == 4 ? MXG_MAX_N / 2 : 32 * b; }
-// Shared memory of a stage whose tiles have up to n tokens: weights, half of the tokens (in whole swizzle atoms), scales.
-__host__ __device__ constexpr int mxg_t_bytes(int n) { return (n / 2 * 128 + 1023) & ~1023; }
-__host__ __device__ constexpr int mxg_stage(int n) { return MXG_W_BYTES + mxg_t_bytes(n) + MXG_S_BYTES * (1 + (n + 127) / 128); }
+// A stage: weights, half of the tokens (whole swizzle atoms), scales of the weights and of all tokens.
+constexpr int MXG_T_BYTES = MXG_MAX_N / 2 * 128, MXG_T_ATOMS = (MXG_MAX_N + 127) / 128;
+constexpr int MXG_STAGE = MXG_W_BYTES + MXG_T_BYTES + MXG_S_BYTES * (1 + MXG_T_ATOMS);
+static_assert(MXG_T_BYTES % 1024 == 0 && MXG_STAGE % 1024 == 0, "swizzle atoms");
 constexpr uint32_t MXG_SCALES_AT = 2 * MXG_MAX_N;
 constexpr uint32_t MXG_SCALE_COLS = 24;             // columns of tensor memory of a set: 8 of weights, 16 of tokens
 static_assert(MXG_SCALES_AT + 2 * MXG_SCALE_COLS <= 512, "tensor memory");
@@ -88,11 +87,9 @@ template <int EPI> constexpr int mxg_static_smem() {
          (EPI == MX_EPI_SWIGLU_BWD ? mxg_sets<EPI>() * 4 * TG_CHUNK * 4 : 0) + 512;
 }
 
-// Slots of the ring: as many as the device's shared memory has room for beside these.
-template <int EPI, int MAX_N> constexpr int mxg_stages() {
-  const int n = (227 * 1024 - 1024 - mxg_static_smem<EPI>()) / mxg_stage(MAX_N);
-  return n < MXG_MAX_STAGES ? n : MXG_MAX_STAGES;
-}
+// Stages: as many as the device's shared memory has room for beside these.  (Short groups do not gain from smaller stages,
+// of 64 tokens, and nine of them: 32 groups of 1 to 64 rows, 7168 -> 2 x 2048 96 - 98 us, 98 - 100; 128, 2048 -> 2 x 768 53 - 55, 51 - 55.)
+template <int EPI> constexpr int mxg_stages() { return (227 * 1024 - 1024 - mxg_static_smem<EPI>()) / MXG_STAGE; }
 
 struct MxTile {
   int g, row0, n;          // first row (a multiple of 32), tokens computed (a multiple of 32)
@@ -134,11 +131,11 @@ __device__ __forceinline__ float mx_sigmoid(float x) {
   return r;
 }
 
-template <int EPI, int MAX_N>
+template <int EPI>
 __global__ void __launch_bounds__(mxg_threads<EPI>(), 1)
 ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
   constexpr int SETS = mxg_sets<EPI>();
-  constexpr int NST = mxg_stages<EPI, MAX_N>(), STAGE = mxg_stage(MAX_N), T_BYTES = mxg_t_bytes(MAX_N);
+  constexpr int NST = mxg_stages<EPI>(), STAGE = MXG_STAGE;
   constexpr bool GATED = EPI != MX_EPI_BF16, SAVE = EPI == MX_EPI_SWIGLU_SAVE, BWD = EPI == MX_EPI_SWIGLU_BWD;
   constexpr int TOK_ROW = mxg_token_row<EPI>();     // bytes of a staged token
   const int crank = (int)cluster_cta_rank();
@@ -197,7 +194,7 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
     int run = 0;
     for (int g0 = 0; g0 < p.ngroups; g0 += 32) {
       const int g = g0 + lane;
-      const int nt = g < p.ngroups ? (s_span[g] + MAX_N - 1) / MAX_N : 0;
+      const int nt = g < p.ngroups ? (s_span[g] + MXG_MAX_N - 1) / MXG_MAX_N : 0;
       int incl = nt;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -267,7 +264,7 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
         if (!ok) break;
         if (!issue) continue;
         uint8_t* sw = stages + (size_t)s * STAGE;
-        uint8_t* ss = sw + MXG_W_BYTES + T_BYTES;
+        uint8_t* ss = sw + MXG_W_BYTES + MXG_T_BYTES;
         const uint32_t bar = mapa_u32(&full[s], 0);
         if (crank == 0) mbar_expect_tx(&full[s], bytes);
         tma_load_2d_pair(sw, &p.w, kb * 128, wrow, bar);
@@ -282,7 +279,7 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
       const bool issue = elect_one();
       const uint64_t desc_w = make_smem_desc(smem_u32(stages), 16, 1024);
       const uint64_t desc_t = make_smem_desc(smem_u32(stages) + MXG_W_BYTES, 16, 1024);
-      const uint64_t desc_s = make_scale_desc(smem_u32(stages) + MXG_W_BYTES + T_BYTES);
+      const uint64_t desc_s = make_scale_desc(smem_u32(stages) + MXG_W_BYTES + MXG_T_BYTES);
       RingSlot st;
       int tile_n = 0, at = 0;
       uint32_t set = 0;
@@ -310,7 +307,7 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
             for (int j = 0; j < 2; ++j) {        // block atoms of the k-block
               tmem_cp_scales_2cta(tsa + 4 * j, ds + j * (MX_ATOM_BYTES >> 4));
 #pragma unroll
-              for (int a = 0; a < (MAX_N + 127) / 128; ++a)
+              for (int a = 0; a < MXG_T_ATOMS; ++a)
                 tmem_cp_scales_2cta(tsb + 8 * j + 4 * a, ds + (((1 + a) * MXG_S_BYTES + j * MX_ATOM_BYTES) >> 4));
             }
             // 64 elements each: two of an atom row's four scales
