@@ -7,9 +7,10 @@
 // operand of the MMA: every code's value times its scale is a bf16, exactly.  What this saves are the bf16 weights in memory,
 // two bytes an element written and read again.  Bound by the decoding, for each k-block a chain of waits, loads, arithmetic
 // and stores, whose turns three teams of four warps take (2 x 768 -> 2048 of 128 groups of 256 rows: one team 379 us, two 240,
-// three 207, and 188 with fewer instructions a code; four no less).  Against the product of bf16 weights and the time to make
-// them: 118 us, 115 + 121 (2048 -> 768); 188, 174 + 178 (2 x 768 -> 2048); 32 x 64 rows, 2 x 2048 -> 7168 386, 313 + 404; 32 x 1024
-// 1740 - 1900, 1275 + 420.  One group of 8192 rows, where a weight is decoded for each of its 32 token tiles: 155, 110 + 11.
+// three 207, and 177 with fewer instructions a code; four no less).  Against the product of bf16 weights and the time to make
+// them: 107 us, 114 + 121 (2048 -> 768); 177, 172 + 179 (2 x 768 -> 2048); 32 x 64 rows, 2 x 2048 -> 7168 355 - 390, 310 + 404;
+// 32 x 1024 1680 - 1900, 1260 - 1360 + 427.  One group of 8192 rows, where a weight is decoded for each of its 32 token tiles:
+// 143 - 169, 113 - 130 + 11.
 // A chain of slots:
 //   warp 0       TMA producer: token rows (counted on the leader's barrier, for both CTAs), codes (on this CTA's own)
 //   warp 1       MMA issuer: waits for the pair's tokens and for both CTAs' eight decoding warps
@@ -47,11 +48,38 @@ struct MxDgradParams {
   unsigned long long timeout_ns;
 };
 
-// The scale byte as bf16, twice.
-__device__ __forceinline__ __nv_bfloat162 mx_scale_bf16x2(uint32_t b) {
-  const uint32_t h = max(b << 7, 0x0040u) | ((b + 1u) >> 8 << 6);       // (0: 2^-127, a subnormal number; 255: NaN)
-  const uint32_t both = __byte_perm(h, h, 0x1010);
-  return *reinterpret_cast<const __nv_bfloat162*>(&both);
+// The values of eight codes and their scale byte, in bf16 and exactly (the smallest is 2^-128).  The conversion to fp16
+// takes two codes an instruction; its exponent and mantissa, moved down three bits, are a bf16's whose exponent lacks 112.
+// One product makes up for that and applies the scale; scales over 2^15, whose factor bf16 does not hold, take a second.
+// (Bytes looked up as in ep_mx_dequant_kernel: 186 us for 2 x 768 -> 2048, by this 177.)
+__device__ __forceinline__ uint4 mx_values8(uint32_t codes, uint32_t scale) {
+  constexpr uint32_t LACK = 112, BIG = 254 - LACK;
+  auto twice = [](uint32_t h) {
+    h = __byte_perm(h, h, 0x1010);
+    return *reinterpret_cast<const __nv_bfloat162*>(&h);
+  };
+  uint32_t w[4];
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+      : "r"(codes));
+  alignas(16) __nv_bfloat162 v[4];
+  const __nv_bfloat162 factor = twice((min(scale, BIG) + LACK) << 7);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w[i] = (w[i] & 0x80008000u) | (w[i] >> 3 & 0x0FFF0FFFu);
+    v[i] = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), factor);
+  }
+  if (scale > BIG) {
+    const __nv_bfloat162 rest = twice(scale == 255u ? 0x7FC0u : (scale - BIG + 127u) << 7);       // (255: NaN)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __hmul2(v[i], rest);
+  }
+  return *reinterpret_cast<const uint4*>(v);
 }
 
 template <bool F32>
@@ -242,13 +270,8 @@ ep_mx_dgrad_kernel(const __grid_constant__ MxDgradParams p) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {          // rows 4 (i / 2) + sub, columns 64 (i % 2) + 8 chunk
           const int j = i >> 1, b = i & 1, row = 4 * j + sub;
-          const __nv_bfloat162 s2 = mx_scale_bf16x2(sc[j] >> (16 * b + 8 * (chunk >> 2)) & 255u);
-          const uint2 lo = mx_bf16x4(code[i]), hi = mx_bf16x4(code[i] >> 16);
-          uint4 q = make_uint4(lo.x, lo.y, hi.x, hi.y);
-          __nv_bfloat162* v = reinterpret_cast<__nv_bfloat162*>(&q);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = __hmul2(v[e], s2);
-          *reinterpret_cast<uint4*>(dst + b * 8192 + j * 4 * 128 + ((chunk ^ ((16 * dw + row) & 7)) << 4)) = q;
+          const uint32_t sb = sc[j] >> (16 * b + 8 * (chunk >> 2)) & 255u;
+          *reinterpret_cast<uint4*>(dst + b * 8192 + j * 4 * 128 + ((chunk ^ ((16 * dw + row) & 7)) << 4)) = mx_values8(code[i], sb);
         }
         // (the fence has this CTA's stores in its shared memory, where its own tensor core reads them, before the arrival
         // leaves; a release at cluster scope on top took as long as all the rest)

@@ -8,6 +8,7 @@
 // atom][512]: the atoms of phase s begin at row 32 s, so that those of a tile that starts at any multiple of 32 rows
 // begin with an atom.  (Tensor memory wants them so: the MMA takes them from columns that start one.)
 #pragma once
+#include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>

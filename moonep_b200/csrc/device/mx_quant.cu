@@ -1,6 +1,6 @@
 // Quantisation into microscaled 4-bit operands (mx_format.cuh) and back.  Both directions are bandwidth kernels: one
 // pass, every element read and written once.  They are launched as programmatic dependents, as the product behind them
-// is: a chain's kernels are in place when their predecessor ends (three launches for a token: 6 us of gaps less).
+// is: a chain's kernels are in place when their predecessor ends (rows quantised and multiplied, 16 tokens: 49.7 -> 46.1 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -230,8 +230,8 @@ struct MxDequantParams {
 };
 
 // A lane takes eight values of a row, a warp MXD_DEPTH times 256.  Bound by HBM (6.0 TB/s); the values' bytes are looked
-// up, which takes half the instructions of computing them.  (Sixteen values a lane: 4.3 TB/s.)  (Exact in bf16 but for what a bf16 subnormal rounds,
-// fp32 always.)
+// up, which takes half the instructions of computing them.  (By the conversions of
+// ep_mx_dgrad_kernel: 5.8 TB/s.  Sixteen values a lane: 4.3.)
 constexpr int MXD_DEPTH = 8;
 
 template <class T, bool VEC>

@@ -192,7 +192,7 @@ class MxTensor:
         return f"MxTensor(shape={self.shape}, device={self.device})"
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16, *, rows_ptr: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """The values, bf16 (exact down to 2^-133, the last bit of its subnormals) or fp32, of this tensor's shape;
+        """The values, exactly, in bf16 or fp32, of this tensor's shape;
         gate first, then up, for a packed pair.  ``rows_ptr`` as in :func:`quantize`."""
         assert dtype is torch.bfloat16 or dtype is torch.float32, "values are bf16 or fp32"
         data, shape = self._data, self.shape

@@ -394,6 +394,19 @@ def test_dgrads(sizes, H, Hp):
 
 
 @gpu
+def test_dgrad_over_all_scales():
+    """One weight row a token, one scale a weight row, from E8M0's smallest to fp32's largest: the sums are the stored values."""
+    from moonep_b200.ops import mx
+    gen = _gen(25)
+    scale = 2.0 ** torch.arange(-130, 126, dtype=torch.float64)
+    w = ((torch.randn(256, 72, generator=gen, dtype=torch.float64).clamp(-1.9, 1.9) * scale[:, None]).float())[None]
+    q = mx.quantize(w.cuda())
+    y = mx.down_dgrad(torch.eye(256).bfloat16().cuda(), q, fp32=True)
+    want = ox.quantise(w)[0]
+    assert torch.equal(q.dequantize(torch.float32)[0].cpu().double(), want) and torch.equal(y.cpu().double(), want)
+
+
+@gpu
 def test_dgrad_padding_and_other_rows():
     from moonep_b200.ops import mx
     gen = _gen(24)
