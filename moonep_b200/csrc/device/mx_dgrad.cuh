@@ -20,6 +20,8 @@
 // Weight rows behind the reduction's end are decoded as zeros (what lies there may be a NaN).
 #pragma once
 
+#include <type_traits>
+
 #include "device/mx_format.cuh"
 
 namespace mep {
@@ -48,38 +50,38 @@ struct MxDgradParams {
   unsigned long long timeout_ns;
 };
 
-// The values of eight codes and their scale byte, in bf16 and exactly (the smallest is 2^-128).  The conversion to fp16
-// takes two codes an instruction; its exponent and mantissa, moved down three bits, are a bf16's whose exponent lacks 112.
-// One product makes up for that and applies the scale; scales over 2^15, whose factor bf16 does not hold, take a second.
-// (Bytes looked up as in ep_mx_dequant_kernel: 186 us for 2 x 768 -> 2048, by this 177.)
+// The bf16 values of eight codes with one scale, exactly (the smallest is 2^-128): word i holds those of codes i and i + 4, an
+// order that costs no more than to move bits (in the codes' own order a byte's two halves go different ways).  A code's sign and its
+// exponent and mantissa are put where bf16 has its own, by a product with two bits set; the exponent then lacks 126, 0.5 is a
+// subnormal number in either format, and one bf16 product makes up for that and applies the scale: 2^126 2^(byte - 127).  Bytes
+// from 128 on need more than bf16's exponents hold and take a second one (BIG).  The logical instructions bound the decoding
+// (half the rate of products), which is why shifts are products here.  (By conversions, two codes an instruction: 177 us for
+// 2 x 768 -> 2048; bytes looked up as in ep_mx_dequant_kernel: 186.)
+// scale: the byte, twice, in the words' halves.
+template <bool BIG>
 __device__ __forceinline__ uint4 mx_values8(uint32_t codes, uint32_t scale) {
-  constexpr uint32_t LACK = 112, BIG = 254 - LACK;
-  auto twice = [](uint32_t h) {
-    h = __byte_perm(h, h, 0x1010);
-    return *reinterpret_cast<const __nv_bfloat162*>(&h);
-  };
-  uint32_t w[4];
-  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
-      : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-      : "r"(codes));
+  auto pair = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+  constexpr uint32_t LOW = 0x000F000Fu, HIGH = 0x00F000F0u, KEEP = 0x81C081C0u;
+  const uint32_t rest = codes >> 8;
+  const uint32_t w[4] = {(codes & LOW) * 0x1040u & KEEP, (codes & HIGH) * 0x104u & KEEP, (rest & LOW) * 0x1040u & KEEP,
+                         (rest & HIGH) * 0x104u & KEEP};
   alignas(16) __nv_bfloat162 v[4];
-  const __nv_bfloat162 factor = twice((min(scale, BIG) + LACK) << 7);
+  const uint32_t b = scale & 255u;
+  const __nv_bfloat162 factor = pair(BIG ? (min(b, 128u) + 126u) * 0x00800080u : scale * 128u + 0x3F003F00u);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    w[i] = (w[i] & 0x80008000u) | (w[i] >> 3 & 0x0FFF0FFFu);
-    v[i] = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), factor);
-  }
-  if (scale > BIG) {
-    const __nv_bfloat162 rest = twice(scale == 255u ? 0x7FC0u : (scale - BIG + 127u) << 7);       // (255: NaN)
+  for (int i = 0; i < 4; ++i) v[i] = __hmul2(pair(w[i]), factor);
+  if constexpr (BIG) {
+    const __nv_bfloat162 more = pair((b == 255u ? 0x7FC0u : (max(b, 128u) - 1u) << 7) * 0x00010001u);       // (255: NaN)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = __hmul2(v[i], rest);
+    for (int i = 0; i < 4; ++i) v[i] = __hmul2(v[i], more);
   }
   return *reinterpret_cast<const uint4*>(v);
+}
+// Where the value at position i of eight stands in that order, and eight bf16 in it back in their own.
+__device__ __forceinline__ int mx_column(int i) { return (i & 1) * 4 + (i >> 1); }
+__device__ __forceinline__ uint4 mx_in_order(uint4 q) {
+  return make_uint4(__byte_perm(q.x, q.y, 0x5410), __byte_perm(q.z, q.w, 0x5410), __byte_perm(q.x, q.y, 0x7632),
+                    __byte_perm(q.z, q.w, 0x7632));
 }
 
 template <bool F32>
@@ -242,6 +244,7 @@ ep_mx_dgrad_kernel(const __grid_constant__ MxDgradParams p) {
   } else if (warp < 2 + MXD_TEAMS * MXD_DECODERS) {
     // ================= decode: 16 rows of the k-block a warp, in steps of four rows x 64 columns =================
     const int team = (warp - 2) / MXD_DECODERS, dw = (warp - 2) % MXD_DECODERS, chunk = lane & 7, sub = lane >> 3;
+    const uint32_t scale_bytes = 0x4040u + 0x0101u * (uint32_t)(chunk >> 2);
     RingSlot st, ct;
     for (int i = 0; i < team; ++i) { st.next(NST); ct.next(NC); }
     int kb = team;
@@ -267,12 +270,16 @@ ep_mx_dgrad_kernel(const __grid_constant__ MxDgradParams p) {
           for (int j = 0; j < 4; ++j)
             if (k + 4 * j + sub >= p.K) { sc[j] = 0x7F7F7F7Fu; code[2 * j] = code[2 * j + 1] = 0u; }
         }
+        auto decode = [&](auto big) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {          // rows 4 (i / 2) + sub, columns 64 (i % 2) + 8 chunk
-          const int j = i >> 1, b = i & 1, row = 4 * j + sub;
-          const uint32_t sb = sc[j] >> (16 * b + 8 * (chunk >> 2)) & 255u;
-          *reinterpret_cast<uint4*>(dst + b * 8192 + j * 4 * 128 + ((chunk ^ ((16 * dw + row) & 7)) << 4)) = mx_values8(code[i], sb);
-        }
+          for (int i = 0; i < 8; ++i) {        // rows 4 (i / 2) + sub, columns 64 (i % 2) + 8 chunk
+            const int j = i >> 1, b = i & 1, row = 4 * j + sub;
+            *reinterpret_cast<uint4*>(dst + b * 8192 + j * 4 * 128 + ((chunk ^ ((16 * dw + row) & 7)) << 4)) =
+                mx_values8<decltype(big)::value>(code[i], __byte_perm(sc[j], 0u, scale_bytes + 0x0202 * b));
+          }
+        };
+        if (((sc[0] | sc[1] | sc[2] | sc[3]) & 0x80808080u) == 0u) decode(std::false_type{});
+        else decode(std::true_type{});
         // (the fence has this CTA's stores in its shared memory, where its own tensor core reads them, before the arrival
         // leaves; a release at cluster scope on top took as long as all the rest)
         fence_proxy_async_smem();
@@ -314,7 +321,7 @@ ep_mx_dgrad_kernel(const __grid_constant__ MxDgradParams p) {
       };
       if constexpr (F32) {
         // thread = output column: a warp's 32 columns of a token leave as one 128-byte line
-        const int col = t.m0 + 128 * crank + q * 32 + lane;
+        const int col = t.m0 + 128 * crank + q * 32 + (lane & 24) + mx_column(lane & 7);
 #pragma unroll 1
         for (int c = first; c < t.n; c += step) {
           __syncwarp();
@@ -365,8 +372,8 @@ ep_mx_dgrad_kernel(const __grid_constant__ MxDgradParams p) {
           for (int i = 0; i < 4; ++i) {
             const int k = (te >> 4) + 8 * i;
             if (c + k >= t.rows || col0 >= p.N) continue;
-            store8(out + (long long)(t.row0 + c + k) * p.ldc + col0, *reinterpret_cast<const uint4*>(sb + k * TG_STAGE_ROW + f * 2),
-                   p.N - col0, vec_ok);
+            store8(out + (long long)(t.row0 + c + k) * p.ldc + col0,
+                   mx_in_order(*reinterpret_cast<const uint4*>(sb + k * TG_STAGE_ROW + f * 2)), p.N - col0, vec_ok);
           }
           epilogue_sync(set);              // every row of the set's buffer has been read: it may be filled again
         }
