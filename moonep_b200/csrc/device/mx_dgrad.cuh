@@ -5,18 +5,19 @@
 //
 // Four warps read the codes of a k-block (64 weight rows x 128 columns a CTA, 4 KB) from shared memory and write the bf16
 // operand of the MMA: every code's value times its scale is a bf16, exactly.  What this saves are the bf16 weights in memory,
-// two bytes an element written and read again.  Bound by the decoding, for each k-block a chain of waits, loads, arithmetic
-// and stores, whose turns three teams of four warps take (2 x 768 -> 2048 of 128 groups of 256 rows: one team 379 us, two 240,
-// three 207, and 177 with fewer instructions a code; four no less).  Against the product of bf16 weights and the time to make
-// them: 107 us, 114 + 121 (2048 -> 768); 177, 172 + 179 (2 x 768 -> 2048); 32 x 64 rows, 2 x 2048 -> 7168 355 - 390, 310 + 404;
-// 32 x 1024 1680 - 1900, 1260 - 1360 + 427.  One group of 8192 rows, where a weight is decoded for each of its 32 token tiles:
-// 143 - 169, 113 - 130 + 11.
+// two bytes an element written and read again.  For each k-block a chain of waits, loads, arithmetic and stores, whose turns
+// four teams of four warps take; long groups are bound by the MMAs (and the power cap), short ones by this chain.  2 x 768 ->
+// 2048 of 128 groups of 256 rows, in us: one team 379, two 240, three 207; with fewer instructions a code 166; with a warp of its own
+// for the codes, which runs ahead of the tokens' slots, 151 (two teams 164, four 150; 32 x 64 rows, 2 x 2048 -> 7168: two 322,
+// three 304 - 343, four 280 - 312).  Against the product of bf16 weights and the time to make them: 92 us, 115 + 121 (2048 -> 768);
+// 150, 174 + 178 (2 x 768 -> 2048); 280 - 312, 313 + 399 (32 x 64 rows, 2 x 2048 -> 7168); 1300 - 1740, 1260 + 420 (32 x 1024).
+// One group of 8192 rows, where a weight is decoded for each of its 32 token tiles: 113 - 171, 103 - 155 + 12 (by the clock).
 // A chain of slots:
-//   warp 0       TMA producer: token rows (counted on the leader's barrier, for both CTAs), codes (on this CTA's own)
+//   warp 0       TMA producer of the token rows (counted on the leader's barrier, for both CTAs)
 //   warp 1       MMA issuer: waits for the pair's tokens and for both CTAs' eight decoding warps
-//   warps 2..13  decode, three teams of four that take k-blocks in turn (a k-block is a chain of waits, loads, stores and a
-//                fence): 16 weight rows a warp, eight columns a lane and step
-//   warps 14..21 epilogue, two sets of four, as in ep_token_gemm_kernel
+//   warp 2       TMA producer of the codes (on this CTA's own barriers)
+//   warps 3..18  decode, four teams of four that take k-blocks in turn: 16 weight rows a warp, eight columns a lane and step
+//   warps 19..26 epilogue, two sets of four, as in ep_token_gemm_kernel
 // Weight rows behind the reduction's end are decoded as zeros (what lies there may be a NaN).
 #pragma once
 
@@ -27,11 +28,16 @@
 namespace mep {
 
 constexpr int MXD_SLOTS = 5;                          // of tokens and decoded weights
-constexpr int MXD_CODE_SLOTS = 6;
+constexpr int MXD_CODE_SLOTS = 8;
 constexpr int MXD_T_BYTES = 128 * 128, MXD_W_BYTES = BM * BK * 2;
 constexpr int MXD_CODE_BYTES = BK * BM / 2, MXD_CODE_SLOT = MXD_CODE_BYTES + MX_ATOM_BYTES;     // codes, and their atom of scales
-constexpr int MXD_DECODERS = 4, MXD_TEAMS = 3;        // warps that decode a k-block, and teams of them that take turns
-constexpr int MXD_THREADS = 64 + MXD_TEAMS * MXD_DECODERS * 32 + TG_SETS * 128;
+constexpr int MXD_DECODERS = 4, MXD_TEAMS = 4;        // warps that decode a k-block, and teams of them that take turns
+// A team waits for every MXD_TEAMS-th use of the rings, and a wait knows phases by their parity alone: a warp that waits for one
+// has to have waited for the one before, on the same barrier.  So code slots, and the barriers that free the other slots, are
+// multiples of the teams in number.
+static_assert(MXD_CODE_SLOTS % MXD_TEAMS == 0, "a code slot belongs to one team");
+constexpr int MXD_EMPTY = MXD_SLOTS * MXD_TEAMS;
+constexpr int MXD_THREADS = 96 + MXD_TEAMS * MXD_DECODERS * 32 + TG_SETS * 128;
 constexpr int MXD_SMEM = MXD_SLOTS * (MXD_T_BYTES + MXD_W_BYTES) + MXD_CODE_SLOTS * MXD_CODE_SLOT + 1024;
 
 struct MxDgradParams {
@@ -91,7 +97,7 @@ ep_mx_dgrad_kernel(const __grid_constant__ MxDgradParams p) {
   const int crank = (int)cluster_cta_rank();
   const int work_id0 = (int)(blockIdx.x >> 1), work_stride = (int)(gridDim.x >> 1);
   extern __shared__ uint8_t smem_dyn[];
-  __shared__ __align__(8) uint64_t t_full[NST], w_full[NST], empty[NST];
+  __shared__ __align__(8) uint64_t t_full[NST], w_full[NST], empty[MXD_EMPTY];   // (k-block n frees its slot at empty[n % MXD_EMPTY])
   __shared__ __align__(8) uint64_t c_full[NC], c_empty[NC];
   __shared__ __align__(8) uint64_t acc_full[2], acc_empty[2];
   __shared__ uint32_t s_tmem;
@@ -107,7 +113,8 @@ ep_mx_dgrad_kernel(const __grid_constant__ MxDgradParams p) {
   volatile int* abortp = &s_abort;
 
   if (warp == 0 && lane == 0) {
-    for (int s = 0; s < NST; ++s) { mbar_init(&t_full[s], 1); mbar_init(&w_full[s], 2 * MXD_DECODERS); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < NST; ++s) { mbar_init(&t_full[s], 1); mbar_init(&w_full[s], 2 * MXD_DECODERS); }
+    for (int s = 0; s < MXD_EMPTY; ++s) mbar_init(&empty[s], 1);
     for (int s = 0; s < NC; ++s) { mbar_init(&c_full[s], 1); mbar_init(&c_empty[s], MXD_DECODERS); }
     for (int a = 0; a < 2; ++a) { mbar_init(&acc_full[a], 1); mbar_init(&acc_empty[a], 8 * TG_SETS); }
     mbar_fence_init();
@@ -176,19 +183,41 @@ ep_mx_dgrad_kernel(const __grid_constant__ MxDgradParams p) {
   // First stored row of the 16 that hold weight rows k .. k + 15 (k a multiple of 16) of a segment.
   auto stored_row = [&](int seg, int k) { return p.nseg == 1 ? k : 2 * k + 16 * seg; };
 
+  // The barrier of the k-block a ring's turn before: the first turn waits for nothing.
+  RingSlot first_free;
+  first_free.slot = MXD_EMPTY - NST;
+
   if (warp == 0) {
-    // ================= TMA producer =================
+    // ================= TMA producer: tokens =================
     const bool issue = elect_one();
     int at = 0;
-    RingSlot st, ct;
+    RingSlot st, free = first_free;
     bool ok = true;
     for (long long id = work_id0; id < total_tiles && ok; id += work_stride) {
       const TokenTile t = get(id, at);
-      const int n = uniform(t.n), row0 = uniform(t.row0), g = uniform(t.g), m0 = uniform(t.m0);
-      const int trow = row0 + crank * (n / 2), box = (n / 2 + 31) / 32;
+      const int n = uniform(t.n), trow = uniform(t.row0) + crank * (n / 2), box = (n / 2 + 31) / 32;
       const uint32_t bytes = 2u * (uint32_t)(box * 32 * 128);
       for (int seg = 0; seg < p.nseg && ok; ++seg)
-        for (int kb = 0; kb < kb_per_seg; ++kb, st.next(NST), ct.next(NC)) {
+        for (int kb = 0; kb < kb_per_seg; ++kb, st.next(NST), free.next(MXD_EMPTY)) {
+          ok = warp_wait(&empty[free.slot], free.parity ^ 1u, 1);
+          if (!ok) break;
+          if (issue) {
+            if (crank == 0) mbar_expect_tx(&t_full[st.slot], bytes);
+            tma_load_2d_pair(t_slots + st.slot * MXD_T_BYTES, &p.tok[seg][box - 1], kb * BK, trow, mapa_u32(&t_full[st.slot], 0));
+          }
+        }
+    }
+  } else if (warp == 2) {
+    // ================= TMA producer: codes =================
+    const bool issue = elect_one();
+    int at = 0;
+    RingSlot ct;
+    bool ok = true;
+    for (long long id = work_id0; id < total_tiles && ok; id += work_stride) {
+      const TokenTile t = get(id, at);
+      const int g = uniform(t.g), m0 = uniform(t.m0);
+      for (int seg = 0; seg < p.nseg && ok; ++seg)
+        for (int kb = 0; kb < kb_per_seg; ++kb, ct.next(NC)) {
           ok = warp_wait(&c_empty[ct.slot], ct.parity ^ 1u, 5);
           if (!ok) break;
           if (issue) {
@@ -201,12 +230,6 @@ ep_mx_dgrad_kernel(const __grid_constant__ MxDgradParams p) {
             tma_load_2d(dst + MXD_CODE_BYTES, &p.scales, (m0 / 128 + crank) * 128, g * p.row_atoms + (stored_row(seg, kb * BK) >> 7),
                         &c_full[ct.slot]);
           }
-          ok = warp_wait(&empty[st.slot], st.parity ^ 1u, 1);
-          if (!ok) break;
-          if (issue) {
-            if (crank == 0) mbar_expect_tx(&t_full[st.slot], bytes);
-            tma_load_2d_pair(t_slots + st.slot * MXD_T_BYTES, &p.tok[seg][box - 1], kb * BK, trow, mapa_u32(&t_full[st.slot], 0));
-          }
         }
     }
   } else if (warp == 1) {
@@ -215,7 +238,7 @@ ep_mx_dgrad_kernel(const __grid_constant__ MxDgradParams p) {
       const bool issue = elect_one();
       const uint64_t desc_w = make_smem_desc(smem_u32(w_slots), 8192, 1024), desc_t = make_smem_desc(smem_u32(t_slots), 16, 1024);
       RingSlot st;
-      int tile_n = 0, at = 0;
+      int used = 0, tile_n = 0, at = 0;
       bool ok = true;
       for (long long id = work_id0; id < total_tiles && ok; id += work_stride, ++tile_n) {
         const uint32_t idesc = make_instr_desc_bf16(256, uniform(get(id, at).n), true, false);
@@ -224,7 +247,7 @@ ep_mx_dgrad_kernel(const __grid_constant__ MxDgradParams p) {
         tc_fence_after();
         const uint32_t tacc = tmem_base + (uint32_t)acc * TG_MAX_N;
         uint32_t add = 0u;
-        for (int kb = 0; kb < num_kb; ++kb, st.next(NST)) {
+        for (int kb = 0; kb < num_kb; ++kb, st.next(NST), used = used + 1 == MXD_EMPTY ? 0 : used + 1) {
           ok = warp_wait(&t_full[st.slot], st.parity, 3) && warp_wait(&w_full[st.slot], st.parity, 6);
           if (!ok) break;
           tc_fence_after();
@@ -233,7 +256,7 @@ ep_mx_dgrad_kernel(const __grid_constant__ MxDgradParams p) {
             umma_bf16_2cta(tacc, da, db, idesc, add);
 #pragma unroll
             for (int kk = 1; kk < BK / 16; ++kk) umma_bf16_2cta(tacc, da + kk * 128, db + kk * 2, idesc, 1u);
-            umma_commit_2cta(&empty[st.slot], 3);
+            umma_commit_2cta(&empty[used], 3);
           }
           add = 1u;
         }
@@ -241,18 +264,18 @@ ep_mx_dgrad_kernel(const __grid_constant__ MxDgradParams p) {
         if (issue) umma_commit_2cta(&acc_full[acc], 3);
       }
     }
-  } else if (warp < 2 + MXD_TEAMS * MXD_DECODERS) {
+  } else if (warp < 3 + MXD_TEAMS * MXD_DECODERS) {
     // ================= decode: 16 rows of the k-block a warp, in steps of four rows x 64 columns =================
-    const int team = (warp - 2) / MXD_DECODERS, dw = (warp - 2) % MXD_DECODERS, chunk = lane & 7, sub = lane >> 3;
+    const int team = (warp - 3) / MXD_DECODERS, dw = (warp - 3) % MXD_DECODERS, chunk = lane & 7, sub = lane >> 3;
     const uint32_t scale_bytes = 0x4040u + 0x0101u * (uint32_t)(chunk >> 2);
-    RingSlot st, ct;
-    for (int i = 0; i < team; ++i) { st.next(NST); ct.next(NC); }
+    RingSlot st, ct, free = first_free;
+    for (int i = 0; i < team; ++i) { st.next(NST); ct.next(NC); free.next(MXD_EMPTY); }
     int kb = team;
     bool ok = true;
     for (long long id = work_id0; id < total_tiles && ok; id += work_stride, kb -= num_kb) {
       for (; kb < num_kb; kb += MXD_TEAMS) {
         const int seg = kb >= kb_per_seg ? 1 : 0, k = (kb - seg * kb_per_seg) * BK + 16 * dw;
-        ok = warp_wait(&c_full[ct.slot], ct.parity, 7) && warp_wait(&empty[st.slot], st.parity ^ 1u, 8);
+        ok = warp_wait(&c_full[ct.slot], ct.parity, 7) && warp_wait(&empty[free.slot], free.parity ^ 1u, 8);
         if (!ok) break;
         const uint8_t* src = c_slots + ct.slot * MXD_CODE_SLOT;
         uint8_t* dst = w_slots + st.slot * MXD_W_BYTES + (16 * dw + sub) * 128;
@@ -290,12 +313,12 @@ ep_mx_dgrad_kernel(const __grid_constant__ MxDgradParams p) {
           else mbar_arrive_remote(&w_full[st.slot], 0);
         }
 #pragma unroll
-        for (int i = 0; i < MXD_TEAMS; ++i) { st.next(NST); ct.next(NC); }
+        for (int i = 0; i < MXD_TEAMS; ++i) { st.next(NST); ct.next(NC); free.next(MXD_EMPTY); }
       }
     }
   } else {
     // ========= epilogue: two sets of four warps, each warp one quarter of the tile's columns =========
-    const int ew = warp - 2 - MXD_TEAMS * MXD_DECODERS, q = warp & 3, set = ew >> 2;
+    const int ew = warp - 3 - MXD_TEAMS * MXD_DECODERS, q = warp & 3, set = ew >> 2;
     const int te = (ew & 3) * 32 + lane;                    // 0..127
     const int first = set * TG_CHUNK, step = TG_SETS * TG_CHUNK;
     int tile_n = 0, at = 0;
