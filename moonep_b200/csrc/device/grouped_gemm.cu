@@ -237,12 +237,27 @@ typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void
                              CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
                              CUtensorMapFloatOOBfill);
 
+// A thread that has made no call yet which needs the device (autograd's, when this product is the first of its backward
+// pass) has no current context, and a driver call does not make one as a runtime call would.
+template <class... Args>
+static int encode_map(Args... args) {
+  EncodeFn enc = (EncodeFn)driver_tensor_map_encode();
+  if (!enc) return fail(-10, "CUDA driver entry cuTensorMapEncodeTiled not available");
+  CUresult r = enc(args...);
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    int dev = 0;
+    MEP_CUDA_OK(cudaGetDevice(&dev));
+    MEP_CUDA_OK(cudaSetDevice(dev));
+    r = enc(args...);
+  }
+  if (r != CUDA_SUCCESS) return fail(-12, "cuTensorMapEncodeTiled failed with code %d", (int)r);
+  return 0;
+}
+
 // 2-D tensor [rows][cols] of bf16, or with F32 of fp32 (row stride ld elements), box [box_rows][box_cols], 128B swizzle.
 template <bool F32 = false>
 static int make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld,
                     int box_cols, int box_rows) {
-  EncodeFn enc = (EncodeFn)driver_tensor_map_encode();
-  if (!enc) return fail(-10, "CUDA driver entry cuTensorMapEncodeTiled not available");
   const int bytes = F32 ? 4 : 2;
   if (((uintptr_t)base & 15) != 0 || (ld * bytes) % 16 != 0)
     return fail(-11, "GEMM operand must be 16-byte aligned with a 16-byte multiple row stride");
@@ -250,19 +265,15 @@ static int make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols
   cuuint64_t strides[1] = {(cuuint64_t)(ld * bytes)};
   cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = enc(m, F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base),
-                   dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                   F32 ? CU_TENSOR_MAP_L2_PROMOTION_NONE : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(-12, "cuTensorMapEncodeTiled failed with code %d", (int)r);
-  return 0;
+  return encode_map(m, F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base),
+                    dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    F32 ? CU_TENSOR_MAP_L2_PROMOTION_NONE : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 // 2-D tensor [rows][cols] of bytes in 128-byte boxes with the 128-byte swizzle, or, unswizzled, (box_rows 0) [rows][cols / 4]
 // words in boxes of one row and box_words, or (box_rows -16) bytes in boxes of 64 x 16 rows.
 static int make_byte_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int box_rows, int box_words = 256) {
-  EncodeFn enc = (EncodeFn)driver_tensor_map_encode();
-  if (!enc) return fail(-10, "CUDA driver entry cuTensorMapEncodeTiled not available");
   if (((uintptr_t)base & 15) != 0 || cols % 16 != 0) return fail(-11, "mx operands must be 16-byte aligned");
   const bool words = box_rows == 0;
   cuuint64_t dims[2] = {(cuuint64_t)(words ? cols / 4 : cols), (cuuint64_t)rows};
@@ -270,12 +281,10 @@ static int make_byte_map(CUtensorMap* m, const void* base, int64_t rows, int64_t
   const bool plain = box_rows < 0;
   cuuint32_t box[2] = {words ? (cuuint32_t)box_words : plain ? 64u : 128u, words ? 1u : (cuuint32_t)(plain ? -box_rows : box_rows)};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = enc(m, words ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims,
-                   strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   words || plain ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(-12, "cuTensorMapEncodeTiled failed with code %d", (int)r);
-  return 0;
+  return encode_map(m, words ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims,
+                    strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    words || plain ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 // Fused dispatch launches: CTAs of different ranks wait for one another's copy warps, so the whole

@@ -2,6 +2,8 @@
 
 Quantised values have to be equal.  A product's result is within half a bf16 step, 2^-8 of its value, and what K sums in
 fp32 can lose, K 2^-24 of the sum of magnitudes."""
+import threading
+
 import pytest
 import torch
 
@@ -818,6 +820,26 @@ def test_two_streams_at_once():
     assert torch.equal(out, want[0])
     for g, w in zip(got, want):
         assert all(torch.equal(y, w) for y in g)
+
+
+@gpu
+@pytest.mark.parametrize("call", ["product", "gate and up", "gradients of rows", "bf16 gradients of rows"])
+def test_first_call_of_a_thread(call):
+    """A thread that has used no device yet, as autograd's before its first backward pass."""
+    from moonep_b200.ops import gemm, mx
+    gen = _gen(50)
+    x, w = torch.randn(64, 128, generator=gen).bfloat16().cuda(), torch.randn(1, 128, 128, generator=gen).bfloat16().cuda()
+    q, wq, pair, ends = mx.quantize(x), mx.quantize(w), mx.pack_gate_up(w, w), _ends([64]).cuda()
+    run = {"product": lambda: mx.matmul(q, wq, ends), "gate and up": lambda: mx.gateup_swiglu(q, pair, ends)[0],
+           "gradients of rows": lambda: mx.down_dgrad(x, wq, ends),
+           "bf16 gradients of rows": lambda: gemm.down_dgrad(x, w, ends)}[call]
+    want = run().cpu()
+    got = []
+    thread = threading.Thread(target=lambda: got.append(run()))
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    assert len(got) == 1 and torch.equal(got[0].cpu(), want)
 
 
 @gpu
