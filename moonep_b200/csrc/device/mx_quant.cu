@@ -231,7 +231,8 @@ struct MxDequantParams {
 
 // A lane takes eight values of a row, a warp MXD_DEPTH times 256.  Bound by HBM (6.0 TB/s); the values' bytes are looked
 // up, which takes half the instructions of computing them.  (By the conversions of
-// ep_mx_dgrad_kernel: 5.8 TB/s.  Sixteen values a lane: 4.3.)
+// ep_mx_dgrad_kernel: 5.8 TB/s.  Sixteen values a lane: 4.3.)  Rows of odd lengths have their eights where the output is
+// aligned and compute them, 3.1 - 3.4 TB/s (by elements 1.4; looked up, with two scales a pair, 2.8 - 3.0).
 constexpr int MXD_DEPTH = 8;
 
 template <class T, bool VEC>
@@ -248,24 +249,36 @@ __global__ void __launch_bounds__(MXQ_WARPS * 32) ep_mx_dequant_kernel(const __g
     const uint8_t* codes = p.codes + ((long long)mat * p.in_rows + r) * p.code_bytes;
     const uint8_t* scales = p.scales + (long long)mat * p.row_atoms * p.k_atoms * MX_ATOM_BYTES + mx_scale_offset(r, 0, p.k_atoms);
     T* out = (T*)p.out + ((long long)out_mat * p.rows + row) * p.cols;
-    if constexpr (!VEC) {        // rows start anywhere: neighbouring lanes take neighbouring elements
-      for (int c0 = blockIdx.y * 256 * MXD_DEPTH + lane; c0 < p.cols; c0 += gridDim.y * 256 * MXD_DEPTH) {
-#pragma unroll 2
-        for (int i = 0; i < 8 * MXD_DEPTH; i += 8) {
-          uint32_t code[8], b[8];
+    if constexpr (!VEC) {        // rows start anywhere: eights begin where the output is aligned, their codes lie in two words
+      constexpr int DEPTH = MXD_DEPTH / 2;
+      const int first = -(int)((uintptr_t)out / sizeof(T) % 8);
+      for (int c0 = first + blockIdx.y * 256 * DEPTH + lane * 8; c0 < p.cols; c0 += gridDim.y * 256 * DEPTH) {
+        uint32_t code[DEPTH][2], b[DEPTH][2];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int c = c0 + (i + e) * 32;
-            code[e] = c < p.cols ? codes[c >> 1] >> (4 * (c & 1)) : 0u;
-            b[e] = c < p.cols ? scales[(long long)(c >> 7) * MX_ATOM_BYTES + (c >> 5 & 3)] : 0u;
+        for (int i = 0; i < DEPTH; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {        // the word with the first of the eight and the next; the first one's scale and the last one's
+            const int c = c0 + i * 256, w = (c >> 3) + h, e = min(max(c + 7 * h, 0), p.cols - 1);
+            code[i][h] = w >= 0 && 4 * w < p.code_bytes ? reinterpret_cast<const uint32_t*>(codes)[w] : 0u;
+            b[i][h] = scales[(long long)(e >> 7) * MX_ATOM_BYTES + (e >> 5 & 3)];
           }
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int c = c0 + (i + e) * 32;
-            if (c >= p.cols) break;
-            const float f = mx_element(code[e]) * mx_value(b[e]);
-            if constexpr (sizeof(T) == 2) out[c] = __float2bfloat16(f);
-            else out[c] = f;
+        for (int i = 0; i < DEPTH; ++i) {
+          const int c = c0 + i * 256;
+          if (c >= p.cols) break;
+          const uint32_t q = __funnelshift_r(code[i][0], code[i][1], 4 * (c & 7));
+          const float s0 = mx_value(b[i][0]), s1 = mx_value(b[i][1]);
+          const int of_first = 32 - (c & 31);        // so many have the first scale
+          MxEight<T> v;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v.p[e / 2].e[e % 2] = T(mx_element(q >> (4 * e)) * (e < of_first ? s0 : s1));
+          if (c >= 0 && c + 8 <= p.cols) {
+#pragma unroll
+            for (int e = 0; e < (int)sizeof(T) / 2; ++e) __stcs(reinterpret_cast<uint4*>(out + c) + e, reinterpret_cast<const uint4*>(&v)[e]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (c + e >= 0 && c + e < p.cols) out[c + e] = v.p[e / 2].e[e % 2];
           }
         }
       }
