@@ -78,26 +78,61 @@ __device__ __forceinline__ uint32_t* mx_scale_row(const MxQuantParams& p, int ma
 // block made a chain of load latencies (the kernel along the columns: 925 us for 32 x 7168 x 2048 in bf16, 4.2x).
 template <class T> struct __align__(16) MxEight { MxPair<T> p[4]; };
 
-// Eight elements of a row from column c on; behind the row's end zeros.
+// Eight elements of a row from column c on, as they were loaded; behind the row's end zeros.
 template <class T, bool VEC>
-__device__ __forceinline__ MxEight<T> mx_load8(const T* row, int c, int cols) {
+struct MxRaw {                            // rows of 16-byte pieces (cols is a multiple of 8)
   MxEight<T> v;
-  if constexpr (VEC) {                    // (cols is a multiple of 8)
+  __device__ __forceinline__ void load(const T* row, int c, int cols) {
     uint4* q = reinterpret_cast<uint4*>(&v);
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i)
       q[i] = c < cols ? __ldcs(reinterpret_cast<const uint4*>(row + c) + i) : make_uint4(0, 0, 0, 0);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v.p[i / 2].e[i % 2] = c + i < cols ? row[c + i] : T(0.f);
   }
-  return v;
-}
+  __device__ __forceinline__ const MxEight<T>& get() const { return v; }
+};
+template <class T>
+struct MxRaw<T, false> {                  // rows that start anywhere: the aligned pieces they lie in, moved when they are used
+  static constexpr int PIECES = sizeof(T) / 2 + 1, WORDS = 2 * sizeof(T);
+  uint32_t w[4 * PIECES];
+  int off;                                // bytes of the first piece in front of them
+  __device__ __forceinline__ void load(const T* row, int c, int cols) {
+    const uintptr_t at = (uintptr_t)(row + c), first = at & ~(uintptr_t)15;
+    const int pieces = at == first ? PIECES - 1 : PIECES;
+    off = (int)(at - first);
+    if (first >= (uintptr_t)row && first + 16 * pieces <= (uintptr_t)(row + cols)) {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const uint4 q = i < pieces ? reinterpret_cast<const uint4*>(first)[i] : make_uint4(0, 0, 0, 0);
+        w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
+      }
+    } else {                              // (nothing outside the row is read)
+      MxEight<T> v;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v.p[i / 2].e[i % 2] = c + i < cols ? row[c + i] : T(0.f);
+#pragma unroll
+      for (int i = 0; i < 4 * PIECES; ++i) w[i] = i < WORDS ? reinterpret_cast<const uint32_t*>(&v)[i] : 0u;
+      off = 0;
+    }
+  }
+  __device__ __forceinline__ MxEight<T> get() const {
+    MxEight<T> v;
+    uint32_t u[WORDS + 2];
+#pragma unroll
+    for (int i = 0; i < WORDS + 2; ++i) u[i] = off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < WORDS + 1; ++i) u[i] = off & 4 ? u[i + 1] : u[i];
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i)
+      reinterpret_cast<uint32_t*>(&v)[i] = sizeof(T) == 2 ? __funnelshift_r(u[i], u[i + 1], 8 * (off & 2)) : u[i];
+    return v;
+  }
+};
 
 // Along the rows.  A warp takes MXQ_DEPTH parts of 256 elements of a row, a lane eight of each: four lanes share a
 // block and store its scale, a phase each.  Bound by HBM: 8192 x 7168 in bf16 30 us, 5.0 TB/s with the launch, fp32 42 us,
 // 6.3.  (Sixteen elements a lane are fewer instructions, but two 16-byte accesses of a lane side by side: 14336 x 7168
-// 51.6 us, 53.7; odd rows 48, 72; 32 x 7168 x 2048 215, 201.)
+// 51.6 us, 53.7; 32 x 7168 x 2048 215, 201.)  Rows of odd lengths: 8192 x 7001 in fp32 54 us, 4.8 TB/s (by elements 68), 7167 in
+// bf16 45 (48).
 constexpr int MXQ_WARPS = 8, MXQ_DEPTH = 4;
 
 template <class T, bool VEC>
@@ -113,16 +148,17 @@ __global__ void __launch_bounds__(MXQ_WARPS * 32) ep_mx_quant_rows_kernel(const 
     uint8_t* codes = p.codes + ((long long)mat * p.out_rows + row) * p.code_bytes;
     uint8_t* scales = reinterpret_cast<uint8_t*>(mx_scale_row(p, mat, row, lane & 3));    // of this lane's phase, if it has one
     for (int c0 = blockIdx.y * 256 * MXQ_DEPTH; c0 < p.cols; c0 += gridDim.y * 256 * MXQ_DEPTH) {
-      MxEight<T> raw[MXQ_DEPTH];
+      MxRaw<T, VEC> raw[MXQ_DEPTH];
 #pragma unroll
-      for (int i = 0; i < MXQ_DEPTH; ++i) raw[i] = mx_load8<T, VEC>(x, c0 + i * 256 + lane * 8, p.cols);
+      for (int i = 0; i < MXQ_DEPTH; ++i) raw[i].load(x, c0 + i * 256 + lane * 8, p.cols);
 #pragma unroll
       for (int i = 0; i < MXQ_DEPTH; ++i) {
         if (c0 + i * 256 >= p.cols) break;          // (the same for the whole warp)
         const int c = c0 + i * 256 + lane * 8;
+        const MxEight<T> u = raw[i].get();
         MxMax<T> m;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) m.add(raw[i].p[e]);
+        for (int e = 0; e < 4; ++e) m.add(u.p[e]);
         uint32_t a = max(m.left(), m.right());
         a = max(a, __shfl_xor_sync(0xffffffffu, a, 1));
         a = max(a, __shfl_xor_sync(0xffffffffu, a, 2));
@@ -130,7 +166,7 @@ __global__ void __launch_bounds__(MXQ_WARPS * 32) ep_mx_quant_rows_kernel(const 
         const float inv = mx_inverse(b);
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) *reinterpret_cast<float2*>(v + 2 * e) = mx_times(raw[i].p[e], inv, inv);
+        for (int e = 0; e < 4; ++e) *reinterpret_cast<float2*>(v + 2 * e) = mx_times(u.p[e], inv, inv);
         // (a NaN scale: zeros, whatever inf * 0 would give)
         const uint32_t q = b == 255u ? 0u : mx_codes(v);
         if (c < 2 * p.code_bytes) *reinterpret_cast<uint32_t*>(codes + c / 2) = q;

@@ -83,6 +83,22 @@ def test_quantise_strides(axis):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_quantise_rows_that_start_anywhere(dtype):
+    """Every offset in 16 bytes, lengths around a lane's eight elements and a warp's 256; a neighbour's NaN stays out."""
+    from moonep_b200.ops import mx
+    base = _spread(_gen(26), 5, 311).clamp(-60000, 60000).to(dtype)
+    for length in (1, 7, 8, 9, 23, 33, 257, 300):
+        for at in range(1, 10):
+            x = base.clone()
+            x[:, :at], x[:, at + length:] = float("nan"), float("nan")
+            q = mx.quantize(x.cuda()[:, at:at + length])
+            want = ox.quantise(base[:, at:at + length].contiguous())
+            _equal(q.dequantize(torch.float32), want)
+            _equal(q.dequantize(), want)
+
+
+@gpu
 def test_quantise_extremes():
     """Largest, smallest, subnormal and non-finite values; zero blocks; a block that is not full."""
     from moonep_b200.ops import mx
