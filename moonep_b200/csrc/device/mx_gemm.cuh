@@ -83,7 +83,7 @@ template <int EPI> constexpr int mxg_threads() { return 64 + mxg_sets<EPI>() * 1
 // Shared memory that the kernel declares itself: staged tokens, group tables, scales of two tiles, barriers (rounded up).
 template <int EPI> constexpr int mxg_token_row() { return (EPI == MX_EPI_SWIGLU_SAVE ? 384 : EPI == MX_EPI_SWIGLU ? 128 : 256) + 16; }
 template <int EPI> constexpr int mxg_static_smem() {
-  return mxg_sets<EPI>() * TG_CHUNK * mxg_token_row<EPI>() + (3 * MAX_GROUPS + 1) * 4 + (EPI == MX_EPI_BF16 ? 8 : 2 * MXG_MAX_N * 4) +
+  return mxg_sets<EPI>() * TG_CHUNK * mxg_token_row<EPI>() + (3 * MAX_GROUPS + 1) * 4 + (EPI == MX_EPI_BF16 ? 8 : mxg_sets<EPI>() * 128 * 4) +
          (EPI == MX_EPI_SWIGLU_BWD ? mxg_sets<EPI>() * 4 * TG_CHUNK * 4 : 0) + 512;
 }
 
@@ -151,7 +151,8 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
   __shared__ int s_prefix[MAX_GROUPS + 1];
   __shared__ __align__(128) uint8_t s_stage[SETS][TG_CHUNK * TOK_ROW];
   __shared__ float s_part[BWD ? SETS : 1][BWD ? 4 : 1][BWD ? TG_CHUNK : 1];     // sums over a quarter's columns
-  __shared__ float s_scale[GATED ? 2 : 1][GATED ? MXG_MAX_N : 1];
+  // row scales of a set's tokens in the present tile, chunk by chunk.  A set's own: it may be a whole tile ahead of another
+  __shared__ float s_scale[GATED ? SETS : 1][GATED ? 128 : 1];
 
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   uint8_t* stages = (uint8_t*)(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
@@ -340,11 +341,11 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
       // this set's chunks start at tokens first, first + step, ...; the sets change places from tile to tile, so that
       // tiles of few tokens keep all of them busy
       const int first = (set + tile_n) % SETS * TG_CHUNK, my_tok = (te >> 5) * step + first + (te & 31);
-      if constexpr (GATED) {       // (published by the barriers below)
-        for (int i = my_tok; i < t.n; i += 4 * step) {
-          const int r = t.row0 + i;
-          s_scale[acc][i] = r >= t.lo && r < t.hi && p.row_scale != nullptr ? p.row_scale[r] : 1.f;
-        }
+      if constexpr (GATED) {
+        // (published by epilogue_all() below; the set's last reads of the tile before were in front of its last epilogue_sync())
+        static_assert(4 * SETS * TG_CHUNK >= MXG_MAX_N, "a thread has one token of its set at most");
+        const int r = t.row0 + my_tok;
+        if (my_tok < t.n) s_scale[set][te] = r >= t.lo && r < t.hi && p.row_scale != nullptr ? p.row_scale[r] : 1.f;
       }
       // the gradients that meet a chunk's fragments: columns 8 half + lane / 4 of the quarter, tokens 8 j + 2 (lane % 4)
       // and the next at [4 j + 2 half]; on their way before the fragments are
@@ -400,7 +401,7 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
         release_acc();
       }
 #pragma unroll 1
-      for (int c = first; c < t.n; c += step) {
+      for (int c = first, own = 0; c < t.n; c += step, own += TG_CHUNK) {      // own: counted over the set's tokens
         __syncwarp();
         tmem_ld_wait();
         uint32_t pk[16];       // [16-row half][token block][lower, upper 8 rows]
@@ -421,7 +422,7 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
             for (int e = 0; e < 2; ++e) {
               const float g = __uint_as_float(r[2 * i + e]), u = __uint_as_float(r[16 + 2 * i + e]);
               const float sig = mx_sigmoid(g), d = da[2 * i + e];
-              const float ds = d * s_scale[acc][c + 8 * (i >> 1) + 2 * (lane & 3) + e];
+              const float ds = d * s_scale[set][own + 8 * (i >> 1) + 2 * (lane & 3) + e];
               // (columns behind the last have whatever lies behind the weights)
               part[2 * (i >> 1) + e] += col + 8 * (i & 1) < p.N ? d * (g * sig) * u : 0.f;
               dg[e] = ds * u * (sig * (1.f + g * (1.f - sig)));
@@ -446,7 +447,7 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const float g = __uint_as_float(r[2 * i + e]), u = __uint_as_float(r[16 + 2 * i + e]);
-              a[e] = g * mx_sigmoid(g) * u * s_scale[acc][c + 8 * (i >> 1) + 2 * (lane & 3) + e];
+              a[e] = g * mx_sigmoid(g) * u * s_scale[set][own + 8 * (i >> 1) + 2 * (lane & 3) + e];
             }
             pa[i] = pack(a[0], a[1]);
           }
