@@ -169,7 +169,7 @@ ep_mx_dgrad_kernel(const __grid_constant__ MxDgradParams p) {
     const int start = g == 0 ? 0 : s_end[g - 1], end = s_end[g];
     t.n = ((s_valid[g] + nt - 1) / nt + 31) & ~31;
     t.row0 = start + ti * t.n;
-    t.rows = max(0, min(t.n, end - t.row0));
+    t.rows = max(0, min(t.n, start + s_valid[g] - t.row0));      // (the padding rows of its last 32 are computed, not stored)
     t.zero_to = ti == nt - 1 ? end : 0;
     t.m0 = mi * 256;
     t.alloc = t.g_local = 0;

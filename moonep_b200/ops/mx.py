@@ -412,7 +412,7 @@ def down_dgrad(dy: torch.Tensor, wd: MxTensor, cu_seqlens: Optional[torch.Tensor
                fp32: bool = False) -> torch.Tensor:
     """``d_act[rows,H'] = dy Wd[g]`` for bf16 ``dy`` ``[rows, H]`` and 4-bit ``wd`` ``[G, H, H']`` (or ``[H, H']``): the
     gradient of :func:`matmul` with respect to the values of its rows.  bf16, or the ``fp32`` sums (padding rows and rows
-    of no group are undefined then; else zeros, padding and behind the last group)."""
+    of no group are undefined then; else zeros, padding and behind the last group, whatever ``dy`` holds there)."""
     assert isinstance(wd, MxTensor) and len(wd.shape) < 4, "wd must come from quantize"
     out = torch.empty(dy.shape[0], wd.shape[-1], dtype=torch.float32 if fp32 else torch.bfloat16, device=wd.device)
     return _dgrad((dy,), wd, cu_seqlens, pads, out)
@@ -421,7 +421,8 @@ def down_dgrad(dy: torch.Tensor, wd: MxTensor, cu_seqlens: Optional[torch.Tensor
 def gateup_dgrad(dg: torch.Tensor, du: torch.Tensor, wgu: MxTensor, cu_seqlens: Optional[torch.Tensor] = None, *,
                  pads: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``dx[rows,H] = dg Wg[g]^T + du Wu[g]^T`` for bf16 ``dg``/``du`` ``[rows, H']`` and the packed weights of
-    :func:`gateup_swiglu`; zeros in padding rows and behind the last group.  ``out`` ``[rows or more, H]`` bf16 takes it."""
+    :func:`gateup_swiglu`; zeros in padding rows and behind the last group, whatever ``dg`` and ``du`` hold there.
+    ``out`` ``[rows or more, H]`` bf16 takes it."""
     assert isinstance(wgu, MxTensor) and len(wgu.shape) == 4, "wgu must come from pack_gate_up"
     if out is None:
         out = torch.empty(dg.shape[0], wgu.shape[-1], dtype=torch.bfloat16, device=wgu.device)
