@@ -456,15 +456,16 @@ def _pack(wg, wu, wd):
 
 class _ExpertFFN(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, wg, wu, wd, row_scale, cu_seqlens, pads):
+    def forward(ctx, x, wg, wu, wd, row_scale, cu_seqlens, pads, recorded):
+        # (needs_input_grad says which inputs require grad, also where nothing is recorded)
         wgu, wdq = _pack(wg, wu, wd)
-        keep = any(ctx.needs_input_grad)
+        keep = recorded and any(ctx.needs_input_grad)
         xq = quantize(x, rows_ptr=None if cu_seqlens is None else cu_seqlens[-1:])
         act, _, _ = gateup_swiglu(xq, wgu, cu_seqlens, row_scale=row_scale, quantize=True, pads=pads)
         y = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
         H = x.shape[1]
         _launch(act, wdq, H, 0, cu_seqlens, pads, None, y.data_ptr(), 0, 0, 0, 0, H, zero_tail=1,
-                check_groups=int(any(ctx.needs_input_grad[1:4])))
+                check_groups=int(recorded and any(ctx.needs_input_grad[1:4])))
         if keep:
             ctx.shapes = None if isinstance(wg, MxTensor) else (wg.shape, wd.shape)
             save_operands(ctx, (xq, act, wgu, wdq), row_scale, cu_seqlens, pads)
@@ -484,7 +485,7 @@ class _ExpertFFN(torch.autograd.Function):
         if dy.shape[0] == 0:
             zeros = lambda need, i: torch.zeros(ctx.shapes[i], **bf16) if need else None
             return (torch.empty_like(dy) if need_x else None, zeros(need_g, 0), zeros(need_u, 0), zeros(need_d, 1),
-                    torch.empty_like(row_scale) if need_s else None, None, None)
+                    torch.empty_like(row_scale) if need_s else None, None, None, None)
         if need_d:
             grads[2] = torch.empty(G, H, Hp, **bf16)
             gemm.wgrad(dy, act.dequantize(rows_ptr=rows_ptr), cu, grads[2], pads=pads)
@@ -499,7 +500,7 @@ class _ExpertFFN(torch.autograd.Function):
                 out = torch.empty(2, G, H, Hp, **bf16)
                 gemm.wgrad2(xq.dequantize(rows_ptr=rows_ptr), (d_gate, d_up), cu, (out[0], out[1]), pads=pads)
                 grads[:2] = (out[i].view(ctx.shapes[0]) for i in range(2))
-        return dx, grads[0], grads[1], grads[2], d_scale, None, None
+        return dx, grads[0], grads[1], grads[2], d_scale, None, None, None
 
 
 def expert_ffn(x: torch.Tensor, wg, wu, wd, cu_seqlens: Optional[torch.Tensor] = None, *,
@@ -517,7 +518,8 @@ def expert_ffn(x: torch.Tensor, wg, wu, wd, cu_seqlens: Optional[torch.Tensor] =
 
     Rows behind the last group get zeros, in ``y`` and in ``x``'s gradient.  For gradients H must be a multiple of 128
     and H' of 8, and for the weights' every group's rows a multiple of 64, padding rows of ``x`` being zero (what
-    ``Buffer.dispatch`` gives), but for a group that ends with ``x`` itself; ``gemm.check_status`` reports others.
+    ``Buffer.dispatch`` gives), but for a group that ends with ``x`` itself; ``gemm.check_status`` reports others, from
+    the forward pass on, where autograd records it.
     Every call can be captured into a CUDA graph, forward and backward (``utils.graph.GraphedStep``); as with any captured
     ``backward()``, no eager graph of the same leaves may be alive meanwhile."""
     assert isinstance(x, torch.Tensor) and x.dim() == 2 and x.dtype == torch.bfloat16, "x must be bf16 [rows, H]"
@@ -540,6 +542,7 @@ def expert_ffn(x: torch.Tensor, wg, wu, wd, cu_seqlens: Optional[torch.Tensor] =
         assert row_scale.dtype == torch.float32 and row_scale.dim() == 1 and row_scale.shape[0] == x.shape[0], "one fp32 scale a row"
         row_scale = row_scale.contiguous()
     assert pads is None or cu_seqlens is not None, "padding ranges go with cu_seqlens"
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, *trained) + (() if row_scale is None else (row_scale,))):
+    recorded = torch.is_grad_enabled()
+    if recorded and any(t.requires_grad for t in (x, *trained) + (() if row_scale is None else (row_scale,))):
         assert H % 128 == 0 and Hp % 8 == 0, "gradients need H % 128 == 0 and H' % 8 == 0"
-    return _ExpertFFN.apply(x, wg, wu, wd, row_scale, cu_seqlens, pads)
+    return _ExpertFFN.apply(x, wg, wu, wd, row_scale, cu_seqlens, pads, recorded)
