@@ -350,6 +350,9 @@ __global__ void __launch_bounds__(WG_THREADS, 1) ep_weight_grad_kernel(const __g
       tc_fence_after();
       const uint32_t tacc = tmem_base + (uint32_t)acc * BN + ((uint32_t)(q * 32) << 16) + (uint32_t)cofs;
       const bool in_rows = t.m0 < p.Mw;      // (the second CTA of a pair may have no rows left)
+      // A group that ends inside a block of rows has its neighbour's in the sum.  Leaves of autograd (WG_BF16), whose user need
+      // not have asked for the status, get NaN instead; behind the last row there are zeros.
+      const bool torn = MODE == WG_BF16 && (s_end[t.g] - t.row0) % BK != 0 && s_end[t.g] != p.total_rows;
       bool go_on = true;
       // the accumulator has been read: the next tile but one may overwrite it
       auto release = [&] {
@@ -397,6 +400,10 @@ __global__ void __launch_bounds__(WG_THREADS, 1) ep_weight_grad_kernel(const __g
         } else {                             // an empty group's grad is zero
 #pragma unroll
           for (int e = 0; e < 32; ++e) r[e] = 0u;
+        }
+        if (torn) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) r[e] = 0x7FC00000u;
         }
         if (k == WG_STEPS - 1) release();
         const int col = ni * BN + cofs;

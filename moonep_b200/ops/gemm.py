@@ -294,7 +294,8 @@ def wgrad(a, b, cu_seqlens, grad_local, *, grad_slot=None, split=None, accumulat
     with ``select=0``.  The stored grads are the ones that ``reduce_grad`` has to move, so computing
     them first lets that transfer run beside the rest of the weight grad.
 
-    A bf16 ``grad_local`` takes the grads rounded (no slots, no ``accumulate``, no ``sgd``; N a multiple of 8).
+    A bf16 ``grad_local`` takes the grads rounded (no slots, no ``accumulate``, no ``sgd``; N a multiple of 8), and NaN for
+    a group whose size is no multiple of 64, unless it ends with ``a`` itself.
 
     ``rows``: how many rows of ``a`` hold tokens, where the caller knows (a Buffer's ``N``; its row tensor has
     spare rows).  It changes no result, only how the launch is split."""

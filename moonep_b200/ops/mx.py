@@ -518,8 +518,8 @@ def expert_ffn(x: torch.Tensor, wg, wu, wd, cu_seqlens: Optional[torch.Tensor] =
 
     Rows behind the last group get zeros, in ``y`` and in ``x``'s gradient.  For gradients H must be a multiple of 128
     and H' of 8, and for the weights' every group's rows a multiple of 64, padding rows of ``x`` being zero (what
-    ``Buffer.dispatch`` gives), but for a group that ends with ``x`` itself; ``gemm.check_status`` reports others, from
-    the forward pass on, where autograd records it.
+    ``Buffer.dispatch`` gives), but for a group that ends with ``x`` itself; the weight grads of other groups are NaN, and
+    ``gemm.check_status`` reports them, from the forward pass on, where autograd records it.
     Every call can be captured into a CUDA graph, forward and backward (``utils.graph.GraphedStep``); as with any captured
     ``backward()``, no eager graph of the same leaves may be alive meanwhile."""
     assert isinstance(x, torch.Tensor) and x.dim() == 2 and x.dtype == torch.bfloat16, "x must be bf16 [rows, H]"

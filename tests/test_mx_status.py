@@ -28,3 +28,29 @@ def test_parameters_without_gradients(mode):
     gemm.check_status()
     assert not y.requires_grad
     assert torch.equal(y, mx.expert_ffn(x, *(t.detach() for t in w), _cu(100, 200)))
+
+
+@gpu
+@pytest.mark.parametrize("ends,bad", [((100, 256), [0]), ((64, 200), [1]), ((128, 256), []), ((64, 256), []), ((128, 250), [1]),
+                                      ((96, 160), [0])])
+def test_gradients_of_groups_that_weight_grads_cannot_take(ends, bad):
+    """They are NaN; those of other groups, and the gradients of rows, are what they are."""
+    from moonep_b200.ops import gemm, mx
+    x, w = _inputs()
+    x.requires_grad_(True)
+    dy = torch.randn(256, 128, generator=_gen(71)).bfloat16().cuda()
+    grads = torch.autograd.grad(mx.expert_ffn(x, *w, _cu(*ends)), (x, *w), dy)
+    if bad:
+        with pytest.raises(RuntimeError, match=f"group {bad[0]} has"):
+            gemm.check_status()
+        gemm.reset_status()
+    gemm.check_status()
+    start = 0
+    for g, end in enumerate(ends):
+        rows = x.detach()[start:end].clone().requires_grad_(True)
+        one = [t.detach()[g].clone().requires_grad_(True) for t in w]
+        want = torch.autograd.grad(mx.expert_ffn(rows, *one), (rows, *one), dy[start:end])
+        assert torch.equal(grads[0][start:end], want[0])
+        for got, ref in zip(grads[1:], want[1:]):
+            assert got[g].isnan().all() if g in bad else torch.equal(got[g], ref)
+        start = end
