@@ -144,13 +144,17 @@ __device__ __forceinline__ bool arrive_wait(const int32_t* ctr, int expect, int 
   return true;
 }
 
-// Rows of a group that hold tokens (its real rows if the padding ranges are known); at least one
-// for a group that is not empty.
+// Rows of a group that hold tokens: its real rows if the padding ranges are known.
 template <class Params>
-__device__ __forceinline__ int group_valid(const Params& p, int g, int start, int end) {
+__device__ __forceinline__ int group_tokens(const Params& p, int g, int start, int end) {
   if (p.pads == nullptr || end <= start) return end - start;
   const int first = p.pads[2 * g], n = p.pads[2 * g + 1];
-  return (n > 0 && first >= start && first < end) ? max(1, first - start) : end - start;
+  return (n > 0 && first >= start && first < end) ? first - start : end - start;
+}
+// The same; at least one for a group that is not empty.
+__device__ __forceinline__ int group_valid(const GemmKParams& p, int g, int start, int end) {
+  const int n = group_tokens(p, g, start, end);
+  return end > start ? max(1, n) : n;
 }
 
 }  // namespace mep

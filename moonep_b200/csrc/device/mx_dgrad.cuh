@@ -127,14 +127,15 @@ ep_mx_dgrad_kernel(const __grid_constant__ MxDgradParams p) {
     const int start = g == 0 || p.cu_seqlens == nullptr ? 0 : clamped(p.cu_seqlens[g - 1]);
     const int end = clamped(p.cu_seqlens != nullptr ? p.cu_seqlens[g] : p.total_rows);
     s_end[g] = end;
-    s_valid[g] = end > start ? group_valid(p, g, start, end) : 0;
+    const int tokens = end > start ? group_tokens(p, g, start, end) : 0;
+    s_valid[g] = end > start && tokens == 0 ? -1 : tokens;       // (-1: nothing but padding, a tile that writes the zeros)
   }
   __syncthreads();
   if (warp == 0) {      // exclusive prefix of token tiles per group
     int run = 0;
     for (int g0 = 0; g0 < p.ngroups; g0 += 32) {
       const int g = g0 + lane;
-      const int nt = g < p.ngroups ? token_tiles(s_valid[g]) : 0;
+      const int nt = g < p.ngroups ? token_tiles(abs(s_valid[g])) : 0;
       int incl = nt;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -167,9 +168,9 @@ ep_mx_dgrad_kernel(const __grid_constant__ MxDgradParams p) {
     const int local = (int)(id - (long long)s_prefix[g] * m_tiles);
     const int mi = local / nt, ti = local - mi * nt;       // tiles that share weights are neighbours
     const int start = g == 0 ? 0 : s_end[g - 1], end = s_end[g];
-    t.n = ((s_valid[g] + nt - 1) / nt + 31) & ~31;
+    t.n = ((abs(s_valid[g]) + nt - 1) / nt + 31) & ~31;
     t.row0 = start + ti * t.n;
-    t.rows = max(0, min(t.n, start + s_valid[g] - t.row0));      // (the padding rows of its last 32 are computed, not stored)
+    t.rows = max(0, min(t.n, start + max(s_valid[g], 0) - t.row0));      // (the padding rows of its last 32 are computed, not stored)
     t.zero_to = ti == nt - 1 ? end : 0;
     t.m0 = mi * 256;
     t.alloc = t.g_local = 0;

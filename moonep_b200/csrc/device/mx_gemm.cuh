@@ -188,14 +188,16 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
         p.status[5] = end - start;
       }
     }
-    s_span[g] = end > start ? (start & 31) + group_valid(p, g, start, end) : 0;
+    // (a group of nothing but padding: negative, of one row, for a tile that writes the zeros)
+    const int tokens = end > start ? group_tokens(p, g, start, end) : 0;
+    s_span[g] = tokens > 0 ? (start & 31) + tokens : end > start ? -((start & 31) + 1) : 0;
   }
   __syncthreads();
   if (warp == 0) {      // exclusive prefix of token tiles per group
     int run = 0;
     for (int g0 = 0; g0 < p.ngroups; g0 += 32) {
       const int g = g0 + lane;
-      const int nt = g < p.ngroups ? (s_span[g] + MXG_MAX_N - 1) / MXG_MAX_N : 0;
+      const int nt = g < p.ngroups ? (abs(s_span[g]) + MXG_MAX_N - 1) / MXG_MAX_N : 0;
       int incl = nt;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -228,7 +230,7 @@ ep_mx_gemm_kernel(const __grid_constant__ MxParams p) {
     const int local = (int)(id - (long long)s_prefix[g] * m_tiles);
     const int mi = local / nt, ti = local - mi * nt;       // tiles that share weights are neighbours
     const int start = g == 0 ? 0 : s_end[g - 1], end = s_end[g];
-    const int length = s_span[g], valid = start + length - (start & 31);
+    const int span = s_span[g], length = abs(span), valid = span < 0 ? start : start + length - (start & 31);
     t.n = ((length + nt - 1) / nt + 31) & ~31;
     t.row0 = (start & ~31) + ti * t.n;
     t.lo = max(t.row0, start);
