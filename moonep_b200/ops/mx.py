@@ -287,6 +287,7 @@ def _launch(a: MxTensor, w: MxTensor, N: int, gated: int, cu_seqlens, pads, row_
     cu = pad = scale = 0
     if cu_seqlens is None:
         assert groups == 1, "several groups need cu_seqlens"
+        assert pads is None, "padding ranges go with cu_seqlens"
     else:
         assert cu_seqlens.dtype is torch.int32 and cu_seqlens.get_device() == index and cu_seqlens.is_contiguous() \
             and cu_seqlens.numel() == groups, "cu_seqlens must be int32, one entry a group"
@@ -394,6 +395,7 @@ def _dgrad(segs, w: MxTensor, cu_seqlens, pads, out: torch.Tensor) -> torch.Tens
     cu = pad = 0
     if cu_seqlens is None:
         assert groups == 1, "several groups need cu_seqlens"
+        assert pads is None, "padding ranges go with cu_seqlens"
     else:
         assert cu_seqlens.dtype is torch.int32 and cu_seqlens.get_device() == index and cu_seqlens.is_contiguous() \
             and cu_seqlens.numel() == groups, "cu_seqlens must be int32, one entry a group"

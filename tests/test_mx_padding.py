@@ -70,3 +70,18 @@ def test_groups_of_padding_alone():
     assert (got[0][padding] == 0).all() and (got[4][padding] == 0).all()
     for t in got[1:4]:
         assert (t[0] == 0).all() and (t[2] == 0).all() and torch.isfinite(t[1]).all()
+
+
+@gpu
+def test_ranges_without_groups_are_refused():
+    """They were taken and not looked at."""
+    from moonep_b200.ops import mx
+    bf = dict(device="cuda", dtype=torch.bfloat16)
+    x, d_act, pads = torch.randn(64, 128, **bf), torch.zeros(64, 96, device="cuda"), torch.tensor([[32, 32]], dtype=torch.int32).cuda()
+    wg, wd = torch.randn(128, 96, **bf), mx.quantize(torch.randn(128, 96, **bf))
+    xq, wgu, dg = mx.quantize(x), mx.pack_gate_up(wg, wg), torch.randn(64, 96, **bf)
+    for call in (lambda: mx.matmul(mx.quantize(dg), wd, pads=pads), lambda: mx.gateup_swiglu(xq, wgu, pads=pads),
+                 lambda: mx.gateup_swiglu_bwd(d_act, xq, wgu, pads=pads), lambda: mx.down_dgrad(x, wd, pads=pads),
+                 lambda: mx.gateup_dgrad(dg, dg, wgu, pads=pads), lambda: mx.expert_ffn(x, wgu, None, wd, pads=pads)):
+        with pytest.raises(AssertionError, match="go with cu_seqlens"):
+            call()
