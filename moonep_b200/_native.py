@@ -63,7 +63,7 @@ def lib() -> ctypes.CDLL:
 # reset it to report how many launches a step takes).
 LAUNCHES = 0
 _LAUNCH_PREFIXES = ("mep_launch_", "mep_gemm_launch", "mep_router_", "mep_swiglu_", "mep_sgd_", "mep_ce_",
-                    "mep_mx_quantize", "mep_mx_dequantize", "mep_mx_gemm_launch", "mep_mx_dgrad_launch")
+                    "mep_mx_quantize", "mep_mx_dequantize", "mep_mx_gemm_launch", "mep_mx_dgrad_launch", "mep_mx_sum_parts")
 
 
 def call(name: str, *args):

@@ -54,3 +54,11 @@ def test_gradients_of_groups_that_weight_grads_cannot_take(ends, bad):
         for got, ref in zip(grads[1:], want[1:]):
             assert got[g].isnan().all() if g in bad else torch.equal(got[g], ref)
         start = end
+
+
+def test_every_launch_is_counted():
+    from moonep_b200 import _native as nat
+    from moonep_b200.ops import mx  # noqa: F401
+    launching = {"mep_mx_quantize", "mep_mx_dequantize", "mep_mx_gemm_launch", "mep_mx_dgrad_launch", "mep_mx_sum_parts"}
+    names = [n for n in nat._SIGNATURES if n.startswith("mep_mx_")]
+    assert launching <= set(names) and all(nat._resolve(n)[1] == (n in launching) for n in names)
