@@ -414,8 +414,8 @@ class MoELayer:
 
     def packed_experts(self):
         """Gate and up projections, and the down projection, quantised: those kept by :meth:`pack_experts`, or while
-        training the present weights'."""
-        if self.training:
+        training, and where none are kept, the present weights'."""
+        if self.training or self._packed is None:
             return mx.pack_gate_up(self.w_gate, self.w_up), mx.quantize(self.w_down)
         return self._packed
 

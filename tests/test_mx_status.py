@@ -62,3 +62,23 @@ def test_every_launch_is_counted():
     launching = {"mep_mx_quantize", "mep_mx_dequantize", "mep_mx_gemm_launch", "mep_mx_dgrad_launch", "mep_mx_sum_parts"}
     names = [n for n in nat._SIGNATURES if n.startswith("mep_mx_")]
     assert launching <= set(names) and all(nat._resolve(n)[1] == (n in launching) for n in names)
+
+
+@gpu
+def test_a_layer_that_stops_training():
+    """`training` set to False on a layer that was built for training: its present weights serve, packed in the call until it is
+    told to keep them."""
+    from tests.test_mx_layer import _buffer, _layer
+    buf = _buffer(64, 256, 2, 8)
+    layer = _layer(buf, 128)
+    x = torch.randn(64, 256, generator=_gen(72)).bfloat16().cuda()
+    with torch.no_grad():
+        want = layer(x).clone()
+        layer.training = False
+        assert torch.equal(layer(x), want)
+        layer.w_gate.mul_(-1.5)
+        turned = layer(x).clone()
+        assert not torch.equal(turned, want)
+        layer.pack_experts()
+        assert torch.equal(layer(x), turned)
+    buf.destroy()
