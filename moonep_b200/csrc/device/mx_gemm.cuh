@@ -123,7 +123,8 @@ __host__ __device__ constexpr uint32_t make_instr_desc_mxf4(int M, int N, int sc
          ((uint32_t)(M >> 4) << 24) | ((uint32_t)scale_byte << 29);
 }
 
-// 1 / (1 + e^-x) to a few units in the last place.  (With the exact division gate and up of the decoder's experts, whose
+// 1 / (1 + e^-x).  Its relative error is that of __expf where x is negative, 2^-23 (2 + 1.2 |x|) or so, and far below the
+// bf16 rounding of what it goes into.  (With the exact division gate and up of the decoder's experts, whose
 // epilogue is as long as their reduction, took 134 us, so 86.)
 __device__ __forceinline__ float mx_sigmoid(float x) {
   float r;

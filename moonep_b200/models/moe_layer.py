@@ -336,8 +336,9 @@ class MoELayer:
     ``expert_format="mxfp4"``: the experts' products run over microscaled 4-bit operands (:mod:`..ops.mx`): rows and
     activations are quantised on the way, weights before.  A layer built with ``train=False`` quantises its weights once
     (:meth:`pack_experts`, again after they were changed in place) and streams 17/64 of their bytes; one that trains does
-    it in every forward pass, and its gradients are those of the quantised operands, passed straight through to the bf16
-    weights and rows.  For a group of one rank, whose experts are all local; router and combine are as ever."""
+    it in every forward pass, evaluations among them, and its gradients are those of the quantised operands, passed straight
+    through to the bf16 weights and rows: what such a layer is for is to train what will be served in 4 bits, its step is not
+    faster than bf16's.  For a group of one rank, whose experts are all local; router and combine are as ever."""
 
     def __init__(self, buf: Buffer, Hp: int, pools: Optional[ExpertPools] = None, *, seed: int = 0,
                  router_bias: Optional[torch.Tensor] = None, init_std: float = 0.02,

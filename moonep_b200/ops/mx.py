@@ -4,7 +4,8 @@ for training (``csrc/device/mx_quant.cu``, ``mx_gemm.cuh``).
 An operand is quantised along the reduction in blocks of 32: with ``a = max |x|`` of a block and
 ``e = floor(log2 a) - 2`` (within [-127, 127]) every element becomes ``x / 2^e`` rounded to the nearest of
 0, 0.5, 1, 1.5, 2, 3, 4, 6 (ties to the even code, larger ones to 6) times ``2^e``.  A block with a NaN or an infinity
-is all NaN.  17 bits stand for 32 of bf16, and the tensor cores multiply such operands as they are.
+is all NaN.  17 bytes stand for 64 of bf16 (20 in one matrix, whose scales lie there four times), and the tensor cores
+multiply such operands as they are.
 
 ========================  ==============================  =======================================
 op                        math                            operands
@@ -519,8 +520,8 @@ def expert_ffn(x: torch.Tensor, wg, wu, wd, cu_seqlens: Optional[torch.Tensor] =
     rounded to bf16, as operands of the bf16 products of :mod:`.gemm`, and the results once more.
 
     Rows behind the last group get zeros, in ``y`` and in ``x``'s gradient.  For gradients H must be a multiple of 128
-    and H' of 8, and for the weights' every group's rows a multiple of 64, padding rows of ``x`` being zero (what
-    ``Buffer.dispatch`` gives), but for a group that ends with ``x`` itself; the weight grads of other groups are NaN, and
+    and H' of 8, and for the weights' every group's rows a multiple of 64, padding rows of ``x`` being zero and of ``y``'s
+    gradient finite (what ``Buffer.dispatch`` gives), but for a group that ends with ``x`` itself; the weight grads of other groups are NaN, and
     ``gemm.check_status`` reports them, from the forward pass on, where autograd records it.
     Every call can be captured into a CUDA graph, forward and backward (``utils.graph.GraphedStep``); as with any captured
     ``backward()``, no eager graph of the same leaves may be alive meanwhile."""
