@@ -106,11 +106,11 @@ class MxTensor:
     """A quantised operand of ``shape`` ``[rows, K]`` or ``[G, rows, K]``, blocks along K; ``[2, G, rows, K]`` for a
     gate and an up projection packed together.
 
-    ``codes`` uint8 ``[..., rows, bytes]``: two elements a byte, the earlier one in the low half, rows padded to whole
-    blocks.  ``scales`` uint8 ``[G, row atoms, K atoms, 512]``: E8M0 bytes in atoms of 128 rows x 4 blocks, row ``r``
-    and block ``j`` at ``16 (r % 32) + 4 (r // 32 % 4) + j % 4``.  One matrix has them at four phases, ``[4, row atoms,
-    K atoms, 512]``: the atoms of phase ``s`` begin at row ``32 s`` (row ``r`` is its row ``r - 32 s``), for the products'
-    tiles of token rows, which start at any multiple of 32."""
+    ``codes`` uint8 ``[..., rows, bytes]``: two elements a byte, the earlier one in the low half, rows padded with
+    zeros to whole blocks.  ``scales`` uint8 ``[G, row atoms, K atoms, 512]``: E8M0 bytes in atoms of 128 rows x 4 blocks,
+    row ``r`` and block ``j`` at ``16 (r % 32) + 4 (r // 32 % 4) + j % 4``; those of blocks behind the last are anything but
+    NaN (255).  One matrix has them at four phases, ``[4, row atoms, K atoms, 512]``: the atoms of phase ``s`` begin at row
+    ``32 s`` (row ``r`` is its row ``r - 32 s``), for the products' tiles of token rows, which start at any multiple of 32."""
 
     __slots__ = ("shape", "_codes", "_scales", "_data", "_index", "_mats", "_rows", "_at")
 
@@ -521,8 +521,8 @@ def expert_ffn(x: torch.Tensor, wg, wu, wd, cu_seqlens: Optional[torch.Tensor] =
 
     Rows behind the last group get zeros, in ``y`` and in ``x``'s gradient.  For gradients H must be a multiple of 128
     and H' of 8, and for the weights' every group's rows a multiple of 64, padding rows of ``x`` being zero and of ``y``'s
-    gradient finite (what ``Buffer.dispatch`` gives), but for a group that ends with ``x`` itself; the weight grads of other groups are NaN, and
-    ``gemm.check_status`` reports them, from the forward pass on, where autograd records it.
+    gradient finite (what ``Buffer.dispatch`` gives), but for a group that ends with ``x`` itself; the weight grads of
+    other groups are NaN, and ``gemm.check_status`` reports them, from the forward pass on, where autograd records it.
     Every call can be captured into a CUDA graph, forward and backward (``utils.graph.GraphedStep``); as with any captured
     ``backward()``, no eager graph of the same leaves may be alive meanwhile."""
     assert isinstance(x, torch.Tensor) and x.dim() == 2 and x.dtype == torch.bfloat16, "x must be bf16 [rows, H]"
